@@ -346,6 +346,81 @@ int rptc_next_token(const void *logits, int64_t ld, int64_t rows, int64_t n, int
 int rptc_embed_mailbox(const void *table, const uint64_t *slots, uint32_t *steps_done, int32_t *ids, void *out, int64_t ld_out,
                        int64_t rows, int64_t n, int64_t vocab, int timeout_ms, rptc_stream_t stream);
 
+/* --- prompts of different lengths, caches in 4 bits, log probabilities (no reference counterpart) --- */
+
+/* Causal attention of packed sequences (prompts of different lengths, one behind the other).  Sequence s has the queries starts[s] ..
+ * starts[s + 1] - 1 (rows of q and out) and the keys kv_first[s] .. kv_first[s] + kv_len[s] - 1 (rows of k and v); without kv_first and
+ * kv_len (both NULL) its keys lie where its queries do.  Its last query sees all of its keys, the one in front all but one, and
+ * so on: query i of n sees kv_len - n + 1 + i of them.  out = softmax(scale q k^T) v, scale > 0; zeros where a query sees no key.  Rows of out
+ * that belong to no sequence are left as they are.  The three index arrays lie on the device: a captured call reads those of its replay.
+ * q, out [tokens][heads][d], k, v [kv_tokens][kv_heads][d], fp16 (dtype 0) or bf16 (1), d 64 or 128, heads a multiple of kv_heads; strides in
+ * elements, multiples of 8, tensors 16-byte aligned.  At most 65536 sequences, 2^24 rows and 4096 heads.  Indices outside the tensors are clamped to them and reported
+ * (RPTC_ERR_RANGE, rptc_device_status).  A key or value that is not finite reaches rows that see it, and rows of its own sequence up to 127 in front of it. */
+typedef struct rptc_prompt_attention {
+    const void *q, *k, *v;
+    void *out;
+    const int32_t *starts, *kv_first, *kv_len;
+    int64_t tokens, kv_tokens, sequences;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;      /* strides */
+    int32_t heads, kv_heads, d, dtype;
+    float scale;
+} rptc_prompt_attention;
+int rptc_attn_prompt(const rptc_prompt_attention *a, rptc_stream_t stream);
+
+/* A decoder layer's KV cache for 128-wide heads.
+ * bits = 16: k, v fp16 [rows][max_pos][kv_heads][128]; no scales.
+ * bits = 4: k, v codes uint8 [rows][kv_heads][max_pos][64], k_scales, v_scales fp16 [rows][kv_heads][max_pos][4][2]: for each group of 32
+ * values (scale, minimum), scale = fp16((max - min) / 15) and code = round((x - min) / scale), half to even, at most 15 (0 where the
+ * scale is 0); the code stands for minimum + code * scale.  Value e of group g is nibble e % 4 of the 16-bit word 4 * (e / 4) + g: dims 4 i .. 4 i + 3 of all four groups
+ * are eight bytes.  All 16-byte aligned, contiguous. */
+typedef struct rptc_kv_cache {
+    void *k, *k_scales, *v, *v_scales;
+    int64_t rows, max_pos;
+    int32_t kv_heads, bits;
+} rptc_kv_cache;
+
+/* Output side of a fused qkv layer for any tokens: y = x * scale, or with `transform` s_out * H(x) * scale in blocks of 128 (signs_out NULL = ones),
+ * rounded to fp16; q and k rotated (pairs (i, i + 64)) by the angles of the token's position; k and v into the cache at [slots[t]][pos[t]]
+ * (slots NULL: row t).  x [tokens][ld_x] = [q heads | k heads | v heads] of 128, fp16 or fp32 (x_is_f32: 16-byte aligned, `clear` zeroes it).
+ * out fp16 [tokens][ld_out]: the q heads, and with out_kv the k and v heads behind them; may be x itself (fp16) with the same stride.  angles: fp32
+ * [max_pos][64][2], cosines and sines (rptc_rope_angles).  pos -1: a token of no sequence, for which nothing is written; any other
+ * position or slot outside the cache: nothing is written, RPTC_ERR_RANGE.  No two tokens of a call go to the same place. */
+typedef struct rptc_append {
+    const void *x;
+    int64_t ld_x;
+    const void *signs_out;
+    const int32_t *slots, *pos;
+    const float *angles;
+    void *out;
+    int64_t ld_out, tokens;
+    int32_t heads, x_is_f32, clear, transform, out_kv;
+    float scale;
+    rptc_kv_cache cache;
+} rptc_append;
+int rptc_qkv_append(const rptc_append *a, rptc_stream_t stream);
+
+/* The values that the first count[r] positions of each row of a 4-bit cache stand for: k_out, v_out fp16 [rows][max_pos][kv_heads][128], other
+ * positions are left as they are.  count outside [0, max_pos]: RPTC_ERR_RANGE, nothing of that row is written. */
+int rptc_kv4_values(const rptc_kv_cache *cache, const int32_t *count, void *k_out, void *v_out, rptc_stream_t stream);
+
+/* Single-query attention of each row's q heads over positions 0 .. pos[row] of a 4-bit cache: rptc_attn_decode for it.  q fp16 [rows][ld_q], 16-byte aligned,
+ * ld_q % 8 == 0; out fp16 [rows][ld_out], q heads of 128.  heads a multiple of cache->kv_heads; signs_in as in rptc_attn_decode.
+ * pos -1: a row of no sequence, whose out is zeros; any other position outside the cache: zeros, RPTC_ERR_RANGE.  workspace: 256-byte aligned device
+ * memory of rptc_attn_decode_kv4_workspace_bytes; it holds nothing between calls. */
+int64_t rptc_attn_decode_kv4_workspace_bytes(const rptc_kv_cache *cache, int heads);
+int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *pos, const rptc_kv_cache *cache, void *out, int64_t ld_out, int heads,
+                         float scale, const void *signs_in, void *workspace, int64_t workspace_bytes, rptc_stream_t stream);
+
+/* Log probabilities: lse = log sum_i exp(x_i) over a row of logits, logprob = x_target - lse, entropy = lse - sum_i p_i x_i (natural logarithms), and the
+ * `top` largest entries as top_logprobs, top_ids, the largest first and equal ones by their index.  logits fp16, bf16 or fp32 (dtype 0, 1, 2)
+ * [rows][ld], at least 1 and at most 2^24 of them in a row, aligned to their size; targets int64 [rows] or NULL (then logprob is NULL); entropy may be NULL; 0 <= top <= 32
+ * and top <= n.  -inf is a forbidden token (probability 0).  A row without an allowed token, with NaN or with +inf gives NaN, and ids of some order (the forbidden
+ * by their index).  target -1: no token, logprob 0; any other outside the row: NaN, RPTC_ERR_RANGE.
+ * workspace: 256-byte aligned device memory of rptc_token_logprobs_workspace_bytes (0: none); it holds nothing between calls. */
+int64_t rptc_token_logprobs_workspace_bytes(int64_t rows, int64_t n, int top);
+int rptc_token_logprobs(const void *logits, int dtype, int64_t ld, const int64_t *targets, float *logprob, float *entropy, float *top_logprobs,
+                        int64_t *top_ids, int64_t rows, int64_t n, int top, void *workspace, int64_t workspace_bytes, rptc_stream_t stream);
+
 /* --- the code-A trellis encoder (rptc.py:13-71 `quantize`, diagonal corrections; K = 2 bits per weight) ---
  * For each of `rows` sample rows (fp32 [rows][ld_samples], n used) the symbols in 0..3 (int32 [rows][ld_sym]) whose
  * shift-register walk from state 0 minimises sum_i pos_weight[i] * (samples[i] - alphabet[state_i])^2, and that
