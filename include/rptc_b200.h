@@ -354,7 +354,7 @@ int rptc_embed_mailbox(const void *table, const uint64_t *slots, uint32_t *steps
  * so on: query i of n sees kv_len - n + 1 + i of them.  out = softmax(scale q k^T) v, scale > 0; zeros where a query sees no key.  Rows of out
  * that belong to no sequence are left as they are.  The three index arrays lie on the device: a captured call reads those of its replay.
  * q, out [tokens][heads][d], k, v [kv_tokens][kv_heads][d], fp16 (dtype 0) or bf16 (1), d 64 or 128, heads a multiple of kv_heads; strides in
- * elements, multiples of 8, tensors 16-byte aligned.  At most 65536 sequences, 2^24 rows and 4096 heads.  Indices outside the tensors are clamped to them and reported
+ * elements, multiples of 8, tensors 16-byte aligned.  At most 65535 sequences, 2^24 rows and 4096 heads.  Indices outside the tensors are clamped to them and reported
  * (RPTC_ERR_RANGE, rptc_device_status).  A key or value that is not finite reaches rows that see it, and rows of its own sequence up to 127 in front of it. */
 typedef struct rptc_prompt_attention {
     const void *q, *k, *v;
@@ -384,7 +384,8 @@ typedef struct rptc_kv_cache {
  * (slots NULL: row t).  x [tokens][ld_x] = [q heads | k heads | v heads] of 128, fp16 or fp32 (x_is_f32: 16-byte aligned, `clear` zeroes it).
  * out fp16 [tokens][ld_out]: the q heads, and with out_kv the k and v heads behind them; may be x itself (fp16) with the same stride.  angles: fp32
  * [max_pos][64][2], cosines and sines (rptc_rope_angles).  pos -1: a token of no sequence, for which nothing is written; any other
- * position or slot outside the cache: nothing is written, RPTC_ERR_RANGE.  No two tokens of a call go to the same place. */
+ * position or slot outside the cache: nothing is written, RPTC_ERR_RANGE.  No two tokens of a call go to the same place.  Values that are not finite have no
+ * code: what a 4-bit cache holds for their group of 32 then means nothing. */
 typedef struct rptc_append {
     const void *x;
     int64_t ld_x;

@@ -77,6 +77,27 @@ class Packed(ctypes.Structure):
                 ("n", ctypes.c_int64), ("banks", ctypes.c_int32), ("bank_blocks", ctypes.c_int32), ("L", ctypes.c_int32)]
 
 
+class KVCache(ctypes.Structure):
+    """Mirror of `rptc_kv_cache`."""
+    _fields_ = [("k", ctypes.c_void_p), ("k_scales", ctypes.c_void_p), ("v", ctypes.c_void_p), ("v_scales", ctypes.c_void_p),
+                ("rows", ctypes.c_int64), ("max_pos", ctypes.c_int64), ("kv_heads", ctypes.c_int32), ("bits", ctypes.c_int32)]
+
+
+class Append(ctypes.Structure):
+    """Mirror of `rptc_append`."""
+    _fields_ = [("x", ctypes.c_void_p), ("ld_x", ctypes.c_int64), ("signs_out", ctypes.c_void_p), ("slots", ctypes.c_void_p), ("pos", ctypes.c_void_p),
+                ("angles", ctypes.c_void_p), ("out", ctypes.c_void_p), ("ld_out", ctypes.c_int64), ("tokens", ctypes.c_int64),
+                ("heads", ctypes.c_int32), ("x_is_f32", ctypes.c_int32), ("clear", ctypes.c_int32), ("transform", ctypes.c_int32),
+                ("out_kv", ctypes.c_int32), ("scale", ctypes.c_float), ("cache", KVCache)]
+
+
+class PromptAttention(ctypes.Structure):
+    """Mirror of `rptc_prompt_attention`."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "out", "starts", "kv_first", "kv_len")] + [
+        (n, ctypes.c_int64) for n in ("tokens", "kv_tokens", "sequences", "q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "out_row",
+                                      "out_head")] + [(n, ctypes.c_int32) for n in ("heads", "kv_heads", "d", "dtype")] + [("scale", ctypes.c_float)]
+
+
 _lib = None
 
 _SIGS = {
@@ -187,6 +208,17 @@ _SIGS = {
     "rptc_rope_cache_prompt": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
                                               ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_float,
                                               ctypes.c_void_p]),
+    "rptc_attn_prompt": (ctypes.c_int, [ctypes.POINTER(PromptAttention), ctypes.c_void_p]),
+    "rptc_qkv_append": (ctypes.c_int, [ctypes.POINTER(Append), ctypes.c_void_p]),
+    "rptc_kv4_values": (ctypes.c_int, [ctypes.POINTER(KVCache), ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "rptc_attn_decode_kv4_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(KVCache), ctypes.c_int]),
+    "rptc_attn_decode_kv4": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.POINTER(KVCache), ctypes.c_void_p,
+                                            ctypes.c_int64, ctypes.c_int, ctypes.c_float, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64,
+                                            ctypes.c_void_p]),
+    "rptc_token_logprobs_workspace_bytes": (ctypes.c_int64, [ctypes.c_int64, ctypes.c_int64, ctypes.c_int]),
+    "rptc_token_logprobs": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                                           ctypes.c_int64, ctypes.c_void_p]),
     "rptc_next_token": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
                                        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     "rptc_embed_mailbox": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,

@@ -354,6 +354,193 @@ def next_token(logits: torch.Tensor, next_ids: torch.Tensor, ids: torch.Tensor |
          ptr(steps_done))
 
 
+# ---- prompts of different lengths, caches in 4 bits, log probabilities ---------------------------------------------------
+
+def _on(device: torch.device, name: str, t: torch.Tensor, dtype, shape: tuple | None = None) -> None:
+    """A tensor that a kernel reads as it is: dtype (or one of several), device, and contiguous in `shape` (None: any)."""
+    if t.device != device or device.type != "cuda":
+        raise RuntimeError(f"{name} must be a CUDA tensor on {device}")
+    if t.dtype != dtype if isinstance(dtype, torch.dtype) else t.dtype not in dtype:
+        raise RuntimeError(f"{name} must have dtype {dtype}, got {t.dtype}")
+    if shape is not None and (tuple(t.shape) != shape or not t.is_contiguous()):
+        raise RuntimeError(f"{name} must be contiguous {list(shape)}, got {list(t.shape)}")
+
+
+def kv4_cache(rows: int, max_pos: int, kv_heads: int, device="cuda") -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """A layer's KV cache in 4 bits for 128-wide heads, empty: codes of k, (scale, minimum) of its groups of 32 values, the same
+    for v (rptc_kv_cache); 160 bytes per position and kv head, where fp16 takes 512."""
+    codes = lambda: torch.zeros((rows, kv_heads, max_pos, 64), dtype=torch.uint8, device=device)
+    scales = lambda: torch.zeros((rows, kv_heads, max_pos, 4, 2), dtype=torch.float16, device=device)
+    return codes(), scales(), codes(), scales()
+
+
+def _kv_cache(cache, device: torch.device) -> _lib.KVCache:
+    """(k, v) in fp16 [rows, max_pos, kv_heads, 128], or the four tensors of `kv4_cache`."""
+    if len(cache) == 2:
+        if cache[0].dim() != 4 or cache[0].shape[3] != 128:
+            raise RuntimeError("an fp16 cache must be [rows, max_pos, kv_heads, 128]")
+        for name, t in zip(("k cache", "v cache"), cache):
+            _on(device, name, t, torch.float16, tuple(cache[0].shape))
+        rows, max_pos, kv_heads, _ = cache[0].shape
+        return _lib.KVCache(ptr(cache[0]), None, ptr(cache[1]), None, rows, max_pos, kv_heads, 16)
+    if len(cache) != 4 or cache[0].dim() != 4:
+        raise RuntimeError("a cache is (k, v) in fp16, or (k codes, k scales, v codes, v scales)")
+    rows, kv_heads, max_pos, _ = cache[0].shape
+    for i, name in enumerate(("k codes", "k scales", "v codes", "v scales")):
+        _on(device, name, cache[i], torch.float16 if i % 2 else torch.uint8, (rows, kv_heads, max_pos) + ((4, 2) if i % 2 else (64,)))
+    return _lib.KVCache(*[ptr(t) for t in cache], rows, max_pos, kv_heads, 4)
+
+
+def _rows_of(name: str, t: torch.Tensor, device: torch.device, dtype, rows: int, width: int) -> None:
+    _on(device, name, t, dtype)
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < width or (t.stride(1) != 1 and t.shape[1] > 1):
+        raise RuntimeError(f"{name} must be [{rows}, >= {width}] with unit column stride, got {list(t.shape)}")
+
+
+def qkv_append(x: torch.Tensor, pos: torch.Tensor, angles: torch.Tensor, cache, heads: int, kv_heads: int, slots: torch.Tensor | None = None,
+               signs_out: torch.Tensor | None = None, scale: float = 1.0, transform: bool = False, out: torch.Tensor | None = None,
+               clear: bool = False) -> torch.Tensor:
+    """Output side of a fused qkv layer for tokens of any sequences (rptc_qkv_append): x fp16 or fp32 [tokens, (heads + 2 kv_heads) * 128],
+    y = x * scale (`transform`: s_out * H(x) * scale in blocks of 128); q and k rotated by `angles` (fp32 [>= max_pos, 64, 2]) of the token's
+    position, k and v appended to `cache` (fp16 pair or `kv4_cache`) at [slots[t], pos[t]] (slots None: row t; pos -1: a token of no
+    sequence, nothing is written).  Returns fp16 [tokens, (heads + 2 kv_heads) * 128] with q, k and v as finished; an `out` of fewer columns
+    takes q alone.  `clear` zeroes an fp32 x.  `out` may be x itself; otherwise the two do not overlap."""
+    device, width = x.device, (heads + 2 * kv_heads) * 128
+    c = _kv_cache(cache, device)
+    if heads <= 0 or kv_heads != c.kv_heads:
+        raise RuntimeError(f"the cache has {c.kv_heads} kv heads, got heads {heads}, kv_heads {kv_heads}")
+    if x.dim() != 2:
+        raise RuntimeError("x must be [tokens, (heads + 2 kv_heads) * 128]")
+    tokens = x.shape[0]
+    _rows_of("x", x, device, (torch.float16, torch.float32), tokens, width)
+    _on(device, "pos", pos, torch.int32, (tokens,))
+    if slots is not None:
+        _on(device, "slots", slots, torch.int32, (tokens,))
+    if angles.dim() != 3 or angles.shape[0] < c.max_pos:
+        raise RuntimeError(f"angles must be [>= {c.max_pos}, 64, 2]")
+    _on(device, "angles", angles, torch.float32, (angles.shape[0], 64, 2))
+    if signs_out is not None:
+        _on(device, "signs_out", signs_out, torch.float16, (width,))
+    if out is None:
+        out = torch.empty((tokens, width), dtype=torch.float16, device=device)
+    _rows_of("out", out, device, torch.float16, tokens, heads * 128)
+    if tokens == 0:
+        return out
+    a = _lib.Append(ptr(x), _ld(x, width), ptr(signs_out), ptr(slots), ptr(pos), ptr(angles), ptr(out), _ld(out, out.shape[1]), tokens, heads,
+                    int(x.dtype == torch.float32), int(clear), int(transform), int(out.shape[1] >= width), scale, c)
+    call("rptc_qkv_append", device, ctypes.byref(a))
+    return out
+
+
+def kv4_values(cache, count: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values that the first count[r] (int32 [rows]) positions of row r of a 4-bit cache stand for, fp16 k and v [rows, max_pos, kv_heads,
+    128]; other positions are left as they are (rptc_kv4_values)."""
+    device = cache[0].device
+    c = _kv_cache(cache, device)
+    if c.bits != 4:
+        raise RuntimeError("the cache must be one of kv4_cache")
+    _on(device, "count", count, torch.int32, (c.rows,))
+    shape = (c.rows, c.max_pos, c.kv_heads, 128)
+    k, v = out if out is not None else (torch.empty(shape, dtype=torch.float16, device=device) for _ in range(2))
+    for t in (k, v):
+        _on(device, "out", t, torch.float16, shape)
+    call("rptc_kv4_values", device, ctypes.byref(c), ptr(count), ptr(k), ptr(v))
+    return k, v
+
+
+def attn_decode_kv4(q: torch.Tensor, pos: torch.Tensor, cache, heads: int, out: torch.Tensor | None = None, scale: float | None = None,
+                    signs_in: torch.Tensor | None = None) -> torch.Tensor:
+    """Single-query attention over positions 0 .. pos[r] of row r of a 4-bit cache (rptc_attn_decode_kv4): q fp16 [rows, >= heads * 128] ->
+    fp16 [rows, heads * 128].  pos -1: a row of no sequence, zeros.  signs_in: each head's output also goes through the 128-wide input
+    transform of the output projection."""
+    device = cache[0].device
+    c = _kv_cache(cache, device)
+    _rows_of("q", q, device, torch.float16, c.rows, heads * 128)
+    _on(device, "pos", pos, torch.int32, (c.rows,))
+    if out is None:
+        out = torch.empty((c.rows, heads * 128), dtype=torch.float16, device=device)
+    _rows_of("out", out, device, torch.float16, c.rows, heads * 128)
+    if signs_in is not None:
+        _on(device, "signs_in", signs_in, torch.float16, (heads * 128,))
+    if c.rows == 0:
+        return out
+    need = lib().rptc_attn_decode_kv4_workspace_bytes(ctypes.byref(c), heads)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    call("rptc_attn_decode_kv4", device, ptr(q), _ld(q, q.shape[1]), ptr(pos), ctypes.byref(c), ptr(out), _ld(out, out.shape[1]), heads,
+         128 ** -0.5 if scale is None else scale, ptr(signs_in), ptr(ws), need)
+    return out
+
+
+def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, kv_first: torch.Tensor | None = None,
+                kv_len: torch.Tensor | None = None, out: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
+    """Causal attention of packed prompts of different lengths (rptc_attn_prompt): q [tokens, heads, d], k and v [kv_tokens, kv_heads, d], fp16 or
+    bf16, d 64 or 128, unit stride along d -> out [tokens, heads, d].  Sequence s has the queries starts[s] .. starts[s + 1] - 1 (int32
+    [sequences + 1]) and, for prompts that continue a cached context, the keys kv_first[s] .. kv_first[s] + kv_len[s] - 1 (int32 [sequences]; None:
+    its keys lie where its queries do); its last query sees all of them.  Rows of `out` behind the last sequence are left as they are."""
+    device = q.device
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        _on(device, name, t, (torch.float16, torch.bfloat16))
+        if t.dim() != 3 or t.dtype != q.dtype or t.shape[2] != q.shape[2] or t.stride(2) != 1:
+            raise RuntimeError(f"{name} must be [rows, heads, d] of q's dtype and d with unit stride along d")
+    if k.shape != v.shape:
+        raise RuntimeError("k and v must have the same shape")
+    tokens, heads, d = q.shape
+    if starts.dim() != 1 or starts.shape[0] < 1:
+        raise RuntimeError("starts must be int32 [sequences + 1]")
+    n = starts.shape[0] - 1
+    _on(device, "starts", starts, torch.int32, (n + 1,))
+    if (kv_first is None) != (kv_len is None):
+        raise RuntimeError("kv_first and kv_len go together")
+    for name, t in (("kv_first", kv_first), ("kv_len", kv_len)):
+        if t is not None:
+            _on(device, name, t, torch.int32, (n,))
+    if out is None:
+        out = torch.empty((tokens, heads, d), dtype=q.dtype, device=device)
+    _on(device, "out", out, q.dtype)
+    if out.shape != q.shape or out.stride(2) != 1:
+        raise RuntimeError("out must have q's shape and unit stride along d")
+    if tokens == 0 or n == 0:
+        return out
+    if k.shape[0] == 0:
+        raise RuntimeError("k and v must have at least one row")
+
+    def strides(t):      # of an axis of one element any
+        return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * d, t.stride(1) if t.shape[1] > 1 else d)
+
+    a = _lib.PromptAttention(ptr(q), ptr(k), ptr(v), ptr(out), ptr(starts), ptr(kv_first), ptr(kv_len), tokens, k.shape[0], n, *strides(q), *strides(k),
+                             *strides(v), *strides(out), heads, k.shape[1], d, int(q.dtype == torch.bfloat16), d ** -0.5 if scale is None else scale)
+    call("rptc_attn_prompt", device, ctypes.byref(a))
+    return out
+
+
+_LOGIT_TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, top: int = 0):
+    """Log probabilities of given tokens, with entropy and alternatives (rptc_token_logprobs): logits fp16, bf16 or fp32 [rows, n], targets int64
+    [rows] (-1: no token, 0) -> (logprob fp32 [rows] or None, entropy fp32 [rows], top_logprobs fp32 [rows, top], top_ids int64 [rows, top], the
+    largest first, equal ones by their index).  -inf is a forbidden token."""
+    device = logits.device
+    _on(device, "logits", logits, tuple(_LOGIT_TYPES))
+    if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise RuntimeError("logits must be [rows, n] with unit column stride")
+    rows, n = logits.shape
+    if not 0 <= top <= min(32, n):
+        raise RuntimeError(f"top must be between 0 and {min(32, n)}, got {top}")
+    if targets is not None:
+        _on(device, "targets", targets, torch.int64, (rows,))
+    f32 = dict(dtype=torch.float32, device=device)
+    logprob, entropy = None if targets is None else torch.empty(rows, **f32), torch.empty(rows, **f32)
+    best, ids = torch.empty((rows, top), **f32), torch.empty((rows, top), dtype=torch.int64, device=device)
+    if rows == 0:
+        return logprob, entropy, best, ids
+    need = lib().rptc_token_logprobs_workspace_bytes(rows, n, top)
+    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    call("rptc_token_logprobs", device, ptr(logits), _LOGIT_TYPES[logits.dtype], _ld(logits, n), ptr(targets), ptr(logprob), ptr(entropy),
+         ptr(best) if top else None, ptr(ids) if top else None, rows, n, top, ptr(ws), need)
+    return logprob, entropy, best, ids
+
+
 def viterbi_encode(alphabet: torch.Tensor, pos_weight: torch.Tensor, samples: torch.Tensor, workspace_limit: int = 12 << 30):
     """Code-A trellis encoder on the GPU (rptc_viterbi_encode): samples fp32 [rows, n] -> (symbols int32 [rows, n],
     loss fp32 [rows])."""
