@@ -355,7 +355,7 @@ int rptc_embed_mailbox(const void *table, const uint64_t *slots, uint32_t *steps
  * that belong to no sequence are left as they are.  The three index arrays lie on the device: a captured call reads those of its replay.
  * q, out [tokens][heads][d], k, v [kv_tokens][kv_heads][d], fp16 (dtype 0) or bf16 (1), d 64 or 128, heads a multiple of kv_heads; strides in
  * elements, multiples of 8, tensors 16-byte aligned.  At most 65535 sequences, 2^24 rows and 4096 heads.  Indices outside the tensors are clamped to them and reported
- * (RPTC_ERR_RANGE, rptc_device_status).  A key or value that is not finite reaches rows that see it, and rows of its own sequence up to 127 in front of it. */
+ * (RPTC_ERR_RANGE, rptc_device_status).  A key or value that is not finite reaches rows that see it, and rows of its own sequence up to 255 in front of it. */
 typedef struct rptc_prompt_attention {
     const void *q, *k, *v;
     void *out;

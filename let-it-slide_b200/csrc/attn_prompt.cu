@@ -1,33 +1,49 @@
-// Causal attention of packed prompts.  No reference counterpart.
+// Causal attention of packed prompts on the sm_100a tensor cores.  No reference counterpart.
+//
+//   o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale q_i . k_j - m_i)   over the keys that query i sees
+//
+// An item is 256 query rows of one kv head's queries, in two halves of 128: `pack` heads of a group (the largest power of two that divides it) x
+// 256 / pack tokens, so that grouped heads of a short prompt fill the tensor core's 128 rows and share the keys' tiles.  A CTA takes items one after
+// the other.  For each tile of 128 keys and each half:
+//   S = Q K^T            tcgen05.mma from shared memory into tensor memory (fp32)
+//   P = exp2(S - m)      a softmax thread owns a row: it reads its 128 scores, keeps the running maximum m and sum l in registers, and puts P back over S in
+//                        16 bits (the one rounding besides the result's: the tensor core multiplies 16-bit operands; l adds the weights up before it)
+//   O += P V             tcgen05.mma with P in tensor memory, V in shared memory as it lies (N-major), O in tensor memory (fp32)
+// The two halves alternate: the tensor core works on one while the other's softmax runs.  m follows the true maximum with a slack of 2^8: only a larger step
+// rescales O and l (by the thread that owns the row; the scores' barrier says that the product before has been added).  exp2 of differences up to 8 stays far inside fp16 and fp32.
+// Warps 0-3 and 4-7: softmax and output of the halves; 8: MMA issue; 9: TMA loads (ring of key and value tiles); 10: the list of items.
+// Masks are applied to tiles that reach beyond a half's first row only.  Value rows behind the last key are zeroed in shared memory: a weight of 0 times whatever
+// lies there has to be 0.
+// Items go to CTAs longest first, there and back again (the longest of a round meets the shortest of the next): the order is worked out from
+// `starts` on the device, by counting items of at least a number of tiles.
 #include <cuda_bf16.h>
 
-#include "common.cuh"
+#include "tc_ptx.cuh"
 
 namespace rptc {
 
+constexpr int kPromptThreads = 352, kPromptMmaWarp = 8, kPromptLoadWarp = 9, kPromptListWarp = 10;
+constexpr int kPromptReaders = 10;                   // warps that take items off the list
+constexpr uint32_t kPromptPanel = 128 * 128;         // 128 rows of 64 values
+constexpr int kTileKeys = 128;
+constexpr float kSlack = 8.f;                        // log2 of how far a score may pass the maximum that its row's weights refer to
+
 struct PromptParams {
-    const uint16_t *q, *k, *v;
     uint16_t *out;
     const int32_t *starts, *kv_first, *kv_len;
-    int64_t tokens, kv_tokens;
-    int64_t q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head;
-    int32_t sequences, group, d;
-    float scale;                     // includes log2(e)
+    int64_t tokens, kv_tokens, out_row, out_head;
+    int32_t sequences, group, pack, kv_heads;
+    float scale;                                     // includes log2(e)
     unsigned int *status;
 };
-
-template <bool BF16>
-__device__ __forceinline__ float load16(const uint16_t *p) {
-    return BF16 ? __bfloat162float(__ushort_as_bfloat16(*p)) : __half2float(__ushort_as_half(*p));
-}
 
 // What a sequence has: queries q0 .. q0 + n - 1, keys k0 .. k0 + m - 1, clamped to the tensors.
 struct Sequence {
     int q0, n, k0, m;
 };
 __device__ __forceinline__ Sequence sequence(const PromptParams &p, int s) {
-    const int a = __ldg(p.starts + s), b = __ldg(p.starts + s + 1);
-    const int k0 = p.kv_first ? __ldg(p.kv_first + s) : a, m = p.kv_len ? __ldg(p.kv_len + s) : b - a;
+    const int a = p.starts[s], b = p.starts[s + 1];
+    const int k0 = p.kv_first ? p.kv_first[s] : a, m = p.kv_len ? p.kv_len[s] : b - a;
     Sequence r;
     r.q0 = min(max(a, 0), (int)p.tokens);
     r.n = min(max(b, r.q0), (int)p.tokens) - r.q0;
@@ -36,37 +52,415 @@ __device__ __forceinline__ Sequence sequence(const PromptParams &p, int s) {
     if (r.q0 != a || r.n != b - a || r.k0 != k0 || r.m != m) atomicExch(p.status, kStatusPosition);
     return r;
 }
+// How many items of a sequence take at least c tiles of keys (its last ones; all take one).
+__device__ __forceinline__ int items_of(const Sequence &s, int tokens_per_item, int c) {
+    const int all = (s.n + tokens_per_item - 1) / tokens_per_item;
+    if (c <= 1 || all == 0) return all;
+    const int reach = kTileKeys * (c - 1);           // an item takes c tiles when its last query sees more keys than these
+    if (s.m <= reach) return 0;
+    const int first = max(0, reach - (s.m - s.n)) / tokens_per_item;
+    return all - min(first, all - 1);
+}
 
-// A warp per query and head.
-template <bool BF16>
-__global__ void __launch_bounds__(128) attn_prompt_kernel(const PromptParams p) {
-    pdl_allow_next_grid();
-    pdl_wait_prior_grids();
-    const int s = blockIdx.z, head = blockIdx.y, lane = threadIdx.x & 31;
-    const Sequence seq = sequence(p, s);
-    const int per = p.d / 32;
-    for (int i = blockIdx.x * 4 + (threadIdx.x >> 5); i < seq.n; i += gridDim.x * 4) {
-        float q[4], acc[4] = {}, m = -INFINITY, l = 0.f;
-        const uint16_t *qp = p.q + (int64_t)(seq.q0 + i) * p.q_row + head * p.q_head + lane;
-        for (int e = 0; e < 4; ++e) q[e] = e < per ? load16<BF16>(qp + 32 * e) * p.scale : 0.f;
-        const int seen = seq.m - seq.n + 1 + i;
-        for (int j = 0; j < seen; ++j) {
-            const uint16_t *kp = p.k + (int64_t)(seq.k0 + j) * p.k_row + (head / p.group) * p.k_head + lane;
-            const uint16_t *vp = p.v + (int64_t)(seq.k0 + j) * p.v_row + (head / p.group) * p.v_head + lane;
-            float x = 0.f;
-            for (int e = 0; e < per; ++e) x = fmaf(q[e], load16<BF16>(kp + 32 * e), x);
-            for (int o = 16; o > 0; o >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, o);
-            const float mn = fmaxf(m, x), f = exp2f(m - mn), w = exp2f(x - mn);
-            m = mn;
-            l = l * f + w;
-            for (int e = 0; e < per; ++e) acc[e] = fmaf(w, load16<BF16>(vp + 32 * e), acc[e] * f);
+struct PromptItem {
+    int32_t go, head, kv_head, token, tokens, k0, keys, seen, tiles0, tiles1;      // seen: index of the last key that the item's first query sees
+    int32_t pad[2];
+};
+
+// Item number `index` of all, by one warp.
+__device__ __forceinline__ PromptItem find_item(const PromptParams &p, int64_t index, int most, int lane) {
+    const int per_item = 256 / p.pack, groups = p.kv_heads * (p.group / p.pack);
+    const int rank = (int)(index / groups), heads = (int)(index - (int64_t)rank * groups);
+    auto count = [&](int c) {
+        int n = 0;
+        for (int s = lane; s < p.sequences; s += 32) n += items_of(sequence(p, s), per_item, c);
+        return __reduce_add_sync(0xFFFFFFFFu, n);
+    };
+    int lo = 1, hi = most;                           // the largest c of which there are more than `rank`
+    while (lo < hi) {
+        const int mid = lo + (hi - lo + 1) / 2;
+        if (count(mid) > rank) lo = mid;
+        else hi = mid - 1;
+    }
+    int left = rank - count(lo + 1);
+    PromptItem it = {};
+    for (int s0 = 0; s0 < p.sequences; s0 += 32) {
+        Sequence q = {0, 0, 0, 0};
+        if (s0 + lane < p.sequences) q = sequence(p, s0 + lane);
+        const int from = items_of(q, per_item, lo), mine = from - items_of(q, per_item, lo + 1);
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+            if (lane >= o) upto += v;
         }
-        uint16_t *op = p.out + (int64_t)(seq.q0 + i) * p.out_row + head * p.out_head + lane;
-        for (int e = 0; e < per; ++e) {
-            const float o = seen > 0 ? acc[e] / l : 0.f;
-            op[32 * e] = BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(o)) : __half_as_ushort(__float2half_rn(o));
+        const unsigned hit = __ballot_sync(0xFFFFFFFFu, left < upto);
+        if (hit) {
+            const int all = (q.n + per_item - 1) / per_item, j = all - from + left - (upto - mine);
+            it.go = 1;
+            it.kv_head = heads / (p.group / p.pack);
+            it.head = it.kv_head * p.group + (heads % (p.group / p.pack)) * p.pack;
+            it.token = q.q0 + j * per_item;
+            it.tokens = min(per_item, q.n - j * per_item);
+            it.k0 = q.k0, it.keys = q.m;
+            it.seen = q.m - q.n + j * per_item;
+            const int last0 = it.seen + min(it.tokens, per_item / 2), last1 = it.seen + it.tokens;      // keys that a half's last query sees
+            it.tiles0 = max(0, (last0 + kTileKeys - 1) / kTileKeys);
+            it.tiles1 = it.tokens > per_item / 2 ? max(0, (last1 + kTileKeys - 1) / kTileKeys) : 0;
+            const int from_lane = __ffs(hit) - 1;
+            int *w = reinterpret_cast<int *>(&it);
+#pragma unroll
+            for (int i = 0; i < 10; ++i) w[i] = __shfl_sync(0xFFFFFFFFu, w[i], from_lane);
+            return it;
+        }
+        left -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    return it;                                       // not reached: the index is below the number of items
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+    uint32_t r;
+    if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const PromptParams p, const __grid_constant__ CUtensorMap q_map,
+                                                                       const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    constexpr uint32_t kTile = DP * kPromptPanel;    // bytes of a half's queries, of a tile of keys or values
+    constexpr int kStages = DP == 2 ? 5 : 8;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0);
+    const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    const uint32_t bars = base, q_addr = base + 1024u, ring = q_addr + 2 * kTile;
+    const uint32_t q_full = bars, q_empty = bars + 8, full = bars + 16, empty = full + 8 * kStages, s_full = empty + 8 * kStages, p_full = s_full + 16,
+                   o_full = p_full + 16, item_full = o_full + 16, item_empty = item_full + 16, tmem_slot = item_empty + 16, items = bars + 256;
+    if (tid == 0) {
+        mbar_init(q_full, 1), mbar_init(q_empty, 1);
+        for (int i = 0; i < kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 4), mbar_init(o_full + 8 * i, 1);
+            mbar_init(item_full + 8 * i, 1), mbar_init(item_empty + 8 * i, kPromptReaders);
+        }
+        mbar_fence_init();
+    }
+    if (warp == kPromptMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "n"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    pdl_allow_next_grid();
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, lds32(tmem_slot), 0);
+    const int rows_per_token = p.pack, half_tokens = 128 / rows_per_token;
+    bool ok = true;
+
+    // the next item off the list; false at its end
+    RingPos list = {0, 0u};
+    auto next_item = [&](PromptItem &it) {
+        ok = ok && mbar_wait(item_full + 8 * list.s, list.phase, p.status);
+        if (!__all_sync(0xFFFFFFFFu, ok)) {
+            ok = false;
+            return false;
+        }
+        const uint32_t at = items + 64u * list.s;
+        const uint4 a = lds128(at), b = lds128(at + 16u), c = lds128(at + 32u);
+        it.go = (int)a.x, it.head = (int)a.y, it.kv_head = (int)a.z, it.token = (int)a.w;
+        it.tokens = (int)b.x, it.k0 = (int)b.y, it.keys = (int)b.z, it.seen = (int)b.w;
+        it.tiles0 = (int)c.x, it.tiles1 = (int)c.y;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(item_empty + 8 * list.s);
+        list.advance(2);
+        return it.go != 0;
+    };
+
+    PromptItem it;
+    if (warp < 8) {
+        // ================= softmax and output of one half: a thread owns a row =================
+        const int half = warp >> 2, row = (warp & 3) * 32 + lane, my_token = half * half_tokens + row / rows_per_token, my_head = row % rows_per_token;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_tmem = tmem + 128u * half + lanes, o_tmem = tmem + 256u + 128u * half + lanes;
+        const uint32_t my_s = s_full + 8 * half, my_p = p_full + 8 * half;
+        uint32_t phase = 0u, o_phase = 0u;
+        while (next_item(it)) {
+            const int tiles = half ? it.tiles1 : it.tiles0, first_seen = it.seen + half * half_tokens;
+            const int last = min(it.seen + my_token, it.keys - 1);                  // the last key that this row sees
+            float m = -INFINITY, l = 0.f;                                           // m: in units of the scores
+            for (int i = 0; i < tiles && ok; ++i) {
+                ok = mbar_wait(my_s, phase, p.status);
+                phase ^= 1u;
+                if (!__all_sync(0xFFFFFFFFu, ok)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                uint32_t s[128];
+                tmem_load64(s_tmem, *reinterpret_cast<uint32_t(*)[64]>(s));
+                tmem_load64(s_tmem + 64u, *reinterpret_cast<uint32_t(*)[64]>(s + 64));
+                if (i * kTileKeys + kTileKeys - 1 > first_seen || i * kTileKeys + kTileKeys > it.keys) {
+                    const int lim = last - i * kTileKeys;
+#pragma unroll
+                    for (int c = 0; c < 128; ++c) s[c] = c <= lim ? s[c] : 0xFF800000u;
+                }
+                float mx[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(s[c]);
+#pragma unroll
+                for (int c = 4; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                if (i == 0) {
+                    m = top == -INFINITY ? 0.f : top;                               // a row that sees nothing has weights of 0
+                } else {
+                    const bool grows = (top - m) * p.scale > kSlack;
+                    if (__any_sync(0xFFFFFFFFu, grows)) {
+                        const float f = grows ? exp2_fast((m - top) * p.scale) : 1.f;
+                        l *= f;
+                        m = grows ? top : m;
+#pragma unroll 1
+                        for (int c = 0; c < DP * 64; c += 32) {
+                            uint32_t o[32];
+                            tmem_load32(o_tmem + (uint32_t)c, o);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                            tmem_store32_begin(o_tmem + (uint32_t)c, o);
+                        }
+                    }
+                }
+                const float shift = -m * p.scale;
+                float sum[2] = {0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < 128; c += 64) {
+                    uint32_t w[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const float a = exp2_fast(fmaf(__uint_as_float(s[c + 2 * e]), p.scale, shift)), b = exp2_fast(fmaf(__uint_as_float(s[c + 2 * e + 1]), p.scale, shift));
+                        sum[0] += a, sum[1] += b;
+                        w[e] = pack16<BF16>(a, b);
+                    }
+                    tmem_store32_begin(s_tmem + (uint32_t)(c / 2), w);
+                }
+                l += sum[0] + sum[1];
+                tmem_store_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(my_p);
+            }
+            if (tiles > 0) {                                                        // the last product has been added
+                ok = ok && mbar_wait(o_full + 8 * half, o_phase, p.status);
+                o_phase ^= 1u;
+                if (!__all_sync(0xFFFFFFFFu, ok)) {
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+            }
+            const bool there = my_token < it.tokens;
+            const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;               // NaN stays
+            uint16_t *out = p.out + (int64_t)(it.token + my_token) * p.out_row + (int64_t)(it.head + my_head) * p.out_head;
+#pragma unroll 1
+            for (int c = 0; c < DP * 64; c += 32) {
+                uint32_t o[32];
+                if (tiles > 0) {
+                    tmem_load32(o_tmem + (uint32_t)c, o);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;
+                }
+                if (!there) continue;
+#pragma unroll
+                for (int e = 0; e < 32; e += 8) {
+                    uint32_t w[4];
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const float a = __uint_as_float(o[e + 2 * q]) * inv, b = __uint_as_float(o[e + 2 * q + 1]) * inv;
+                        w[q] = inv == 0.f ? 0u : pack16<BF16>(a, b);
+                    }
+                    *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            }
+            tc_fence_before();
+        }
+    } else if (warp == kPromptMmaWarp) {
+        // ================= MMA issue: the whole warp waits, one lane issues =================
+        RingPos pos = {0, 0u};
+        uint32_t q_phase = 0u, p_phase = 0u;                                        // p_phase: bit h for half h
+        const uint32_t idesc_s = instr_desc(kTileKeys) | (BF16 ? kInstrBf16 : 0u), idesc_o = instr_desc(DP * 64) | (BF16 ? kInstrBf16 : 0u) | kInstrBMajorN;
+        while (next_item(it)) {
+            const int tiles = max(it.tiles0, it.tiles1);
+            if (tiles == 0) continue;
+            auto scores = [&](int h, uint32_t k_addr) {                             // by the elected lane
+#pragma unroll
+                for (uint32_t c = 0; c < 4 * DP; ++c) {
+                    const uint32_t off = (c >> 2) * kPromptPanel + (c & 3u) * 32u;
+                    tc_mma_f16(tmem + 128u * h, umma_desc_sw128(q_addr + h * kTile + off), umma_desc_sw128(k_addr + off), idesc_s, c != 0);
+                }
+            };
+            {
+                const bool issues = elect_one();
+                ok = ok && mbar_wait(q_full, q_phase, p.status) && mbar_wait(full + 8 * pos.s, pos.phase, p.status);
+                q_phase ^= 1u;
+                tc_fence_after();
+                if (issues && ok) {
+                    if (it.tiles0 > 0) scores(0, ring + pos.s * kTile), tc_commit(s_full);
+                    if (it.tiles1 > 0) scores(1, ring + pos.s * kTile), tc_commit(s_full + 8);
+                    tc_commit(empty + 8 * pos.s);
+                    if (tiles == 1) tc_commit(q_empty);
+                }
+                __syncwarp();
+                pos.advance(kStages);
+            }
+            for (int i = 0; i < tiles; ++i) {
+                const uint32_t v_stage = pos.s;
+                ok = ok && mbar_wait(full + 8 * pos.s, pos.phase, p.status);
+                const int rows = it.keys - i * kTileKeys;
+                if (rows < kTileKeys) {                                             // rows behind the last key
+                    const uint32_t v_addr = ring + v_stage * kTile;
+                    for (int x = lane; x < (kTileKeys - rows) * 8 * DP; x += 32) {
+                        const int r = rows + x / (8 * DP), piece = x % (8 * DP);
+                        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(v_addr + (piece >> 3) * kPromptPanel + r * 128u + (piece & 7) * 16u), "r"(0u) : "memory");
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                }
+                pos.advance(kStages);
+                const bool more = i + 1 < tiles;
+                const uint32_t k_stage = pos.s;
+                if (more) {
+                    ok = ok && mbar_wait(full + 8 * pos.s, pos.phase, p.status);
+                    pos.advance(kStages);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int mine = h ? it.tiles1 : it.tiles0;
+                    if (i >= mine) continue;
+                    const bool issues = elect_one();
+                    ok = ok && mbar_wait(p_full + 8 * h, (p_phase >> h) & 1u, p.status);
+                    p_phase ^= 1u << h;
+                    tc_fence_after();
+                    if (issues && ok) {
+#pragma unroll
+                        for (uint32_t c = 0; c < kTileKeys / 16; ++c)
+                            tc_mma_f16_ta(tmem + 256u + 128u * h, tmem + 128u * h + 8u * c, umma_desc_sw128_mn(ring + v_stage * kTile + 2048u * c, kPromptPanel), idesc_o,
+                                          (uint32_t)(i | c) != 0u);
+                        // a barrier of its own for the finished sums: the next item's first scores may follow before the softmax warps have looked
+                        if (i + 1 < mine) scores(h, ring + k_stage * kTile), tc_commit(s_full + 8 * h);
+                        else tc_commit(o_full + 8 * h);
+                    }
+                    __syncwarp();
+                }
+                if (elect_one() && ok) {
+                    tc_commit(empty + 8 * v_stage);
+                    if (more) tc_commit(empty + 8 * k_stage);
+                    if (i + 2 == tiles) tc_commit(q_empty);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == kPromptLoadWarp) {
+        // ================= loads =================
+        pdl_wait_prior_grids();
+        if (lane == 0) tma_prefetch_map(&q_map), tma_prefetch_map(&k_map), tma_prefetch_map(&v_map);
+        RingPos pos = {0, 1u};
+        uint32_t q_phase = 1u;
+        int64_t loads = 0;
+        auto load_tile = [&](const CUtensorMap *map, int tile) {
+            const bool issues = elect_one();
+            ok = ok && mbar_wait(empty + 8 * pos.s, pos.phase, p.status);
+            loads += __all_sync(0xFFFFFFFFu, ok) ? 1 : 0;
+            if (issues && ok) {
+                mbar_expect_tx(full + 8 * pos.s, kTile);
+#pragma unroll
+                for (int d = 0; d < DP; ++d) tma_load_3d(ring + pos.s * kTile + d * kPromptPanel, map, 64 * d, it.kv_head, it.k0 + tile * kTileKeys, full + 8 * pos.s);
+            }
+            __syncwarp();
+            pos.advance(kStages);
+        };
+        while (next_item(it)) {
+            const int tiles = max(it.tiles0, it.tiles1);
+            if (tiles == 0) continue;
+            {
+                const bool issues = elect_one();
+                ok = ok && mbar_wait(q_empty, q_phase, p.status);
+                q_phase ^= 1u;
+                if (issues && ok) {
+                    mbar_expect_tx(q_full, (it.tiles1 > 0 ? 2u : 1u) * kTile);
+                    for (int h = 0; h < (it.tiles1 > 0 ? 2 : 1); ++h)
+#pragma unroll
+                        for (int d = 0; d < DP; ++d)
+                            tma_load_3d(q_addr + h * kTile + d * kPromptPanel, &q_map, 64 * d, it.head, it.token + h * half_tokens, q_full);
+                }
+                __syncwarp();
+            }
+            load_tile(&k_map, 0);
+            for (int i = 0; i < tiles; ++i) {
+                if (i + 1 < tiles) {
+                    load_tile(&v_map, i);
+                    load_tile(&k_map, i + 1);
+                } else {
+                    load_tile(&v_map, i);
+                }
+            }
+        }
+        if (!__all_sync(0xFFFFFFFFu, ok)) {                                         // copies in flight land before the CTA leaves
+            for (int i = 0; i < kStages; ++i)
+                if (const int64_t n = (loads - i + kStages - 1) / kStages; loads > i) mbar_wait(full + 8 * i, (uint32_t)(n - 1) & 1u, p.status);
+        }
+    } else {
+        // ================= the list of items =================
+        pdl_wait_prior_grids();
+        PromptParams q = p;
+        q.starts = after_wait(p.starts), q.kv_first = after_wait(p.kv_first), q.kv_len = after_wait(p.kv_len);
+        const int per_item = 256 / p.pack;
+        int all = 0, most = 1;
+        for (int s = lane; s < p.sequences; s += 32) {
+            const Sequence seq = sequence(q, s);
+            all += items_of(seq, per_item, 1);
+            if (seq.n > 0) most = max(most, (seq.m + kTileKeys - 1) / kTileKeys);
+        }
+        all = __reduce_add_sync(0xFFFFFFFFu, all);
+        most = __reduce_max_sync(0xFFFFFFFFu, most);
+        const int64_t total = (int64_t)all * p.kv_heads * (p.group / p.pack);
+        int64_t round = 0;
+        for (bool go = true; go; ++round) {
+            const int64_t index = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            go = round * gridDim.x < total;
+            if (go && index >= total) continue;                                     // the last round is not full
+            PromptItem next = {};
+            if (go) next = find_item(q, index, most, lane);
+            ok = ok && mbar_wait(item_empty + 8 * list.s, list.phase ^ 1u, p.status);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            if (lane == 0) {
+                const uint32_t at = items + 64u * list.s;
+                const int *w = reinterpret_cast<const int *>(&next);
+#pragma unroll
+                for (int i = 0; i < 12; ++i) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + 4u * i), "r"(w[i]) : "memory");
+                mbar_arrive(item_full + 8 * list.s);
+            }
+            __syncwarp();
+            list.advance(2);
         }
     }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == kPromptMmaWarp) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+    }
+}
+
+template <int DP, bool BF16>
+static int launch_prompt(const PromptParams &p, const CUtensorMap &q, const CUtensorMap &k, const CUtensorMap &v, unsigned grid, cudaStream_t s) {
+    static SmemOptIn opted;
+    auto kern = attn_prompt_kernel<DP, BF16>;
+    if (int e = allow_max_smem(kern, opted)) return e;
+    return launch(kern, dim3(grid), dim3(kPromptThreads), 2048 + (2 + (DP == 2 ? 5 : 8)) * DP * kPromptPanel, s, p, q, k, v);
 }
 
 }  // namespace rptc
@@ -88,19 +482,27 @@ extern "C" int rptc_attn_prompt(const rptc_prompt_attention *a, rptc_stream_t st
     }
     if (int e = rptc_check_device()) return e;
     if (a->tokens == 0 || a->sequences == 0) return RPTC_OK;
+    if (a->kv_tokens == 0) return RPTC_ERR_SHAPE;
     PromptParams p;
-    p.q = static_cast<const uint16_t *>(a->q), p.k = static_cast<const uint16_t *>(a->k), p.v = static_cast<const uint16_t *>(a->v);
     p.out = static_cast<uint16_t *>(a->out);
     p.starts = a->starts, p.kv_first = a->kv_first, p.kv_len = a->kv_len;
     p.tokens = a->tokens, p.kv_tokens = a->kv_tokens;
-    p.q_row = a->q_row, p.q_head = a->q_head, p.k_row = a->k_row, p.k_head = a->k_head;
-    p.v_row = a->v_row, p.v_head = a->v_head, p.out_row = a->out_row, p.out_head = a->out_head;
-    p.sequences = (int32_t)a->sequences, p.group = a->heads / a->kv_heads, p.d = a->d;
+    p.out_row = a->out_row, p.out_head = a->out_head;
+    p.sequences = (int32_t)a->sequences, p.group = a->heads / a->kv_heads, p.kv_heads = a->kv_heads;
+    p.pack = p.group & -p.group;
+    if (p.pack > 128) p.pack = 128;
     p.scale = a->scale * 1.4426950408889634f;
     p.status = device_status_word();
     if (!p.status) return RPTC_ERR_CUDA;
-    const int64_t per = (a->tokens + 3) / 4;
-    const dim3 grid((unsigned)(per < 2048 ? per : 2048), (unsigned)a->heads, (unsigned)a->sequences);
+    CUtensorMap q, k, v;
+    const bool bf16 = a->dtype == 1;
+    if (int e = encode_heads_map(q, a->q, bf16, a->d, a->heads, a->q_head, a->tokens, a->q_row, p.pack, 128 / p.pack)) return e;
+    if (int e = encode_heads_map(k, a->k, bf16, a->d, a->kv_heads, a->k_head, a->kv_tokens, a->k_row, 1, kTileKeys)) return e;
+    if (int e = encode_heads_map(v, a->v, bf16, a->d, a->kv_heads, a->v_head, a->kv_tokens, a->v_row, 1, kTileKeys)) return e;
+    // at most this many items: what `starts` makes of the rows is known on the device alone
+    const int64_t most = (a->tokens * p.pack / 256 + a->sequences) * a->kv_heads * (p.group / p.pack);
+    const unsigned grid = (unsigned)(most < num_sms() ? most : num_sms());
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return a->dtype ? launch(attn_prompt_kernel<true>, grid, dim3(128), 0, s, p) : launch(attn_prompt_kernel<false>, grid, dim3(128), 0, s, p);
+    if (a->d == 128) return bf16 ? launch_prompt<2, true>(p, q, k, v, grid, s) : launch_prompt<2, false>(p, q, k, v, grid, s);
+    return bf16 ? launch_prompt<1, true>(p, q, k, v, grid, s) : launch_prompt<1, false>(p, q, k, v, grid, s);
 }

@@ -471,6 +471,20 @@ int encode_map(CUtensorMap &map, const void *base, int64_t cols, int64_t rows, i
     return RPTC_ERR_CUDA;
 }
 
+int encode_heads_map(CUtensorMap &map, const void *base, bool bf16, int64_t d, int64_t heads, int64_t head_stride, int64_t rows, int64_t row_stride, int box_heads,
+                     int box_rows) {
+    auto encode = encode_tiled_fn();
+    if (!encode) return RPTC_ERR_CUDA;
+    const cuuint64_t dim[3] = {(cuuint64_t)d, (cuuint64_t)heads, (cuuint64_t)rows};
+    const cuuint64_t stride[2] = {(cuuint64_t)head_stride * 2, (cuuint64_t)row_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_rows}, estride[3] = {1, 1, 1};
+    const CUresult r = encode(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void *>(base), dim, stride, box, estride,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r == CUDA_SUCCESS) return RPTC_OK;
+    g_last_cuda_error = (int)r;
+    return RPTC_ERR_CUDA;
+}
+
 // How a product is cut into CTAs.
 struct GemmShape {
     int rows, halves, split;      // weight rows and 128-token halves of a tile, CTAs that share a tile's reduction
