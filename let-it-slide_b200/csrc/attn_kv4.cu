@@ -1,8 +1,33 @@
 // Single-query attention over a KV cache in 4 bits (rptc_kv_cache, bits = 4).  No reference counterpart.
+//
+//   s_j = scale q . k_j,  o = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j - m);   k = min + scale_g * code in groups g of 32 values, v alike
+//
+// The cache is read once, 160 bytes per position and kv head, for up to eight q heads of its group at a time.  A warp takes tiles of 32 positions through a
+// private ring of bulk copies and multiplies the codes as they are on mma.sync (m16n8k16, fp32 accumulation):
+//   scores   A = codes of 16 positions x 16 dims, B = q (column = q head).  A nibble put into the low bits of an fp16 is the number code * 2^-24, exactly, and one
+//            four bits higher 16 times that: two masks and half a shift per register, and q's values in the odd places are divided by 16 beforehand (q is first brought to
+//            at most 2 by a power of two, so that this loses nothing above 2^-25 of its largest value).  A group's sum is then scaled in fp32:
+//            s = sum_g scale_g sum_g(q code) + min_g sum_g(q).
+//   output   A = codes of 16 dims x 16 positions, B = p_j * scale_g in fp16 (one set per group; transposed from the scores' layout by movmatrix), and the same
+//            weights against a column of ones:  sum p scale (code - 8) + sum p (min + 8 scale).  Codes counted from the middle, so that what the weights' rounding
+//            (2^-11, as that of P in any 16-bit product) is multiplied with is not larger than the values; the second sum is in fp32.
+// Weights refer to the running maximum of s + log2(the position's largest scale): the products p * scale then fit fp16 whatever the scales are (2^11 at most, 2^4 of slack above
+// it before anything is rescaled; what falls below 2^-14 is 2^-25 of the largest).
+// Bound: HBM.  About 290 warp instructions per 16 positions (2560 bytes), two thirds of the issue slots at the measured copy rate.
+// Long contexts: all tiles of all rows and heads, laid end to end, are cut into equal ranges for the CTAs of one wave, so that rows of different lengths balance; a range's
+// part of a row goes to the workspace (fp32) and a second kernel joins the parts.  Short caches (max_pos up to kKv4Whole) take one CTA per row and head and no second kernel.
 #include "fwht.cuh"
 #include "kv4.cuh"
+#include "tc_ptx.cuh"
 
 namespace rptc {
+
+constexpr int kKv4Warps = 8, kKv4Tile = 32, kKv4Stages = 2;
+constexpr uint32_t kKv4StageBytes = 2 * kKv4Tile * (kKv4Codes + kKv4Scales);
+constexpr uint32_t kKv4Ring = kKv4Warps * kKv4Stages * kKv4StageBytes, kKv4Merge = kKv4Warps * 8 * 128 * 4, kKv4Smem = kKv4Ring + kKv4Merge + kKv4Warps * 8 * 8 + 256;
+constexpr int kKv4CtasPerSm = 2;
+constexpr int64_t kKv4Whole = 1024;
+constexpr float kKv4Bias = 11.f, kKv4Slack = 4.f;
 
 struct AttnKv4Params {
     const __half *q;
@@ -11,75 +36,414 @@ struct AttnKv4Params {
     const uint8_t *k, *v;
     const __half2 *k_scales, *v_scales;
     __half *out;
-    int64_t ld_out, max_pos;
-    int32_t hq, hkv;
-    float scale;
+    int64_t ld_out;
+    int32_t max_pos, rows, hkv, group, blocks;       // blocks: of eight q heads in a group
+    float scale;                                     // includes log2(e)
     const __half *signs_in;
+    float4 *part;                                    // [2 * CTAs][8][32]: a part's sums, not divided
+    float2 *part_ml;                                 // [2 * CTAs][8]: its maximum and weights' sum
     unsigned int *status;
 };
 
-// One CTA of four warps per (row, q head); eight lanes take a position, a lane four dims of each group.
-__global__ void __launch_bounds__(128) attn_kv4_kernel(const AttnKv4Params p) {
-    __shared__ float part[16][128], pm[16], pl[16], tr[128];
+__device__ __forceinline__ int kv4_context(const AttnKv4Params &p, const int32_t *pos, int row) {
+    const int at = pos[row];
+    return at >= 0 && at < p.max_pos ? at + 1 : 0;
+}
+__device__ __forceinline__ int kv4_tiles(int context) { return (context + kKv4Tile - 1) / kKv4Tile; }
+
+// How the tiles of all rows and heads are cut: `rows` rows' tiles laid end to end, each row `heads` times.
+struct Kv4Cut {
+    int64_t total, ctas;
+    __device__ __forceinline__ int64_t begin(int64_t cta) const { return total * cta / ctas; }
+    __device__ __forceinline__ int64_t cta_of(int64_t tile) const {       // the range that a tile is in
+        int64_t c = tile * ctas / total;
+        while (begin(c + 1) <= tile) ++c;
+        while (begin(c) > tile) --c;
+        return c;
+    }
+};
+__device__ __forceinline__ Kv4Cut kv4_cut(const AttnKv4Params &p, const int32_t *pos, int64_t most_ctas, int lane) {
+    int64_t sum = 0;
+    for (int r0 = 0; r0 < p.rows; r0 += 32) sum += __reduce_add_sync(0xFFFFFFFFu, r0 + lane < p.rows ? kv4_tiles(kv4_context(p, pos, r0 + lane)) : 0);
+    Kv4Cut c;
+    c.total = sum * p.hkv * p.blocks;
+    c.ctas = min(most_ctas, max((c.total + kKv4Warps - 1) / kKv4Warps, (int64_t)1));
+    return c;
+}
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t d;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
+    return d;
+}
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float lg2(float x) {
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Four neighbouring values of 128 per lane -> the same of the output, after the output projection's input transform where that is asked for.
+__device__ __forceinline__ void kv4_store(const AttnKv4Params &p, int row, int head, int lane, float (&o)[4]) {
+    if (p.signs_in) {
+        const uint2 s = *reinterpret_cast<const uint2 *>(p.signs_in + head * 128 + 4 * lane);
+        const float2 s0 = __half22float2(u32_as_half2(s.x)), s1 = __half22float2(u32_as_half2(s.y));
+        o[0] *= s0.x, o[1] *= s0.y, o[2] *= s1.x, o[3] *= s1.y;
+        const float a = o[0] + o[1], b = o[0] - o[1], c = o[2] + o[3], d = o[2] - o[3];
+        o[0] = a + c, o[1] = b + d, o[2] = a - c, o[3] = b - d;
+#pragma unroll
+        for (int m = 1; m < 32; m <<= 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = __shfl_xor_sync(0xFFFFFFFFu, o[i], m);
+                o[i] = (lane & m) ? x - o[i] : o[i] + x;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] *= hadamard_norm_dev(128);
+    }
+    *reinterpret_cast<uint2 *>(p.out + (int64_t)row * p.ld_out + head * 128 + 4 * lane) =
+        make_uint2(half2_as_u32(__floats2half2_rn(o[0], o[1])), half2_as_u32(__floats2half2_rn(o[2], o[3])));
+}
+
+template <bool WHOLE>
+__global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel(const AttnKv4Params p) {
+    extern __shared__ __align__(128) unsigned char smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const uint32_t ring = smem_addr(smem) + (uint32_t)warp * kKv4Stages * kKv4StageBytes;
+    float *merge = reinterpret_cast<float *>(smem + kKv4Ring);
+    float2 *merge_ml = reinterpret_cast<float2 *>(smem + kKv4Ring + kKv4Merge);
+    const uint32_t bars = smem_addr(smem) + kKv4Ring + kKv4Merge + kKv4Warps * 8 * 8 + 8u * kKv4Stages * warp;
     pdl_allow_next_grid();
+    if (lane == 0) {
+        for (int i = 0; i < kKv4Stages; ++i) mbar_init(bars + 8 * i, 1);
+        mbar_fence_init();
+    }
+    __syncwarp();
     pdl_wait_prior_grids();
-    const int row = blockIdx.y, head = blockIdx.x, kvh = head / (p.hq / p.hkv), t = threadIdx.x, g = t & 7, grp = t >> 3;
-    const int pos = __ldg(after_wait(p.pos) + row);
-    __half *out = p.out + (int64_t)row * p.ld_out + head * 128;
-    if (pos < 0 || pos >= p.max_pos) {
-        if (pos != -1 && t == 0) atomicExch(p.status, kStatusPosition);
-        out[t] = __float2half_rn(0.f);
+    const int32_t *pos = after_wait(p.pos);
+    const int heads = p.hkv * p.blocks;              // of a row, in the order of the cut
+    int64_t at = 0, end = 0;
+    if (!WHOLE) {
+        const Kv4Cut cut = kv4_cut(p, pos, gridDim.x, lane);
+        if (blockIdx.x >= cut.ctas || cut.total == 0) return;
+        at = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
+    }
+    RingPos ring_pos = {0, 0u};
+    bool ok = true;
+    do {
+        // ---- a row's head, its tiles t0 .. t1 - 1 ----
+        int row, head, context, t0, t1, tiles;
+        if (WHOLE) {
+            row = blockIdx.y, head = blockIdx.x;
+            context = kv4_context(p, pos, row);
+            if (context == 0 && pos[row] != -1 && tid == 0) atomicExch(p.status, kStatusPosition);
+            t0 = 0, t1 = tiles = kv4_tiles(context);
+        } else {
+            int64_t before = 0;
+            row = 0;
+            tiles = 0;
+            for (int r0 = 0; r0 < p.rows; r0 += 32) {
+                const int mine = r0 + lane < p.rows ? kv4_tiles(kv4_context(p, pos, r0 + lane)) : 0;
+                int upto = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                const unsigned hit = __ballot_sync(0xFFFFFFFFu, (before + upto) * heads > at);
+                if (hit) {
+                    const int from = __ffs(hit) - 1;
+                    row = r0 + from;
+                    tiles = __shfl_sync(0xFFFFFFFFu, mine, from);
+                    before += __shfl_sync(0xFFFFFFFFu, upto - mine, from);
+                    break;
+                }
+                before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+            }
+            const int64_t in_row = at - before * heads;
+            head = (int)(in_row / tiles);
+            t0 = (int)(in_row - (int64_t)head * tiles);
+            t1 = (int)min((int64_t)tiles, t0 + (end - at));
+            context = kv4_context(p, pos, row);
+            at += t1 - t0;
+        }
+        const int kvh = head / p.blocks, first = (head - kvh * p.blocks) * 8, in_block = min(8, p.group - first), q_head = kvh * p.group + first;
+        const int64_t cache_at = ((int64_t)row * p.hkv + kvh) * p.max_pos;
+        const uint8_t *k = after_wait(p.k) + cache_at * kKv4Codes, *v = after_wait(p.v) + cache_at * kKv4Codes;
+        const __half2 *ks = after_wait(p.k_scales) + cache_at * 4, *vs = after_wait(p.v_scales) + cache_at * 4;
+        auto fetch = [&](int tile, int stage) {      // by lane 0
+            const uint32_t n = (uint32_t)min(kKv4Tile, context - tile * kKv4Tile), dst = ring + (uint32_t)stage * kKv4StageBytes, bar = bars + 8u * stage;
+            const int64_t from = (int64_t)tile * kKv4Tile;
+            mbar_expect_tx(bar, 2 * n * (kKv4Codes + kKv4Scales));
+            bulk_g2s(dst, k + from * kKv4Codes, n * kKv4Codes, bar);
+            bulk_g2s(dst + kKv4Tile * kKv4Codes, ks + from * 4, n * kKv4Scales, bar);
+            bulk_g2s(dst + kKv4Tile * (kKv4Codes + kKv4Scales), v + from * kKv4Codes, n * kKv4Codes, bar);
+            bulk_g2s(dst + kKv4Tile * (2 * kKv4Codes + kKv4Scales), vs + from * 4, n * kKv4Scales, bar);
+        };
+        if (lane == 0) {
+            int s = ring_pos.s;
+            for (int i = 0; i < kKv4Stages; ++i, s = s + 1 == kKv4Stages ? 0 : s + 1)
+                if (t0 + warp + i * kKv4Warps < t1) fetch(t0 + warp + i * kKv4Warps, s);
+        }
+        // ---- q: this lane's operand values are those of q head g, dims 8 t .. 8 t + 7 of each group ----
+        uint32_t qb[4][4];
+        float q_sum[4][2], factor[2];                // of the q heads 2 t and 2 t + 1, whose scores this lane gets
+        {
+            float x[4][8], big = 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+                if (g < in_block) raw = ld_ordered_u128(p.q + (int64_t)row * p.ld_q + (q_head + g) * 128 + 32 * j + 8 * t);
+                unpack8(raw, x[j]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[j][i]));
+            }
+            big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
+            const int e = big > 0.f ? (int)(__float_as_uint(big) >> 23) - 127 : 0;
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23), mine = __uint_as_float((uint32_t)(127 + 24 + e) << 23) * p.scale;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float sum = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[j][i] *= down;
+                    sum += x[j][i];
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float odd = (i & 1) ? 0.0625f : 1.f;
+                    qb[j][i] = half2_as_u32(__floats2half2_rn(x[j][i] * odd, x[j][i + 4] * odd));
+                }
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
+                sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
+                sum *= 5.9604644775390625e-8f;       // 2^-24, the codes' unit
+                q_sum[j][0] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t);
+                q_sum[j][1] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4);
+            }
+            factor[0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * t);
+            factor[1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * t + 4);
+        }
+        // ---- this warp's tiles ----
+        float o[8][4] = {}, ones[4][4] = {}, low[4][2] = {}, l[2] = {0.f, 0.f}, m[2] = {-INFINITY, -INFINITY};
+        const int my_row = (g >> 1) + 4 * (g & 1);   // the position of an operand's row g, so that the V operand's rows t and t + 4 are neighbours in the product
+        constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
+#pragma unroll 1
+        for (int tile = t0 + warp; tile < t1 && ok; tile += kKv4Warps) {
+            const uint32_t src = ring + (uint32_t)ring_pos.s * kKv4StageBytes, v_src = src + kKv4Tile * (kKv4Codes + kKv4Scales);
+            ok = __all_sync(0xFFFFFFFFu, mbar_wait(bars + 8u * ring_pos.s, ring_pos.phase, p.status));
+            const int left = context - tile * kKv4Tile;
+            float s[2][4];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t a = 16 * u + my_row, b = a + 8;
+                const uint4 xa = lds128(src + a * kKv4Codes + 16 * t), xb = lds128(src + b * kKv4Codes + 16 * t);
+                uint4 sa = lds128(src + kKv4Tile * kKv4Codes + a * kKv4Scales), sb = lds128(src + kKv4Tile * kKv4Codes + b * kKv4Scales);
+                if ((int)a >= left) sa = make_uint4(0u, 0u, 0u, 0u);
+                if ((int)b >= left) sb = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[u][i] = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+                    const uint32_t wa = j < 2 ? prmt(xa.x, xa.z, sel) : prmt(xa.y, xa.w, sel), wb = j < 2 ? prmt(xb.x, xb.z, sel) : prmt(xb.y, xb.w, sel);
+                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma_16816(c, wa & kLow, wb & kLow, wa & kHigh, wb & kHigh, qb[j][0], qb[j][1]);
+                    mma_16816(c, (wa >> 8) & kLow, (wb >> 8) & kLow, (wa >> 8) & kHigh, (wb >> 8) & kHigh, qb[j][2], qb[j][3]);
+                    const float2 fa = __half22float2(u32_as_half2(j == 0 ? sa.x : j == 1 ? sa.y : j == 2 ? sa.z : sa.w));
+                    const float2 fb = __half22float2(u32_as_half2(j == 0 ? sb.x : j == 1 ? sb.y : j == 2 ? sb.z : sb.w));
+                    s[u][0] = fmaf(fa.x, c[0], fmaf(fa.y, q_sum[j][0], s[u][0]));
+                    s[u][1] = fmaf(fa.x, c[1], fmaf(fa.y, q_sum[j][1], s[u][1]));
+                    s[u][2] = fmaf(fb.x, c[2], fmaf(fb.y, q_sum[j][0], s[u][2]));
+                    s[u][3] = fmaf(fb.x, c[3], fmaf(fb.y, q_sum[j][1], s[u][3]));
+                }
+                s[u][0] = (int)a < left ? s[u][0] * factor[0] : -INFINITY;
+                s[u][1] = (int)a < left ? s[u][1] * factor[1] : -INFINITY;
+                s[u][2] = (int)b < left ? s[u][2] * factor[0] : -INFINITY;
+                s[u][3] = (int)b < left ? s[u][3] * factor[1] : -INFINITY;
+            }
+            // ---- the positions' v scales, and the running maximum of score + log2(largest scale) ----
+            float2 va[2][4], vb[2][4];               // scale, minimum + 8 scales
+            float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const uint32_t a = 16 * u + my_row, b = a + 8, at_s = v_src + kKv4Tile * kKv4Codes;
+                uint4 sa = lds128(at_s + a * kKv4Scales), sb = lds128(at_s + b * kKv4Scales);
+                if ((int)a >= left) sa = make_uint4(0u, 0u, 0u, 0u);
+                if ((int)b >= left) sb = make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t ra[4] = {sa.x, sa.y, sa.z, sa.w}, rb[4] = {sb.x, sb.y, sb.z, sb.w};
+                float big_a = 5.9604644775390625e-8f, big_b = big_a;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    va[u][j] = __half22float2(u32_as_half2(ra[j])), vb[u][j] = __half22float2(u32_as_half2(rb[j]));
+                    big_a = fmaxf(big_a, va[u][j].x), big_b = fmaxf(big_b, vb[u][j].x);
+                    va[u][j].y = fmaf(8.f, va[u][j].x, va[u][j].y), vb[u][j].y = fmaf(8.f, vb[u][j].x, vb[u][j].y);
+                }
+                const float la = lg2(big_a), lb = lg2(big_b);
+                top[0] = fmaxf(top[0], fmaxf(s[u][0] + la, s[u][2] + lb));
+                top[1] = fmaxf(top[1], fmaxf(s[u][1] + la, s[u][3] + lb));
+            }
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+                top[0] = fmaxf(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], x));
+                top[1] = fmaxf(top[1], __shfl_xor_sync(0xFFFFFFFFu, top[1], x));
+            }
+            if (__any_sync(0xFFFFFFFFu, top[0] > m[0] + kKv4Slack || top[1] > m[1] + kKv4Slack)) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float to = fmaxf(m[c], top[c]), f = m[c] == -INFINITY ? 0.f : ex2(m[c] - to);
+                    m[c] = to;
+                    l[c] *= f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i][c] *= f, o[i][2 + c] *= f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) ones[j][c] *= f, ones[j][2 + c] *= f, low[j][c] *= f;
+                }
+            }
+            // ---- weights, and what they are multiplied with ----
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float pa0 = ex2(s[u][0] - (m[0] - kKv4Bias)), pa1 = ex2(s[u][1] - (m[1] - kKv4Bias));
+                const float pb0 = ex2(s[u][2] - (m[0] - kKv4Bias)), pb1 = ex2(s[u][3] - (m[1] - kKv4Bias));
+                l[0] += pa0 + pb0, l[1] += pa1 + pb1;
+                const uint32_t at_v = v_src + (16 * u + t) * kKv4Codes + 8 * g;
+                const uint2 v0 = lds64(at_v), v1 = lds64(at_v + 4 * kKv4Codes), v2 = lds64(at_v + 8 * kKv4Codes), v3 = lds64(at_v + 12 * kKv4Codes);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
+                    const uint32_t b0 = transpose8(half2_as_u32(__floats2half2_rn(pa0 * va[u][j].x, pa1 * va[u][j].x)));
+                    const uint32_t b1 = transpose8(half2_as_u32(__floats2half2_rn(pb0 * vb[u][j].x, pb1 * vb[u][j].x)));
+                    const uint32_t w0 = j < 2 ? prmt(v0.x, v1.x, sel) : prmt(v0.y, v1.y, sel), w1 = j < 2 ? prmt(v2.x, v3.x, sel) : prmt(v2.y, v3.y, sel);
+                    mma_16816(o[2 * j], w0 & kLow, w0 & kHigh, w1 & kLow, w1 & kHigh, b0, b1);
+                    mma_16816(o[2 * j + 1], (w0 >> 8) & kLow, (w0 >> 8) & kHigh, (w1 >> 8) & kLow, (w1 >> 8) & kHigh, b0, b1);
+                    mma_16816(ones[j], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, b0, b1);
+                    low[j][0] = fmaf(pa0, va[u][j].y, fmaf(pb0, vb[u][j].y, low[j][0]));
+                    low[j][1] = fmaf(pa1, va[u][j].y, fmaf(pb1, vb[u][j].y, low[j][1]));
+                }
+            }
+            __syncwarp();                            // the stage is free
+            if (lane == 0 && ok && tile + kKv4Stages * kKv4Warps < t1) fetch(tile + kKv4Stages * kKv4Warps, ring_pos.s);
+            ring_pos.advance(kKv4Stages);
+        }
+        // ---- the warps' sums into one ----
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                l[c] += __shfl_xor_sync(0xFFFFFFFFu, l[c], x);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) low[j][c] += __shfl_xor_sync(0xFFFFFFFFu, low[j][c], x);
+            }
+        }
+        __syncthreads();                             // the last segment's sums have been taken
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float *dst = merge + (warp * 8 + 2 * t + c) * 128 + 4 * g;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float mid = fmaf(-8.f, ones[j][c], low[j][c]);
+                *reinterpret_cast<float4 *>(dst + 32 * j) = make_float4(fmaf(16777216.f, o[2 * j][c], mid), fmaf(1048576.f, o[2 * j][2 + c], mid),
+                                                                         fmaf(16777216.f, o[2 * j + 1][c], mid), fmaf(1048576.f, o[2 * j + 1][2 + c], mid));
+            }
+            if (g == 0) merge_ml[warp * 8 + 2 * t + c] = make_float2(m[c], l[c]);
+        }
+        __syncthreads();
+        if (warp < in_block) {                       // a warp per q head
+            float2 ml[kKv4Warps];
+            float mx = -INFINITY, den = 0.f, sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < kKv4Warps; ++w) ml[w] = merge_ml[w * 8 + warp], mx = fmaxf(mx, ml[w].x);
+#pragma unroll
+            for (int w = 0; w < kKv4Warps; ++w) {
+                const float f = ml[w].x == -INFINITY && ml[w].y == 0.f ? 0.f : ex2(ml[w].x - mx);      // a warp without a tile
+                const float4 x = *reinterpret_cast<const float4 *>(merge + (w * 8 + warp) * 128 + 4 * lane);
+                den = fmaf(ml[w].y, f, den);
+                sum[0] = fmaf(x.x, f, sum[0]), sum[1] = fmaf(x.y, f, sum[1]), sum[2] = fmaf(x.z, f, sum[2]), sum[3] = fmaf(x.w, f, sum[3]);
+            }
+            if (WHOLE || (t0 == 0 && t1 == tiles)) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[i] = context ? sum[i] / den : 0.f;
+                kv4_store(p, row, q_head + warp, lane, sum);
+            } else {
+                const int64_t slot = (2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * 8 + warp;
+                p.part[slot * 32 + lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+                if (lane == 0) p.part_ml[slot] = make_float2(mx, den);
+            }
+        }
+    } while (!WHOLE && at < end && ok);
+    if (!ok) {                                       // copies in flight land before the CTA leaves
+        for (int i = 0; i < kKv4Stages; ++i, ring_pos.advance(kKv4Stages)) mbar_wait(bars + 8u * ring_pos.s, ring_pos.phase, p.status);
+    }
+}
+
+// A CTA per row and q head: joins the parts that ranges have left of it, and writes the zeros of a row without positions.
+__global__ void __launch_bounds__(512) attn_kv4_join_kernel(const AttnKv4Params p, int64_t most_ctas) {
+    __shared__ float4 sums[16][32];
+    __shared__ float dens[16];
+    pdl_allow_next_grid();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    pdl_wait_prior_grids();
+    const int32_t *pos = after_wait(p.pos);
+    const int row = blockIdx.y, q_head = blockIdx.x, kvh = q_head / p.group, in_group = q_head - kvh * p.group, head = kvh * p.blocks + in_group / 8;
+    const int tiles = kv4_tiles(kv4_context(p, pos, row));
+    if (tiles == 0) {
+        if (q_head == 0 && threadIdx.x == 0 && pos[row] != -1) atomicExch(p.status, kStatusPosition);
+        float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        if (warp == 0) kv4_store(p, row, q_head, lane, zero);
         return;
     }
-    float q[16], acc[16] = {}, m = -INFINITY, l = 0.f;
-    const __half *qp = after_wait(p.q) + (int64_t)row * p.ld_q + head * 128;
+    const Kv4Cut cut = kv4_cut(p, pos, most_ctas, lane);
+    int64_t before = 0;
+    for (int r0 = 0; r0 < row; r0 += 32) before += __reduce_add_sync(0xFFFFFFFFu, r0 + lane < row ? kv4_tiles(kv4_context(p, pos, r0 + lane)) : 0);
+    const int64_t begin = before * p.hkv * p.blocks + (int64_t)head * tiles;
+    const int64_t c0 = cut.cta_of(begin), c1 = cut.cta_of(begin + tiles - 1);
+    if (c0 == c1) return;                            // one range had it all
+    const float4 *part = after_wait(p.part);
+    const float2 *part_ml = after_wait(p.part_ml);
+    float mx = -INFINITY, den = 0.f;
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int64_t c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, __ldcg(part_ml + (2 * c + (c == c0 ? 1 : 0)) * 8 + (in_group & 7)).x);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) q[i] = __half2float(qp[32 * (i >> 2) + 4 * g + (i & 3)]) * p.scale * 1.4426950408889634f;
-    for (int j0 = 0; j0 <= pos; j0 += 16) {
-        const int j = j0 + grp;
-        const int64_t at = ((int64_t)row * p.hkv + kvh) * p.max_pos + min(j, pos);
-        auto values = [&](const uint8_t *c, const __half2 *s, float (&x)[16]) {
-            const uint2 w = *reinterpret_cast<const uint2 *>(c + at * kKv4Codes + 8 * g);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float2 f = __half22float2(s[at * 4 + (i >> 2)]);
-                x[i] = fmaf((float)(((i < 8 ? w.x : w.y) >> (4 * (i & 7))) & 15u), f.x, f.y);
-            }
-        };
-        float x[16], s = 0.f;
-        values(after_wait(p.k), after_wait(p.k_scales), x);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s = fmaf(q[i], x[i], s);
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
-        if (j > pos) continue;                               // of eight lanes, which meet again at the next shuffle
-        const float mn = fmaxf(m, s), f = exp2f(m - mn), e = exp2f(s - mn);
-        values(after_wait(p.v), after_wait(p.v_scales), x);
-        l = l * f + e;
-        m = mn;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) acc[i] = fmaf(e, x[i], acc[i] * f);
+    for (int o = 1; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+#pragma unroll 4
+    for (int64_t c = c0 + warp; c <= c1; c += 16) {
+        const int64_t slot = (2 * c + (c == c0 ? 1 : 0)) * 8 + (in_group & 7);
+        const float2 ml = __ldcg(part_ml + slot);
+        const float4 x = __ldcg(part + slot * 32 + lane);
+        const float f = ex2(ml.x - mx);
+        den = fmaf(ml.y, f, den);
+        sum.x = fmaf(x.x, f, sum.x), sum.y = fmaf(x.y, f, sum.y), sum.z = fmaf(x.z, f, sum.z), sum.w = fmaf(x.w, f, sum.w);
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) part[grp][32 * (i >> 2) + 4 * g + (i & 3)] = acc[i];
-    if (g == 0) pm[grp] = m, pl[grp] = l;
+    sums[warp][lane] = sum;
+    if (lane == 0) dens[warp] = den;
     __syncthreads();
-    float mx = pm[0], num = 0.f, den = 0.f;
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, pm[i]);
-    for (int i = 0; i < 16; ++i) {
-        const float f = exp2f(pm[i] - mx);
-        num += part[i][t] * f;
-        den += pl[i] * f;
+    if (warp) return;
+    float out[4] = {0.f, 0.f, 0.f, 0.f};
+    den = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        const float4 x = sums[w][lane];
+        den += dens[w];
+        out[0] += x.x, out[1] += x.y, out[2] += x.z, out[3] += x.w;
     }
-    float o = num / den;
-    if (p.signs_in) {
-        tr[t] = __half2float(__float2half_rn(o)) * __half2float(p.signs_in[head * 128 + t]);
-        __syncthreads();
-        o = 0.f;
-        for (int i = 0; i < 128; ++i) o += (__popc(i & t) & 1) ? -tr[i] : tr[i];
-        o *= hadamard_norm_dev(128);
-    }
-    out[t] = __float2half_rn(o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) out[i] /= den;
+    kv4_store(p, row, q_head, lane, out);
 }
 
 }  // namespace rptc
@@ -87,8 +451,8 @@ __global__ void __launch_bounds__(128) attn_kv4_kernel(const AttnKv4Params p) {
 using namespace rptc;
 
 extern "C" int64_t rptc_attn_decode_kv4_workspace_bytes(const rptc_kv_cache *cache, int heads) {
-    (void)cache, (void)heads;
-    return 0;
+    if (!cache || check_kv_cache(*cache) || cache->bits != 4 || cache->max_pos <= kKv4Whole || heads <= 0) return 0;
+    return (int64_t)num_sms() * kKv4CtasPerSm * 2 * 8 * (128 * 4 + 8);
 }
 
 extern "C" int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *pos, const rptc_kv_cache *cache, void *out, int64_t ld_out, int heads,
@@ -111,10 +475,25 @@ extern "C" int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *
     p.q = static_cast<const __half *>(q), p.ld_q = ld_q, p.pos = pos;
     p.k = static_cast<const uint8_t *>(cache->k), p.v = static_cast<const uint8_t *>(cache->v);
     p.k_scales = static_cast<const __half2 *>(cache->k_scales), p.v_scales = static_cast<const __half2 *>(cache->v_scales);
-    p.out = static_cast<__half *>(out), p.ld_out = ld_out, p.max_pos = cache->max_pos;
-    p.hq = heads, p.hkv = cache->kv_heads, p.scale = scale;
+    p.out = static_cast<__half *>(out), p.ld_out = ld_out;
+    p.max_pos = (int32_t)cache->max_pos, p.rows = (int32_t)cache->rows, p.hkv = cache->kv_heads;
+    p.group = heads / cache->kv_heads, p.blocks = (p.group + 7) / 8;
+    p.scale = scale * 1.4426950408889634f;
     p.signs_in = static_cast<const __half *>(signs_in);
     p.status = device_status_word();
     if (!p.status) return RPTC_ERR_CUDA;
-    return launch(attn_kv4_kernel, dim3((unsigned)heads, (unsigned)cache->rows), dim3(128), 0, static_cast<cudaStream_t>(stream), p);
+    p.part = nullptr, p.part_ml = nullptr;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (cache->max_pos <= kKv4Whole) {
+        static SmemOptIn opted;
+        if (int e = allow_max_smem(attn_kv4_kernel<true>, opted)) return e;
+        return launch(attn_kv4_kernel<true>, dim3((unsigned)(p.hkv * p.blocks), (unsigned)p.rows), dim3(32 * kKv4Warps), kKv4Smem, s, p);
+    }
+    const int64_t ctas = (int64_t)num_sms() * kKv4CtasPerSm;
+    p.part = static_cast<float4 *>(workspace);
+    p.part_ml = reinterpret_cast<float2 *>(p.part + ctas * 2 * 8 * 32);
+    static SmemOptIn opted;
+    if (int e = allow_max_smem(attn_kv4_kernel<false>, opted)) return e;
+    if (int e = launch(attn_kv4_kernel<false>, dim3((unsigned)ctas), dim3(32 * kKv4Warps), kKv4Smem, s, p)) return e;
+    return launch(attn_kv4_join_kernel, dim3((unsigned)heads, (unsigned)p.rows), dim3(512), 0, s, p, ctas);
 }
