@@ -7,7 +7,8 @@
 //   scores   A = codes of 16 positions x 16 dims, B = q (column = q head).  A nibble put into the low bits of an fp16 is the number code * 2^-24, exactly, and one
 //            four bits higher 16 times that: two masks and half a shift per register, and q's values in the odd places are divided by 16 beforehand (q is first brought to
 //            at most 2 by a power of two, so that this loses nothing above 2^-25 of its largest value).  A group's sum is then scaled in fp32:
-//            s = sum_g scale_g sum_g(q code) + min_g sum_g(q).
+//            s = sum_g scale_g sum_g(q code) + min_g sum_g(q), the second sum as one more product, of the stored (scale, minimum) pairs with (0, sum_g(q)) in two
+//            fp16 parts.
 //   output   A = codes of 16 dims x 16 positions, B = p_j * scale_g in fp16 (one set per group; transposed from the scores' layout by movmatrix), and the same
 //            weights against a column of ones:  sum p scale (code - 8) + sum p (min + 8 scale).  Codes counted from the middle, so that what the weights' rounding
 //            (2^-11, as that of P in any 16-bit product) is multiplied with is not larger than the values; the second sum is in fp32.
@@ -80,6 +81,12 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
     uint32_t d;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
     return d;
+}
+// The first product of a sum: mma_16816 from zeros.
+__device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
     uint2 v;
@@ -201,10 +208,10 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                 if (t0 + warp + i * kKv4Warps < t1) fetch(t0 + warp + i * kKv4Warps, s);
         }
         // ---- q: this lane's operand values are those of q head g, dims 8 t .. 8 t + 7 of each group ----
-        uint32_t qb[4][4];
-        float q_sum[4][2], factor[2];                // of the q heads 2 t and 2 t + 1, whose scores this lane gets
+        uint32_t qb[4][4], q_low[2];                 // q_low: (0, sum of q over group t) in two fp16 parts, against (scale, minimum) pairs
+        float code_unit[2], low_unit[2];             // of the q heads 2 t and 2 t + 1, whose scores this lane gets
         {
-            float x[4][8], big = 0.f;
+            float x[4][8], big = 0.f, mine = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 uint4 raw = make_uint4(0u, 0u, 0u, 0u);
@@ -216,7 +223,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
             big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
             const int e = big > 0.f ? (int)(__float_as_uint(big) >> 23) - 127 : 0;
-            const float down = __uint_as_float((uint32_t)(127 - e) << 23), mine = __uint_as_float((uint32_t)(127 + 24 + e) << 23) * p.scale;
+            const float down = __uint_as_float((uint32_t)(127 - e) << 23), up = __uint_as_float((uint32_t)(127 + e) << 23) * p.scale;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 float sum = 0.f;
@@ -232,12 +239,13 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                 }
                 sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 1);
                 sum += __shfl_xor_sync(0xFFFFFFFFu, sum, 2);
-                sum *= 5.9604644775390625e-8f;       // 2^-24, the codes' unit
-                q_sum[j][0] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t);
-                q_sum[j][1] = __shfl_sync(0xFFFFFFFFu, sum, 8 * t + 4);
+                mine = j == t ? sum : mine;
             }
-            factor[0] = __shfl_sync(0xFFFFFFFFu, mine, 8 * t);
-            factor[1] = __shfl_sync(0xFFFFFFFFu, mine, 8 * t + 4);
+            const __half hi = __float2half_rn(mine);
+            q_low[0] = half2_as_u32(__halves2half2(__float2half_rn(0.f), hi));
+            q_low[1] = half2_as_u32(__halves2half2(__float2half_rn(0.f), __float2half_rn(mine - __half2float(hi))));
+            low_unit[0] = __shfl_sync(0xFFFFFFFFu, up, 8 * t), low_unit[1] = __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4);
+            code_unit[0] = low_unit[0] * 16777216.f, code_unit[1] = low_unit[1] * 16777216.f;
         }
         // ---- this warp's tiles ----
         float o[8][4] = {}, ones[4][4] = {}, low[4][2] = {}, l[2] = {0.f, 0.f}, m[2] = {-INFINITY, -INFINITY};
@@ -245,58 +253,51 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
         constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
 #pragma unroll 1
         for (int tile = t0 + warp; tile < t1 && ok; tile += kKv4Warps) {
-            const uint32_t src = ring + (uint32_t)ring_pos.s * kKv4StageBytes, v_src = src + kKv4Tile * (kKv4Codes + kKv4Scales);
+            const uint32_t src = ring + (uint32_t)ring_pos.s * kKv4StageBytes, ks_src = src + kKv4Tile * kKv4Codes + my_row * kKv4Scales;
+            const uint32_t v_src = src + kKv4Tile * (kKv4Codes + kKv4Scales), vs_src = v_src + kKv4Tile * kKv4Codes + my_row * kKv4Scales;
             ok = __all_sync(0xFFFFFFFFu, mbar_wait(bars + 8u * ring_pos.s, ring_pos.phase, p.status));
             const int left = context - tile * kKv4Tile;
             float s[2][4];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const uint32_t a = 16 * u + my_row, b = a + 8;
-                const uint4 xa = lds128(src + a * kKv4Codes + 16 * t), xb = lds128(src + b * kKv4Codes + 16 * t);
-                uint4 sa = lds128(src + kKv4Tile * kKv4Codes + a * kKv4Scales), sb = lds128(src + kKv4Tile * kKv4Codes + b * kKv4Scales);
-                if ((int)a >= left) sa = make_uint4(0u, 0u, 0u, 0u);
-                if ((int)b >= left) sb = make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[u][i] = 0.f;
+                const uint32_t a = src + (16 * u + my_row) * kKv4Codes + 16 * t;
+                const uint4 xa = lds128(a), xb = lds128(a + 8 * kKv4Codes);
+                const uint4 sa = lds128(ks_src + 16 * u * kKv4Scales), sb = lds128(ks_src + (16 * u + 8) * kKv4Scales);
+                const uint32_t pa = lds32(ks_src + 16 * u * kKv4Scales + 4 * t), pb = lds32(ks_src + (16 * u + 8) * kKv4Scales + 4 * t);
+                float low_part[4], part[4];
+                mma_first(low_part, pa, pb, pa, pb, q_low[0], q_low[1]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
                     const uint32_t wa = j < 2 ? prmt(xa.x, xa.z, sel) : prmt(xa.y, xa.w, sel), wb = j < 2 ? prmt(xb.x, xb.z, sel) : prmt(xb.y, xb.w, sel);
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
-                    mma_16816(c, wa & kLow, wb & kLow, wa & kHigh, wb & kHigh, qb[j][0], qb[j][1]);
+                    float c[4];
+                    mma_first(c, wa & kLow, wb & kLow, wa & kHigh, wb & kHigh, qb[j][0], qb[j][1]);
                     mma_16816(c, (wa >> 8) & kLow, (wb >> 8) & kLow, (wa >> 8) & kHigh, (wb >> 8) & kHigh, qb[j][2], qb[j][3]);
-                    const float2 fa = __half22float2(u32_as_half2(j == 0 ? sa.x : j == 1 ? sa.y : j == 2 ? sa.z : sa.w));
-                    const float2 fb = __half22float2(u32_as_half2(j == 0 ? sb.x : j == 1 ? sb.y : j == 2 ? sb.z : sb.w));
-                    s[u][0] = fmaf(fa.x, c[0], fmaf(fa.y, q_sum[j][0], s[u][0]));
-                    s[u][1] = fmaf(fa.x, c[1], fmaf(fa.y, q_sum[j][1], s[u][1]));
-                    s[u][2] = fmaf(fb.x, c[2], fmaf(fb.y, q_sum[j][0], s[u][2]));
-                    s[u][3] = fmaf(fb.x, c[3], fmaf(fb.y, q_sum[j][1], s[u][3]));
+                    const float fa = __low2float(u32_as_half2(j == 0 ? sa.x : j == 1 ? sa.y : j == 2 ? sa.z : sa.w));
+                    const float fb = __low2float(u32_as_half2(j == 0 ? sb.x : j == 1 ? sb.y : j == 2 ? sb.z : sb.w));
+                    part[0] = j ? fmaf(fa, c[0], part[0]) : fa * c[0];
+                    part[1] = j ? fmaf(fa, c[1], part[1]) : fa * c[1];
+                    part[2] = j ? fmaf(fb, c[2], part[2]) : fb * c[2];
+                    part[3] = j ? fmaf(fb, c[3], part[3]) : fb * c[3];
                 }
-                s[u][0] = (int)a < left ? s[u][0] * factor[0] : -INFINITY;
-                s[u][1] = (int)a < left ? s[u][1] * factor[1] : -INFINITY;
-                s[u][2] = (int)b < left ? s[u][2] * factor[0] : -INFINITY;
-                s[u][3] = (int)b < left ? s[u][3] * factor[1] : -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[u][i] = fmaf(part[i], code_unit[i & 1], low_part[i] * low_unit[i & 1]);
             }
-            // ---- the positions' v scales, and the running maximum of score + log2(largest scale) ----
-            float2 va[2][4], vb[2][4];               // scale, minimum + 8 scales
+            if (left < kKv4Tile) {                   // positions behind the last: whatever the ring holds there
+#pragma unroll
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[u][i] = 16 * u + 8 * (i >> 1) + my_row < left ? s[u][i] : -INFINITY;
+            }
+            // ---- the running maximum of score + log2(the position's largest v scale) ----
             float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint32_t a = 16 * u + my_row, b = a + 8, at_s = v_src + kKv4Tile * kKv4Codes;
-                uint4 sa = lds128(at_s + a * kKv4Scales), sb = lds128(at_s + b * kKv4Scales);
-                if ((int)a >= left) sa = make_uint4(0u, 0u, 0u, 0u);
-                if ((int)b >= left) sb = make_uint4(0u, 0u, 0u, 0u);
-                const uint32_t ra[4] = {sa.x, sa.y, sa.z, sa.w}, rb[4] = {sb.x, sb.y, sb.z, sb.w};
-                float big_a = 5.9604644775390625e-8f, big_b = big_a;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    va[u][j] = __half22float2(u32_as_half2(ra[j])), vb[u][j] = __half22float2(u32_as_half2(rb[j]));
-                    big_a = fmaxf(big_a, va[u][j].x), big_b = fmaxf(big_b, vb[u][j].x);
-                    va[u][j].y = fmaf(8.f, va[u][j].x, va[u][j].y), vb[u][j].y = fmaf(8.f, vb[u][j].x, vb[u][j].y);
-                }
-                const float la = lg2(big_a), lb = lg2(big_b);
-                top[0] = fmaxf(top[0], fmaxf(s[u][0] + la, s[u][2] + lb));
-                top[1] = fmaxf(top[1], fmaxf(s[u][1] + la, s[u][3] + lb));
+            for (int u = 0; u < 4; ++u) {
+                const uint4 r = lds128(vs_src + 8 * u * kKv4Scales);
+                const __half2 big = __hmax2(__hmax2(u32_as_half2(r.x), u32_as_half2(r.y)), __hmax2(u32_as_half2(r.z), u32_as_half2(r.w)));
+                const float lb = lg2(fmaxf(__low2float(big), 5.9604644775390625e-8f));
+                top[0] = fmaxf(top[0], s[u >> 1][2 * (u & 1)] + lb);
+                top[1] = fmaxf(top[1], s[u >> 1][2 * (u & 1) + 1] + lb);
             }
 #pragma unroll
             for (int x = 4; x < 32; x <<= 1) {
@@ -316,24 +317,32 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                 }
             }
             // ---- weights, and what they are multiplied with ----
+            const float from0 = m[0] - kKv4Bias, from1 = m[1] - kKv4Bias;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const float pa0 = ex2(s[u][0] - (m[0] - kKv4Bias)), pa1 = ex2(s[u][1] - (m[1] - kKv4Bias));
-                const float pb0 = ex2(s[u][2] - (m[0] - kKv4Bias)), pb1 = ex2(s[u][3] - (m[1] - kKv4Bias));
+                const float pa0 = ex2(s[u][0] - from0), pa1 = ex2(s[u][1] - from1), pb0 = ex2(s[u][2] - from0), pb1 = ex2(s[u][3] - from1);
                 l[0] += pa0 + pb0, l[1] += pa1 + pb1;
+                uint4 sa = lds128(vs_src + 16 * u * kKv4Scales), sb = lds128(vs_src + (16 * u + 8) * kKv4Scales);
+                if (left < kKv4Tile) {
+                    if (16 * u + my_row >= left) sa = make_uint4(0u, 0u, 0u, 0u);
+                    if (16 * u + 8 + my_row >= left) sb = make_uint4(0u, 0u, 0u, 0u);
+                }
                 const uint32_t at_v = v_src + (16 * u + t) * kKv4Codes + 8 * g;
                 const uint2 v0 = lds64(at_v), v1 = lds64(at_v + 4 * kKv4Codes), v2 = lds64(at_v + 8 * kKv4Codes), v3 = lds64(at_v + 12 * kKv4Codes);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
+                    const float2 fa = __half22float2(u32_as_half2(j == 0 ? sa.x : j == 1 ? sa.y : j == 2 ? sa.z : sa.w));
+                    const float2 fb = __half22float2(u32_as_half2(j == 0 ? sb.x : j == 1 ? sb.y : j == 2 ? sb.z : sb.w));
                     const uint32_t sel = (j & 1) ? 0x7632u : 0x5410u;
-                    const uint32_t b0 = transpose8(half2_as_u32(__floats2half2_rn(pa0 * va[u][j].x, pa1 * va[u][j].x)));
-                    const uint32_t b1 = transpose8(half2_as_u32(__floats2half2_rn(pb0 * vb[u][j].x, pb1 * vb[u][j].x)));
+                    const uint32_t b0 = transpose8(half2_as_u32(__floats2half2_rn(pa0 * fa.x, pa1 * fa.x)));
+                    const uint32_t b1 = transpose8(half2_as_u32(__floats2half2_rn(pb0 * fb.x, pb1 * fb.x)));
                     const uint32_t w0 = j < 2 ? prmt(v0.x, v1.x, sel) : prmt(v0.y, v1.y, sel), w1 = j < 2 ? prmt(v2.x, v3.x, sel) : prmt(v2.y, v3.y, sel);
                     mma_16816(o[2 * j], w0 & kLow, w0 & kHigh, w1 & kLow, w1 & kHigh, b0, b1);
                     mma_16816(o[2 * j + 1], (w0 >> 8) & kLow, (w0 >> 8) & kHigh, (w1 >> 8) & kLow, (w1 >> 8) & kHigh, b0, b1);
                     mma_16816(ones[j], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, b0, b1);
-                    low[j][0] = fmaf(pa0, va[u][j].y, fmaf(pb0, vb[u][j].y, low[j][0]));
-                    low[j][1] = fmaf(pa1, va[u][j].y, fmaf(pb1, vb[u][j].y, low[j][1]));
+                    const float mid_a = fmaf(8.f, fa.x, fa.y), mid_b = fmaf(8.f, fb.x, fb.y);
+                    low[j][0] = fmaf(pa0, mid_a, fmaf(pb0, mid_b, low[j][0]));
+                    low[j][1] = fmaf(pa1, mid_a, fmaf(pb1, mid_b, low[j][1]));
                 }
             }
             __syncwarp();                            // the stage is free

@@ -11,7 +11,7 @@
 //   O += P V             tcgen05.mma with P in tensor memory, V in shared memory as it lies (N-major), O in tensor memory (fp32)
 // The two halves alternate: the tensor core works on one while the other's softmax runs.  m follows the true maximum with a slack of 2^8: only a larger step
 // rescales O and l (by the thread that owns the row; the scores' barrier says that the product before has been added).  exp2 of differences up to 8 stays far inside fp16 and fp32.
-// Warps 0-3 and 4-7: softmax and output of the halves; 8: MMA issue; 9: TMA loads (ring of key and value tiles); 10: the list of items.
+// Warps 0-3 and 4-7: softmax and output of the halves; 8: MMAs; 9: TMA loads (ring of key and value tiles); 10: the list of items.
 // Masks are applied to tiles that reach beyond a half's first row only.  Value rows behind the last key are zeroed in shared memory: a weight of 0 times whatever
 // lies there has to be 0.
 // Items go to CTAs longest first, there and back again (the longest of a round meets the shortest of the next): the order is worked out from
@@ -22,7 +22,10 @@
 
 namespace rptc {
 
-constexpr int kPromptThreads = 352, kPromptMmaWarp = 8, kPromptLoadWarp = 9, kPromptListWarp = 10;
+constexpr int kPromptThreads = 384, kPromptMmaWarp = 8, kPromptLoadWarp = 9, kPromptListWarp = 10;
+// 384 threads are launched with 168 registers each, 64512 in all: the same as 256 with 216 and 128 with 72.
+constexpr int kPromptSoftmaxRegs = 216, kPromptOtherRegs = 72;
+static_assert(256 * kPromptSoftmaxRegs + 128 * kPromptOtherRegs <= 384 * 168, "registers that the block is launched with");
 constexpr int kPromptReaders = 10;                   // warps that take items off the list
 constexpr uint32_t kPromptPanel = 128 * 128;         // 128 rows of 64 values
 constexpr int kTileKeys = 128;
@@ -32,7 +35,7 @@ struct PromptParams {
     uint16_t *out;
     const int32_t *starts, *kv_first, *kv_len;
     int64_t tokens, kv_tokens, out_row, out_head;
-    int32_t sequences, group, pack, kv_heads;
+    int32_t sequences, group, pack, kv_heads, wide;      // wide: rows and heads of out on 32-byte boundaries
     float scale;                                     // includes log2(e)
     unsigned int *status;
 };
@@ -52,13 +55,13 @@ __device__ __forceinline__ Sequence sequence(const PromptParams &p, int s) {
     if (r.q0 != a || r.n != b - a || r.k0 != k0 || r.m != m) atomicExch(p.status, kStatusPosition);
     return r;
 }
-// How many items of a sequence take at least c tiles of keys (its last ones; all take one).
-__device__ __forceinline__ int items_of(const Sequence &s, int tokens_per_item, int c) {
-    const int all = (s.n + tokens_per_item - 1) / tokens_per_item;
+// How many items of a sequence, of 2^shift tokens each, take at least c tiles of keys (its last ones; all take one).
+__device__ __forceinline__ int items_of(const Sequence &s, int shift, int c) {
+    const int all = (s.n + (1 << shift) - 1) >> shift;
     if (c <= 1 || all == 0) return all;
     const int reach = kTileKeys * (c - 1);           // an item takes c tiles when its last query sees more keys than these
     if (s.m <= reach) return 0;
-    const int first = max(0, reach - (s.m - s.n)) / tokens_per_item;
+    const int first = max(0, reach - (s.m - s.n)) >> shift;
     return all - min(first, all - 1);
 }
 
@@ -67,39 +70,60 @@ struct PromptItem {
     int32_t pad[2];
 };
 
-// Item number `index` of all, by one warp.
-__device__ __forceinline__ PromptItem find_item(const PromptParams &p, int64_t index, int most, int lane) {
-    const int per_item = 256 / p.pack, groups = p.kv_heads * (p.group / p.pack);
-    const int rank = (int)(index / groups), heads = (int)(index - (int64_t)rank * groups);
-    auto count = [&](int c) {
-        int n = 0;
-        for (int s = lane; s < p.sequences; s += 32) n += items_of(sequence(p, s), per_item, c);
-        return __reduce_add_sync(0xFFFFFFFFu, n);
-    };
-    int lo = 1, hi = most;                           // the largest c of which there are more than `rank`
-    while (lo < hi) {
-        const int mid = lo + (hi - lo + 1) / 2;
-        if (count(mid) > rank) lo = mid;
-        else hi = mid - 1;
+// The items in their order, by one warp.  A lane holds sequence number `lane`; those from 32 on are read again whenever they are counted.
+struct ItemList {
+    const PromptParams &p;
+    int lane, shift, groups, most;                   // most: tiles of the longest item
+    uint32_t total;
+    Sequence mine;
+    __device__ __forceinline__ ItemList(const PromptParams &params, int l) : p(params), lane(l) {
+        shift = 8 - (31 - __clz(p.pack));
+        groups = p.kv_heads * p.group / p.pack;
+        mine = {0, 0, 0, 0};
+        if (lane < p.sequences) mine = sequence(p, lane);
+        most = mine.n > 0 ? (mine.m + kTileKeys - 1) / kTileKeys : 1;
+        for (int s = lane + 32; s < p.sequences; s += 32)
+            if (const Sequence q = sequence(p, s); q.n > 0) most = max(most, (q.m + kTileKeys - 1) / kTileKeys);
+        most = max(1, __reduce_max_sync(0xFFFFFFFFu, most));
+        total = (uint32_t)count(1) * groups;         // at most 2^28 for the rows and 2^28 for the sequences
     }
-    int left = rank - count(lo + 1);
-    PromptItem it = {};
-    for (int s0 = 0; s0 < p.sequences; s0 += 32) {
-        Sequence q = {0, 0, 0, 0};
-        if (s0 + lane < p.sequences) q = sequence(p, s0 + lane);
-        const int from = items_of(q, per_item, lo), mine = from - items_of(q, per_item, lo + 1);
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-            if (lane >= o) upto += v;
+    __device__ __forceinline__ int count(int c) const {
+        int n = items_of(mine, shift, c);
+        for (int s = lane + 32; s < p.sequences; s += 32) n += items_of(sequence(p, s), shift, c);
+        return __reduce_add_sync(0xFFFFFFFFu, n);
+    }
+    __device__ __forceinline__ PromptItem item(uint32_t index) const {
+        const int per_item = 1 << shift, rank = (int)(index / (uint32_t)groups), heads = (int)(index - (uint32_t)rank * groups);
+        int lo = 1, hi = most;                       // the largest c of which there are more than `rank`
+        while (lo < hi) {
+            const int mid = lo + (hi - lo + 1) / 2;
+            if (count(mid) > rank) lo = mid;
+            else hi = mid - 1;
         }
-        const unsigned hit = __ballot_sync(0xFFFFFFFFu, left < upto);
-        if (hit) {
-            const int all = (q.n + per_item - 1) / per_item, j = all - from + left - (upto - mine);
+        int left = rank - count(lo + 1);
+        PromptItem it = {};
+        for (int s0 = 0; s0 < p.sequences; s0 += 32) {
+            Sequence q = mine;
+            if (s0 > 0) q = s0 + lane < p.sequences ? sequence(p, s0 + lane) : Sequence{0, 0, 0, 0};
+            const int from = items_of(q, shift, lo), here = from - items_of(q, shift, lo + 1);
+            int upto = here;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                if (lane >= o) upto += v;
+            }
+            const unsigned hit = __ballot_sync(0xFFFFFFFFu, left < upto);
+            if (hit == 0) {
+                left -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+                continue;
+            }
+            const int in = __ffs(hit) - 1, j = __shfl_sync(0xFFFFFFFFu, ((q.n + per_item - 1) >> shift) - from + left - (upto - here), in);
+            q.q0 = __shfl_sync(0xFFFFFFFFu, q.q0, in), q.n = __shfl_sync(0xFFFFFFFFu, q.n, in);
+            q.k0 = __shfl_sync(0xFFFFFFFFu, q.k0, in), q.m = __shfl_sync(0xFFFFFFFFu, q.m, in);
+            const int splits = p.group / p.pack;
             it.go = 1;
-            it.kv_head = heads / (p.group / p.pack);
-            it.head = it.kv_head * p.group + (heads % (p.group / p.pack)) * p.pack;
+            it.kv_head = heads / splits;
+            it.head = it.kv_head * p.group + (heads - it.kv_head * splits) * p.pack;
             it.token = q.q0 + j * per_item;
             it.tokens = min(per_item, q.n - j * per_item);
             it.k0 = q.k0, it.keys = q.m;
@@ -107,21 +131,29 @@ __device__ __forceinline__ PromptItem find_item(const PromptParams &p, int64_t i
             const int last0 = it.seen + min(it.tokens, per_item / 2), last1 = it.seen + it.tokens;      // keys that a half's last query sees
             it.tiles0 = max(0, (last0 + kTileKeys - 1) / kTileKeys);
             it.tiles1 = it.tokens > per_item / 2 ? max(0, (last1 + kTileKeys - 1) / kTileKeys) : 0;
-            const int from_lane = __ffs(hit) - 1;
-            int *w = reinterpret_cast<int *>(&it);
-#pragma unroll
-            for (int i = 0; i < 10; ++i) w[i] = __shfl_sync(0xFFFFFFFFu, w[i], from_lane);
-            return it;
+            break;
         }
-        left -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+        return it;
     }
-    return it;                                       // not reached: the index is below the number of items
-}
+};
 
+// mbar_wait without a call: a function called from here would have to make do with the fewest registers that any warp of the kernel has.
+__device__ __forceinline__ bool await(uint32_t bar, uint32_t parity, unsigned int *status) {
+#pragma unroll 1
+    for (uint32_t spin = 0; spin < kSpinLimit; ++spin)
+        if (mbar_try_wait(bar, parity)) return true;
+    atomicExch(status, kStatusWaitExpired);
+    return false;
+}
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -141,12 +173,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
     const uint32_t base = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t bars = base, q_addr = base + 1024u, ring = q_addr + 2 * kTile;
     const uint32_t q_full = bars, q_empty = bars + 8, full = bars + 16, empty = full + 8 * kStages, s_full = empty + 8 * kStages, p_full = s_full + 16,
-                   o_full = p_full + 16, item_full = o_full + 16, item_empty = item_full + 16, tmem_slot = item_empty + 16, items = bars + 256;
+                   o_full = p_full + 32, item_full = o_full + 16, item_empty = item_full + 16, tail = item_empty + 16, tmem_slot = tail + 8, items = bars + 256;
     if (tid == 0) {
-        mbar_init(q_full, 1), mbar_init(q_empty, 1);
+        mbar_init(q_full, 1), mbar_init(q_empty, 1), mbar_init(tail, 1);
         for (int i = 0; i < kStages; ++i) mbar_init(full + 8 * i, 1), mbar_init(empty + 8 * i, 1);
         for (int i = 0; i < 2; ++i) {
-            mbar_init(s_full + 8 * i, 1), mbar_init(p_full + 8 * i, 4), mbar_init(o_full + 8 * i, 1);
+            mbar_init(s_full + 8 * i, 1), mbar_init(o_full + 8 * i, 1);
+            mbar_init(p_full + 16 * i, 4), mbar_init(p_full + 16 * i + 8, 4);
             mbar_init(item_full + 8 * i, 1), mbar_init(item_empty + 8 * i, kPromptReaders);
         }
         mbar_fence_init();
@@ -155,10 +188,47 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    pdl_allow_next_grid();
+    auto set_up = [&]() {
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        pdl_allow_next_grid();
+    };
+    if (warp == kPromptListWarp) {                   // the first item is found while the others set up
+        pdl_wait_prior_grids();
+        PromptParams q = p;
+        q.starts = after_wait(p.starts), q.kv_first = after_wait(p.kv_first), q.kv_len = after_wait(p.kv_len);
+        const ItemList items_in_order(q, lane);
+        const uint32_t total = items_in_order.total;
+        PromptItem next = {};
+        if (blockIdx.x < total) next = items_in_order.item(blockIdx.x);
+        set_up();
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptOtherRegs));
+        RingPos list = {0, 0u};
+        bool ok = true;
+        for (uint32_t round = 0;;) {
+            ok = ok && await(item_empty + 8 * list.s, list.phase ^ 1u, p.status);
+            if (!__all_sync(0xFFFFFFFFu, ok)) break;
+            if (lane == 0) {
+                const uint32_t at = items + 64u * list.s;
+                const int *w = reinterpret_cast<const int *>(&next);
+#pragma unroll
+                for (int i = 0; i < 12; ++i) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + 4u * i), "r"(w[i]) : "memory");
+                mbar_arrive(item_full + 8 * list.s);
+            }
+            __syncwarp();
+            list.advance(2);
+            if (!next.go) break;                     // the end of the list
+            next = {};
+            uint32_t index = total;
+            while (++round * gridDim.x < total) {    // there and back; the last round may not be full
+                index = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                if (index < total) break;
+            }
+            if (index < total) next = items_in_order.item(index);
+        }
+    }
+    if (warp != kPromptListWarp) set_up();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, lds32(tmem_slot), 0);
     const int rows_per_token = p.pack, half_tokens = 128 / rows_per_token;
     bool ok = true;
@@ -166,7 +236,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
     // the next item off the list; false at its end
     RingPos list = {0, 0u};
     auto next_item = [&](PromptItem &it) {
-        ok = ok && mbar_wait(item_full + 8 * list.s, list.phase, p.status);
+        ok = ok && await(item_full + 8 * list.s, list.phase, p.status);
         if (!__all_sync(0xFFFFFFFFu, ok)) {
             ok = false;
             return false;
@@ -184,24 +254,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
 
     PromptItem it;
     if (warp < 8) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kPromptSoftmaxRegs));
         // ================= softmax and output of one half: a thread owns a row =================
         const int half = warp >> 2, row = (warp & 3) * 32 + lane, my_token = half * half_tokens + row / rows_per_token, my_head = row % rows_per_token;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_tmem = tmem + 128u * half + lanes, o_tmem = tmem + 256u + 128u * half + lanes;
-        const uint32_t my_s = s_full + 8 * half, my_p = p_full + 8 * half;
+        const uint32_t my_s = s_full + 8 * half, my_p = p_full + 16 * half;
         uint32_t phase = 0u, o_phase = 0u;
         while (next_item(it)) {
             const int tiles = half ? it.tiles1 : it.tiles0, first_seen = it.seen + half * half_tokens;
             const int last = min(it.seen + my_token, it.keys - 1);                  // the last key that this row sees
             float m = -INFINITY, l = 0.f;                                           // m: in units of the scores
             for (int i = 0; i < tiles && ok; ++i) {
-                ok = mbar_wait(my_s, phase, p.status);
+                ok = await(my_s, phase, p.status);
                 phase ^= 1u;
                 if (!__all_sync(0xFFFFFFFFu, ok)) {
                     ok = false;
                     break;
                 }
                 tc_fence_after();
-                uint32_t s[128];
+                uint32_t s[128], w[32];
                 tmem_load64(s_tmem, *reinterpret_cast<uint32_t(*)[64]>(s));
                 tmem_load64(s_tmem + 64u, *reinterpret_cast<uint32_t(*)[64]>(s + 64));
                 if (i * kTileKeys + kTileKeys - 1 > first_seen || i * kTileKeys + kTileKeys > it.keys) {
@@ -213,7 +284,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
 #pragma unroll
                 for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(s[c]);
 #pragma unroll
-                for (int c = 4; c < 128; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
+                for (int c = 4; c < 124; c += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1]));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[124 + e]));
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                 if (i == 0) {
                     m = top == -INFINITY ? 0.f : top;                               // a row that sees nothing has weights of 0
@@ -233,27 +308,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
                         }
                     }
                 }
-                const float shift = -m * p.scale;
-                float sum[2] = {0.f, 0.f};
+                const f32x2 scale2 = pack2(p.scale, p.scale), shift2 = pack2(-m * p.scale, -m * p.scale);
+                f32x2 sum[4];
 #pragma unroll
-                for (int c = 0; c < 128; c += 64) {
-                    uint32_t w[32];
+                for (int c = 0; c < 2; ++c) {                                       // 64 keys: the product takes them while the next are made
 #pragma unroll
                     for (int e = 0; e < 32; ++e) {
-                        const float a = exp2_fast(fmaf(__uint_as_float(s[c + 2 * e]), p.scale, shift)), b = exp2_fast(fmaf(__uint_as_float(s[c + 2 * e + 1]), p.scale, shift));
-                        sum[0] += a, sum[1] += b;
-                        w[e] = pack16<BF16>(a, b);
+                        float x, y;
+                        unpack2(fma2(pack2(__uint_as_float(s[64 * c + 2 * e]), __uint_as_float(s[64 * c + 2 * e + 1])), scale2, shift2), x, y);
+                        x = exp2_fast(x), y = exp2_fast(y);
+                        sum[e & 3] = c == 0 && e < 4 ? pack2(x, y) : add2(sum[e & 3], pack2(x, y));
+                        w[e] = pack16<BF16>(x, y);
                     }
-                    tmem_store32_begin(s_tmem + (uint32_t)(c / 2), w);
+                    tmem_store32_begin(s_tmem + 32u * c, w);
+                    tmem_store_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(my_p + 8 * c);
                 }
-                l += sum[0] + sum[1];
-                tmem_store_wait();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(my_p);
+                float x, y;
+                unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), x, y);
+                l += x + y;
             }
             if (tiles > 0) {                                                        // the last product has been added
-                ok = ok && mbar_wait(o_full + 8 * half, o_phase, p.status);
+                ok = ok && await(o_full + 8 * half, o_phase, p.status);
                 o_phase ^= 1u;
                 if (!__all_sync(0xFFFFFFFFu, ok)) {
                     ok = false;
@@ -275,111 +353,142 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
                 }
                 if (!there) continue;
 #pragma unroll
-                for (int e = 0; e < 32; e += 8) {
-                    uint32_t w[4];
+                for (int e = 0; e < 32; e += 16) {
+                    uint32_t w[8];
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
+                    for (int q = 0; q < 8; ++q) {
                         const float a = __uint_as_float(o[e + 2 * q]) * inv, b = __uint_as_float(o[e + 2 * q + 1]) * inv;
                         w[q] = inv == 0.f ? 0u : pack16<BF16>(a, b);
                     }
-                    *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (p.wide) {
+                        st_32_bytes(out + c + e, w);
+                    } else {
+                        *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                        *reinterpret_cast<uint4 *>(out + c + e + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                    }
                 }
             }
             tc_fence_before();
         }
     } else if (warp == kPromptMmaWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptOtherRegs));
         // ================= MMA issue: the whole warp waits, one lane issues =================
+        // One warp for both halves: the order of issue keeps them half a tile apart.  (Two warps: their MMAs interleave, both halves' softmax runs at the same time and
+        // the tensor core waits for it.)  What a tile needs besides the weights is waited for under the tile before.
         RingPos pos = {0, 0u};
-        uint32_t q_phase = 0u, p_phase = 0u;                                        // p_phase: bit h for half h
+        uint32_t q_phase = 0u, p_phase[2] = {0u, 0u};
         const uint32_t idesc_s = instr_desc(kTileKeys) | (BF16 ? kInstrBf16 : 0u), idesc_o = instr_desc(DP * 64) | (BF16 ? kInstrBf16 : 0u) | kInstrBMajorN;
+        const uint64_t q_desc = umma_desc_sw128(q_addr), k_desc = umma_desc_sw128(ring), v_desc = umma_desc_sw128_mn(ring, kPromptPanel);
+        const bool issues = elect_one();
+        auto scores = [&](uint32_t half, uint32_t stage) {                          // S = Q K^T
+            const uint64_t q = q_desc + half * (kTile >> 4), k = k_desc + stage * (kTile >> 4);
+#pragma unroll
+            for (uint32_t c = 0; c < 4 * DP; ++c) {
+                const uint32_t off = ((c >> 2) * kPromptPanel + (c & 3u) * 32u) >> 4;
+                tc_mma_f16(tmem + 128u * half, q + off, k + off, idesc_s, c != 0);
+            }
+            tc_commit(s_full + 8 * half);
+        };
+        auto take = [&]() {                                                         // the next stage of the ring, full
+            const uint32_t stage = pos.s;
+            ok = ok && await(full + 8 * stage, pos.phase, p.status);
+            pos.advance(kStages);
+            return stage;
+        };
         while (next_item(it)) {
             const int tiles = max(it.tiles0, it.tiles1);
             if (tiles == 0) continue;
-            auto scores = [&](int h, uint32_t k_addr) {                             // by the elected lane
-#pragma unroll
-                for (uint32_t c = 0; c < 4 * DP; ++c) {
-                    const uint32_t off = (c >> 2) * kPromptPanel + (c & 3u) * 32u;
-                    tc_mma_f16(tmem + 128u * h, umma_desc_sw128(q_addr + h * kTile + off), umma_desc_sw128(k_addr + off), idesc_s, c != 0);
-                }
-            };
-            {
-                const bool issues = elect_one();
-                ok = ok && mbar_wait(q_full, q_phase, p.status) && mbar_wait(full + 8 * pos.s, pos.phase, p.status);
-                q_phase ^= 1u;
-                tc_fence_after();
-                if (issues && ok) {
-                    if (it.tiles0 > 0) scores(0, ring + pos.s * kTile), tc_commit(s_full);
-                    if (it.tiles1 > 0) scores(1, ring + pos.s * kTile), tc_commit(s_full + 8);
-                    tc_commit(empty + 8 * pos.s);
-                    if (tiles == 1) tc_commit(q_empty);
-                }
-                __syncwarp();
-                pos.advance(kStages);
+            ok = ok && await(q_full, q_phase, p.status);
+            q_phase ^= 1u;
+            uint32_t k_stage = take();
+            tc_fence_after();
+            if (issues && ok) {
+                if (it.tiles0 > 0) scores(0, k_stage);
+                if (it.tiles1 > 0) scores(1, k_stage);
+                tc_commit(empty + 8 * k_stage);
+                if (tiles == 1) tc_commit(q_empty);
             }
+            uint32_t v_stage = take();
+            if (tiles > 1) k_stage = take();
+#pragma unroll 1
             for (int i = 0; i < tiles; ++i) {
-                const uint32_t v_stage = pos.s;
-                ok = ok && mbar_wait(full + 8 * pos.s, pos.phase, p.status);
-                const int rows = it.keys - i * kTileKeys;
-                if (rows < kTileKeys) {                                             // rows behind the last key
-                    const uint32_t v_addr = ring + v_stage * kTile;
-                    for (int x = lane; x < (kTileKeys - rows) * 8 * DP; x += 32) {
-                        const int r = rows + x / (8 * DP), piece = x % (8 * DP);
-                        asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(v_addr + (piece >> 3) * kPromptPanel + r * 128u + (piece & 7) * 16u), "r"(0u) : "memory");
-                    }
-                    fence_proxy_async_smem();
-                    __syncwarp();
-                }
-                pos.advance(kStages);
-                const bool more = i + 1 < tiles;
-                const uint32_t k_stage = pos.s;
-                if (more) {
-                    ok = ok && mbar_wait(full + 8 * pos.s, pos.phase, p.status);
-                    pos.advance(kStages);
-                }
+                uint32_t v_next = 0, k_next = 0;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
+                for (uint32_t h = 0; h < 2; ++h) {
                     const int mine = h ? it.tiles1 : it.tiles0;
-                    if (i >= mine) continue;
-                    const bool issues = elect_one();
-                    ok = ok && mbar_wait(p_full + 8 * h, (p_phase >> h) & 1u, p.status);
-                    p_phase ^= 1u << h;
-                    tc_fence_after();
-                    if (issues && ok) {
+                    if (i < mine) {
+                        const uint64_t v = v_desc + v_stage * (kTile >> 4);
+                        const uint32_t o_tmem = tmem + 256u + 128u * h, w_tmem = tmem + 128u * h;
+                        ok = ok && await(p_full + 16 * h, p_phase[h], p.status);
+                        tc_fence_after();
+                        if (issues && ok) {                                         // O += P V, 64 keys at a time
 #pragma unroll
-                        for (uint32_t c = 0; c < kTileKeys / 16; ++c)
-                            tc_mma_f16_ta(tmem + 256u + 128u * h, tmem + 128u * h + 8u * c, umma_desc_sw128_mn(ring + v_stage * kTile + 2048u * c, kPromptPanel), idesc_o,
-                                          (uint32_t)(i | c) != 0u);
-                        // a barrier of its own for the finished sums: the next item's first scores may follow before the softmax warps have looked
-                        if (i + 1 < mine) scores(h, ring + k_stage * kTile), tc_commit(s_full + 8 * h);
-                        else tc_commit(o_full + 8 * h);
+                            for (uint32_t c = 0; c < 4; ++c) tc_mma_f16_ta(o_tmem, w_tmem + 8u * c, v + 128u * c, idesc_o, (uint32_t)(i | c) != 0u);
+                        }
+                        ok = ok && await(p_full + 16 * h + 8, p_phase[h], p.status);
+                        p_phase[h] ^= 1u;
+                        tc_fence_after();
+                        if (issues && ok) {
+#pragma unroll
+                            for (uint32_t c = 4; c < 8; ++c) tc_mma_f16_ta(o_tmem, w_tmem + 8u * c, v + 128u * c, idesc_o, 1u);
+                            // a barrier of its own for the finished sums: the next item's first scores may follow before the softmax warps have looked
+                            if (i + 1 < mine) scores(h, k_stage);
+                            else tc_commit(o_full + 8 * h);
+                        }
                     }
-                    __syncwarp();
+                    if (h == 0 && i + 1 < tiles) {
+                        v_next = take();
+                        if (i + 2 < tiles) k_next = take();
+                    }
                 }
-                if (elect_one() && ok) {
+                if (issues && ok) {
                     tc_commit(empty + 8 * v_stage);
-                    if (more) tc_commit(empty + 8 * k_stage);
+                    if (i + 1 < tiles) tc_commit(empty + 8 * k_stage);
                     if (i + 2 == tiles) tc_commit(q_empty);
                 }
-                __syncwarp();
+                v_stage = v_next, k_stage = k_next;
             }
         }
     } else if (warp == kPromptLoadWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptOtherRegs));
         // ================= loads =================
         pdl_wait_prior_grids();
         if (lane == 0) tma_prefetch_map(&q_map), tma_prefetch_map(&k_map), tma_prefetch_map(&v_map);
         RingPos pos = {0, 1u};
-        uint32_t q_phase = 1u;
+        uint32_t q_phase = 1u, tail_phase = 0u;
         int64_t loads = 0;
-        auto load_tile = [&](const CUtensorMap *map, int tile) {
+        auto load_tile = [&](const CUtensorMap *map, int tile, uint32_t bar) {
             const bool issues = elect_one();
-            ok = ok && mbar_wait(empty + 8 * pos.s, pos.phase, p.status);
+            ok = ok && await(empty + 8 * pos.s, pos.phase, p.status);
             loads += __all_sync(0xFFFFFFFFu, ok) ? 1 : 0;
             if (issues && ok) {
-                mbar_expect_tx(full + 8 * pos.s, kTile);
+                mbar_expect_tx(bar, kTile);
 #pragma unroll
-                for (int d = 0; d < DP; ++d) tma_load_3d(ring + pos.s * kTile + d * kPromptPanel, map, 64 * d, it.kv_head, it.k0 + tile * kTileKeys, full + 8 * pos.s);
+                for (int d = 0; d < DP; ++d) tma_load_3d(ring + pos.s * kTile + d * kPromptPanel, map, 64 * d, it.kv_head, it.k0 + tile * kTileKeys, bar);
             }
             __syncwarp();
+        };
+        auto load_values = [&](int tile) {
+            const int rows = it.keys - tile * kTileKeys;
+            if (rows >= kTileKeys) {
+                load_tile(&v_map, tile, full + 8 * pos.s);
+            } else {                                                                // the last: rows behind the last key become zeros before anyone reads them
+                load_tile(&v_map, tile, tail);
+                ok = ok && await(tail, tail_phase, p.status);
+                tail_phase ^= 1u;
+                for (int x = lane; x < (kTileKeys - rows) * 8 * DP; x += 32) {
+                    const int r = rows + x / (8 * DP), piece = x % (8 * DP);
+                    asm volatile("st.shared.v4.u32 [%0], {%1,%1,%1,%1};" ::"r"(ring + pos.s * kTile + (piece >> 3) * kPromptPanel + r * 128u + (piece & 7) * 16u), "r"(0u)
+                                 : "memory");
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (elect_one() && ok) mbar_arrive(full + 8 * pos.s);
+            }
+            pos.advance(kStages);
+        };
+        auto load_keys = [&](int tile) {
+            load_tile(&k_map, tile, full + 8 * pos.s);
             pos.advance(kStages);
         };
         while (next_item(it)) {
@@ -387,7 +496,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
             if (tiles == 0) continue;
             {
                 const bool issues = elect_one();
-                ok = ok && mbar_wait(q_empty, q_phase, p.status);
+                ok = ok && await(q_empty, q_phase, p.status);
                 q_phase ^= 1u;
                 if (issues && ok) {
                     mbar_expect_tx(q_full, (it.tiles1 > 0 ? 2u : 1u) * kTile);
@@ -398,54 +507,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
                 }
                 __syncwarp();
             }
-            load_tile(&k_map, 0);
+            load_keys(0);
             for (int i = 0; i < tiles; ++i) {
-                if (i + 1 < tiles) {
-                    load_tile(&v_map, i);
-                    load_tile(&k_map, i + 1);
-                } else {
-                    load_tile(&v_map, i);
-                }
+                load_values(i);
+                if (i + 1 < tiles) load_keys(i + 1);
             }
         }
         if (!__all_sync(0xFFFFFFFFu, ok)) {                                         // copies in flight land before the CTA leaves
             for (int i = 0; i < kStages; ++i)
-                if (const int64_t n = (loads - i + kStages - 1) / kStages; loads > i) mbar_wait(full + 8 * i, (uint32_t)(n - 1) & 1u, p.status);
+                if (const int64_t n = (loads - i + kStages - 1) / kStages; loads > i) await(full + 8 * i, (uint32_t)(n - 1) & 1u, p.status);
         }
-    } else {
-        // ================= the list of items =================
-        pdl_wait_prior_grids();
-        PromptParams q = p;
-        q.starts = after_wait(p.starts), q.kv_first = after_wait(p.kv_first), q.kv_len = after_wait(p.kv_len);
-        const int per_item = 256 / p.pack;
-        int all = 0, most = 1;
-        for (int s = lane; s < p.sequences; s += 32) {
-            const Sequence seq = sequence(q, s);
-            all += items_of(seq, per_item, 1);
-            if (seq.n > 0) most = max(most, (seq.m + kTileKeys - 1) / kTileKeys);
-        }
-        all = __reduce_add_sync(0xFFFFFFFFu, all);
-        most = __reduce_max_sync(0xFFFFFFFFu, most);
-        const int64_t total = (int64_t)all * p.kv_heads * (p.group / p.pack);
-        int64_t round = 0;
-        for (bool go = true; go; ++round) {
-            const int64_t index = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-            go = round * gridDim.x < total;
-            if (go && index >= total) continue;                                     // the last round is not full
-            PromptItem next = {};
-            if (go) next = find_item(q, index, most, lane);
-            ok = ok && mbar_wait(item_empty + 8 * list.s, list.phase ^ 1u, p.status);
-            if (!__all_sync(0xFFFFFFFFu, ok)) break;
-            if (lane == 0) {
-                const uint32_t at = items + 64u * list.s;
-                const int *w = reinterpret_cast<const int *>(&next);
-#pragma unroll
-                for (int i = 0; i < 12; ++i) asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + 4u * i), "r"(w[i]) : "memory");
-                mbar_arrive(item_full + 8 * list.s);
-            }
-            __syncwarp();
-            list.advance(2);
-        }
+    } else if (warp != kPromptListWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPromptOtherRegs));      // a warp of the third group with nothing to do
     }
     tc_fence_before();
     __syncthreads();
@@ -491,6 +564,7 @@ extern "C" int rptc_attn_prompt(const rptc_prompt_attention *a, rptc_stream_t st
     p.sequences = (int32_t)a->sequences, p.group = a->heads / a->kv_heads, p.kv_heads = a->kv_heads;
     p.pack = p.group & -p.group;
     if (p.pack > 128) p.pack = 128;
+    p.wide = reinterpret_cast<uintptr_t>(a->out) % 32 == 0 && a->out_row % 16 == 0 && a->out_head % 16 == 0;
     p.scale = a->scale * 1.4426950408889634f;
     p.status = device_status_word();
     if (!p.status) return RPTC_ERR_CUDA;

@@ -185,6 +185,16 @@ __device__ __forceinline__ uint4 ldg128_stream(const void *p) {
                  : "l"(p));
     return v;
 }
+__device__ __forceinline__ void ld_32_bytes(const void *p, uint32_t (&r)[8]) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "l"(p));
+}
+__device__ __forceinline__ void st_32_bytes(void *p, const uint32_t (&r)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
+                 "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 // Loads of data that a prior grid writes.  Volatile asm with a memory clobber: they stay behind griddepcontrol.wait,
 // whereas the compiler may hoist a plain (or __ldg) load through a const __restrict__ pointer above the wait.
 __device__ __forceinline__ uint4 ld_ordered_u128(const void *p) {

@@ -168,16 +168,6 @@ struct Far16 {
         for (int k = 0; k < 16; ++k) v[k] = at[(k >> 1) & 3][16 * k];
     }
 };
-__device__ __forceinline__ void ld_32_bytes(const void *p, uint32_t (&r)[8]) {
-    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-                 : "l"(p));
-}
-__device__ __forceinline__ void st_32_bytes(void *p, const uint32_t (&r)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]),
-                 "r"(r[6]), "r"(r[7])
-                 : "memory");
-}
 __device__ __forceinline__ void unpack_pairs(const uint32_t (&r)[8], float (&v)[16]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
