@@ -150,11 +150,6 @@ __device__ __forceinline__ float exp2_fast(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
     uint32_t r;
@@ -280,16 +275,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
 #pragma unroll
                     for (int c = 0; c < 128; ++c) s[c] = c <= lim ? s[c] : 0xFF800000u;
                 }
-                float mx[4];
+                float mx[8];                                                        // (the three-operand maximum takes longer: 2048 tokens, 32 heads 41.9 us, 38.9 so)
 #pragma unroll
-                for (int c = 0; c < 4; ++c) mx[c] = __uint_as_float(s[c]);
+                for (int c = 0; c < 8; ++c) mx[c] = __uint_as_float(s[c]);
 #pragma unroll
-                for (int c = 4; c < 124; c += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(s[c + 2 * e]), __uint_as_float(s[c + 2 * e + 1]));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(s[124 + e]));
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                for (int c = 8; c < 128; ++c) mx[c & 7] = fmaxf(mx[c & 7], __uint_as_float(s[c]));
+                const float top = fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
                 if (i == 0) {
                     m = top == -INFINITY ? 0.f : top;                               // a row that sees nothing has weights of 0
                 } else {
