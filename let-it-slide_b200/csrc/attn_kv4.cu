@@ -10,13 +10,15 @@
 //            s = sum_g scale_g sum_g(q code) + min_g sum_g(q), the second sum as one more product, of the stored (scale, minimum) pairs with (0, sum_g(q)) in two
 //            fp16 parts.
 //   output   A = codes of 16 dims x 16 positions, B = p_j * scale_g in fp16 (one set per group; transposed from the scores' layout by movmatrix), and the same
-//            weights against a column of ones:  sum p scale (code - 8) + sum p (min + 8 scale).  Codes counted from the middle, so that what the weights' rounding
+//            weights against a constant -8:  sum p scale (code - 8) + sum p (min + 8 scale).  Codes counted from the middle, so that what the weights' rounding
 //            (2^-11, as that of P in any 16-bit product) is multiplied with is not larger than the values; the second sum is in fp32.
-// Weights refer to the running maximum of s + log2(the position's largest scale): the products p * scale then fit fp16 whatever the scales are (2^11 at most, 2^4 of slack above
-// it before anything is rescaled; what falls below 2^-14 is 2^-25 of the largest).
+// Weights refer to a running maximum of s + log2(a tile's largest scale): the products p * scale then fit fp16 whatever the scales are (2^11 where the reference was set, and
+// it moves only when they may pass 2^15, which their sum shows: no maximum is looked for otherwise; what falls below 2^-14 is 2^-25 of the largest).
 // Bound: HBM.  About 290 warp instructions per 16 positions (2560 bytes), two thirds of the issue slots at the measured copy rate.
 // Long contexts: all tiles of all rows and heads, laid end to end, are cut into equal ranges for the CTAs of one wave, so that rows of different lengths balance; a range's
 // part of a row goes to the workspace (fp32) and a second kernel joins the parts.  Short caches (max_pos up to kKv4Whole) take one CTA per row and head and no second kernel.
+#include <type_traits>
+
 #include "fwht.cuh"
 #include "kv4.cuh"
 #include "tc_ptx.cuh"
@@ -28,7 +30,7 @@ constexpr uint32_t kKv4StageBytes = 2 * kKv4Tile * (kKv4Codes + kKv4Scales);
 constexpr uint32_t kKv4Ring = kKv4Warps * kKv4Stages * kKv4StageBytes, kKv4Merge = kKv4Warps * 8 * 128 * 4, kKv4Smem = kKv4Ring + kKv4Merge + kKv4Warps * 8 * 8 + 256;
 constexpr int kKv4CtasPerSm = 2;
 constexpr int64_t kKv4Whole = 1024;
-constexpr float kKv4Bias = 11.f, kKv4Slack = 4.f;
+constexpr float kKv4Bias = 11.f;
 
 struct AttnKv4Params {
     const __half *q;
@@ -88,9 +90,23 @@ __device__ __forceinline__ void mma_first(float (&c)[4], uint32_t a0, uint32_t a
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+// Loads from shared memory at a constant distance from an address, which costs no addition.
+template <uint32_t OFF>
+__device__ __forceinline__ uint4 lds128_at(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4 + %5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr), "n"(OFF));
+    return v;
+}
+template <uint32_t OFF>
+__device__ __forceinline__ uint2 lds64_at(uint32_t addr) {
     uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2 + %3];" : "=r"(v.x), "=r"(v.y) : "r"(addr), "n"(OFF));
+    return v;
+}
+template <uint32_t OFF>
+__device__ __forceinline__ uint32_t lds32_at(uint32_t addr) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(v) : "r"(addr), "n"(OFF));
     return v;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -193,23 +209,24 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
         const int64_t cache_at = ((int64_t)row * p.hkv + kvh) * p.max_pos;
         const uint8_t *k = after_wait(p.k) + cache_at * kKv4Codes, *v = after_wait(p.v) + cache_at * kKv4Codes;
         const __half2 *ks = after_wait(p.k_scales) + cache_at * 4, *vs = after_wait(p.v_scales) + cache_at * 4;
-        auto fetch = [&](int tile, int stage) {      // by lane 0
-            const uint32_t n = (uint32_t)min(kKv4Tile, context - tile * kKv4Tile), dst = ring + (uint32_t)stage * kKv4StageBytes, bar = bars + 8u * stage;
-            const int64_t from = (int64_t)tile * kKv4Tile;
-            mbar_expect_tx(bar, 2 * n * (kKv4Codes + kKv4Scales));
-            bulk_g2s(dst, k + from * kKv4Codes, n * kKv4Codes, bar);
-            bulk_g2s(dst + kKv4Tile * kKv4Codes, ks + from * 4, n * kKv4Scales, bar);
-            bulk_g2s(dst + kKv4Tile * (kKv4Codes + kKv4Scales), v + from * kKv4Codes, n * kKv4Codes, bar);
-            bulk_g2s(dst + kKv4Tile * (2 * kKv4Codes + kKv4Scales), vs + from * 4, n * kKv4Scales, bar);
+        // Lanes 0 .. 3 copy the four pieces of a tile: codes and scales of k, of v.
+        const char *from = reinterpret_cast<const char *>(lane == 0 ? (const void *)k : lane == 1 ? (const void *)ks : lane == 2 ? (const void *)v : (const void *)vs);
+        const uint32_t size = (lane & 1) ? kKv4Scales : kKv4Codes;
+        const uint32_t piece = ring + (lane & 1) * kKv4Tile * kKv4Codes + ((lane >> 1) & 1) * kKv4Tile * (kKv4Codes + kKv4Scales);
+        auto fetch = [&](int tile, int stage) {
+            const uint32_t n = (uint32_t)min(kKv4Tile, context - tile * kKv4Tile), bar = bars + 8u * stage;
+            if (lane == 0) mbar_expect_tx(bar, 2 * n * (kKv4Codes + kKv4Scales));
+            __syncwarp();
+            if (lane < 4) bulk_g2s(piece + (uint32_t)stage * kKv4StageBytes, from + (int64_t)tile * kKv4Tile * size, n * size, bar);
         };
-        if (lane == 0) {
+        {
             int s = ring_pos.s;
             for (int i = 0; i < kKv4Stages; ++i, s = s + 1 == kKv4Stages ? 0 : s + 1)
                 if (t0 + warp + i * kKv4Warps < t1) fetch(t0 + warp + i * kKv4Warps, s);
         }
         // ---- q: this lane's operand values are those of q head g, dims 8 t .. 8 t + 7 of each group ----
         uint32_t qb[4][4], q_low[2];                 // q_low: (0, sum of q over group t) in two fp16 parts, against (scale, minimum) pairs
-        float code_unit[2], low_unit[2];             // of the q heads 2 t and 2 t + 1, whose scores this lane gets
+        float unit[2];                               // of the q heads 2 t and 2 t + 1, whose scores this lane gets
         {
             float x[4][8], big = 0.f, mine = 0.f;
 #pragma unroll
@@ -244,26 +261,25 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             const __half hi = __float2half_rn(mine);
             q_low[0] = half2_as_u32(__halves2half2(__float2half_rn(0.f), hi));
             q_low[1] = half2_as_u32(__halves2half2(__float2half_rn(0.f), __float2half_rn(mine - __half2float(hi))));
-            low_unit[0] = __shfl_sync(0xFFFFFFFFu, up, 8 * t), low_unit[1] = __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4);
-            code_unit[0] = low_unit[0] * 16777216.f, code_unit[1] = low_unit[1] * 16777216.f;
+            unit[0] = __shfl_sync(0xFFFFFFFFu, up, 8 * t), unit[1] = __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4);
         }
         // ---- this warp's tiles ----
-        float o[8][4] = {}, ones[4][4] = {}, low[4][2] = {}, l[2] = {0.f, 0.f}, m[2] = {-INFINITY, -INFINITY};
+        float o[8][4] = {}, low[4][2] = {}, l[2] = {0.f, 0.f}, m[2] = {-INFINITY, -INFINITY};
         const int my_row = (g >> 1) + 4 * (g & 1);   // the position of an operand's row g, so that the V operand's rows t and t + 4 are neighbours in the product
-        constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
+        constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u, kMinus8Low = 0x80088008u, kMinus8High = 0x80808080u;
+        constexpr uint32_t kC = kKv4Codes, kS = kKv4Scales, kKs = kKv4Tile * kC, kV = kKs + kKv4Tile * kS, kVs = kV + kKv4Tile * kC;      // in a stage
+        const uint32_t k_lane = ring + my_row * kC + 16 * t, s_lane = ring + my_row * kS, v_lane = ring + t * kC + 8 * g;
 #pragma unroll 1
         for (int tile = t0 + warp; tile < t1 && ok; tile += kKv4Warps) {
-            const uint32_t src = ring + (uint32_t)ring_pos.s * kKv4StageBytes, ks_src = src + kKv4Tile * kKv4Codes + my_row * kKv4Scales;
-            const uint32_t v_src = src + kKv4Tile * (kKv4Codes + kKv4Scales), vs_src = v_src + kKv4Tile * kKv4Codes + my_row * kKv4Scales;
+            const uint32_t stage = (uint32_t)ring_pos.s * kKv4StageBytes, k_src = k_lane + stage, s_src = s_lane + stage, v_src = v_lane + stage;
             ok = __all_sync(0xFFFFFFFFu, mbar_wait(bars + 8u * ring_pos.s, ring_pos.phase, p.status));
             const int left = context - tile * kKv4Tile;
             float s[2][4];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const uint32_t a = src + (16 * u + my_row) * kKv4Codes + 16 * t;
-                const uint4 xa = lds128(a), xb = lds128(a + 8 * kKv4Codes);
-                const uint4 sa = lds128(ks_src + 16 * u * kKv4Scales), sb = lds128(ks_src + (16 * u + 8) * kKv4Scales);
-                const uint32_t pa = lds32(ks_src + 16 * u * kKv4Scales + 4 * t), pb = lds32(ks_src + (16 * u + 8) * kKv4Scales + 4 * t);
+            auto scores = [&](auto half) {           // of sixteen positions
+                constexpr int u = decltype(half)::value;
+                const uint4 xa = lds128_at<16 * u * kC>(k_src), xb = lds128_at<(16 * u + 8) * kC>(k_src);
+                const uint4 sa = lds128_at<kKs + 16 * u * kS>(s_src), sb = lds128_at<kKs + (16 * u + 8) * kS>(s_src);
+                const uint32_t pa = lds32_at<kKs + 16 * u * kS>(s_src + 4 * t), pb = lds32_at<kKs + (16 * u + 8) * kS>(s_src + 4 * t);
                 float low_part[4], part[4];
                 mma_first(low_part, pa, pb, pa, pb, q_low[0], q_low[1]);
 #pragma unroll
@@ -281,54 +297,59 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                     part[3] = j ? fmaf(fb, c[3], part[3]) : fb * c[3];
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) s[u][i] = fmaf(part[i], code_unit[i & 1], low_part[i] * low_unit[i & 1]);
-            }
+                for (int i = 0; i < 4; ++i) s[u][i] = fmaf(part[i], 16777216.f, low_part[i]);      // in units of q's power of two and the scale
+            };
+            scores(std::integral_constant<int, 0>());
+            scores(std::integral_constant<int, 1>());
             if (left < kKv4Tile) {                   // positions behind the last: whatever the ring holds there
 #pragma unroll
                 for (int u = 0; u < 2; ++u)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) s[u][i] = 16 * u + 8 * (i >> 1) + my_row < left ? s[u][i] : -INFINITY;
             }
-            // ---- the running maximum of score + log2(the position's largest v scale) ----
-            float top[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                const uint4 r = lds128(vs_src + 8 * u * kKv4Scales);
-                const __half2 big = __hmax2(__hmax2(u32_as_half2(r.x), u32_as_half2(r.y)), __hmax2(u32_as_half2(r.z), u32_as_half2(r.w)));
-                const float lb = lg2(fmaxf(__low2float(big), 5.9604644775390625e-8f));
-                top[0] = fmaxf(top[0], s[u >> 1][2 * (u & 1)] + lb);
-                top[1] = fmaxf(top[1], s[u >> 1][2 * (u & 1) + 1] + lb);
+            // ---- weights; their reference moves when a product with the tile's largest v scale may pass 2^15 ----
+            float big;
+            {
+                const uint4 r = lds128_at<kVs>(ring + stage + lane * kS);
+                const uint32_t b = half2_as_u32(__hmax2(__hmax2(u32_as_half2(r.x), u32_as_half2(r.y)), __hmax2(u32_as_half2(r.z), u32_as_half2(r.w)))) & 0xFFFFu;
+                big = fmaxf(__half2float(__ushort_as_half((unsigned short)__reduce_max_sync(0xFFFFFFFFu, lane < left ? b : 0u))), 5.9604644775390625e-8f);
             }
+            float w[2][4], sum[2];
+            for (bool known = false;; known = true) {
+                const float from0 = kKv4Bias - m[0], from1 = kKv4Bias - m[1];
 #pragma unroll
-            for (int x = 4; x < 32; x <<= 1) {
-                top[0] = fmaxf(top[0], __shfl_xor_sync(0xFFFFFFFFu, top[0], x));
-                top[1] = fmaxf(top[1], __shfl_xor_sync(0xFFFFFFFFu, top[1], x));
-            }
-            if (__any_sync(0xFFFFFFFFu, top[0] > m[0] + kKv4Slack || top[1] > m[1] + kKv4Slack)) {
+                for (int u = 0; u < 2; ++u)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) w[u][i] = ex2(fmaf(s[u][i], unit[i & 1], (i & 1) ? from1 : from0));
+                sum[0] = (w[0][0] + w[0][2]) + (w[1][0] + w[1][2]), sum[1] = (w[0][1] + w[0][3]) + (w[1][1] + w[1][3]);
+                if (known || !__any_sync(0xFFFFFFFFu, !(fmaxf(sum[0], sum[1]) * big <= 32768.f))) break;
+                const float log_big = lg2(big);
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const float to = fmaxf(m[c], top[c]), f = m[c] == -INFINITY ? 0.f : ex2(m[c] - to);
+                    float top = fmaxf(fmaxf(s[0][c], s[0][2 + c]), fmaxf(s[1][c], s[1][2 + c]));
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+                    const float to = fmaxf(m[c], fmaf(top, unit[c], log_big)), f = m[c] == -INFINITY ? 0.f : ex2(m[c] - to);
                     m[c] = to;
                     l[c] *= f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) o[i][c] *= f, o[i][2 + c] *= f;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) ones[j][c] *= f, ones[j][2 + c] *= f, low[j][c] *= f;
+                    for (int j = 0; j < 4; ++j) low[j][c] *= f;
                 }
             }
-            // ---- weights, and what they are multiplied with ----
-            const float from0 = m[0] - kKv4Bias, from1 = m[1] - kKv4Bias;
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const float pa0 = ex2(s[u][0] - from0), pa1 = ex2(s[u][1] - from1), pb0 = ex2(s[u][2] - from0), pb1 = ex2(s[u][3] - from1);
-                l[0] += pa0 + pb0, l[1] += pa1 + pb1;
-                uint4 sa = lds128(vs_src + 16 * u * kKv4Scales), sb = lds128(vs_src + (16 * u + 8) * kKv4Scales);
+            l[0] += sum[0], l[1] += sum[1];
+            // ---- what they are multiplied with ----
+            auto values = [&](auto half) {           // of sixteen positions
+                constexpr int u = decltype(half)::value;
+                const float pa0 = w[u][0], pa1 = w[u][1], pb0 = w[u][2], pb1 = w[u][3];
+                uint4 sa = lds128_at<kVs + 16 * u * kS>(s_src), sb = lds128_at<kVs + (16 * u + 8) * kS>(s_src);
                 if (left < kKv4Tile) {
                     if (16 * u + my_row >= left) sa = make_uint4(0u, 0u, 0u, 0u);
                     if (16 * u + 8 + my_row >= left) sb = make_uint4(0u, 0u, 0u, 0u);
                 }
-                const uint32_t at_v = v_src + (16 * u + t) * kKv4Codes + 8 * g;
-                const uint2 v0 = lds64(at_v), v1 = lds64(at_v + 4 * kKv4Codes), v2 = lds64(at_v + 8 * kKv4Codes), v3 = lds64(at_v + 12 * kKv4Codes);
+                const uint2 v0 = lds64_at<kV + 16 * u * kC>(v_src), v1 = lds64_at<kV + (16 * u + 4) * kC>(v_src);
+                const uint2 v2 = lds64_at<kV + (16 * u + 8) * kC>(v_src), v3 = lds64_at<kV + (16 * u + 12) * kC>(v_src);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float2 fa = __half22float2(u32_as_half2(j == 0 ? sa.x : j == 1 ? sa.y : j == 2 ? sa.z : sa.w));
@@ -339,14 +360,17 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                     const uint32_t w0 = j < 2 ? prmt(v0.x, v1.x, sel) : prmt(v0.y, v1.y, sel), w1 = j < 2 ? prmt(v2.x, v3.x, sel) : prmt(v2.y, v3.y, sel);
                     mma_16816(o[2 * j], w0 & kLow, w0 & kHigh, w1 & kLow, w1 & kHigh, b0, b1);
                     mma_16816(o[2 * j + 1], (w0 >> 8) & kLow, (w0 >> 8) & kHigh, (w1 >> 8) & kLow, (w1 >> 8) & kHigh, b0, b1);
-                    mma_16816(ones[j], 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u, b0, b1);
+                    mma_16816(o[2 * j], kMinus8Low, kMinus8High, kMinus8Low, kMinus8High, b0, b1);
+                    mma_16816(o[2 * j + 1], kMinus8Low, kMinus8High, kMinus8Low, kMinus8High, b0, b1);
                     const float mid_a = fmaf(8.f, fa.x, fa.y), mid_b = fmaf(8.f, fb.x, fb.y);
                     low[j][0] = fmaf(pa0, mid_a, fmaf(pb0, mid_b, low[j][0]));
                     low[j][1] = fmaf(pa1, mid_a, fmaf(pb1, mid_b, low[j][1]));
                 }
-            }
+            };
+            values(std::integral_constant<int, 0>());
+            values(std::integral_constant<int, 1>());
             __syncwarp();                            // the stage is free
-            if (lane == 0 && ok && tile + kKv4Stages * kKv4Warps < t1) fetch(tile + kKv4Stages * kKv4Warps, ring_pos.s);
+            if (ok && tile + kKv4Stages * kKv4Warps < t1) fetch(tile + kKv4Stages * kKv4Warps, ring_pos.s);
             ring_pos.advance(kKv4Stages);
         }
         // ---- the warps' sums into one ----
@@ -365,7 +389,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             float *dst = merge + (warp * 8 + 2 * t + c) * 128 + 4 * g;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float mid = fmaf(-8.f, ones[j][c], low[j][c]);
+                const float mid = low[j][c];
                 *reinterpret_cast<float4 *>(dst + 32 * j) = make_float4(fmaf(16777216.f, o[2 * j][c], mid), fmaf(1048576.f, o[2 * j][2 + c], mid),
                                                                          fmaf(16777216.f, o[2 * j + 1][c], mid), fmaf(1048576.f, o[2 * j + 1][2 + c], mid));
             }
