@@ -54,23 +54,25 @@ __device__ __forceinline__ int kv4_context(const AttnKv4Params &p, const int32_t
 }
 __device__ __forceinline__ int kv4_tiles(int context) { return (context + kKv4Tile - 1) / kKv4Tile; }
 
-// How the tiles of all rows and heads are cut: `rows` rows' tiles laid end to end, each row `heads` times.
+// How the work is cut: every row's heads laid end to end, each worth its tiles and kKv4Start for what a CTA does around them (q, the ring's first copies, the warps' sums: as
+// long as about twelve tiles; without it the CTAs that got the short rows took 365,000 clocks where the others took 270,000: 32 rows of 500 to 32768).  In numbers of 32
+// bits: a unit stands for a tile of 5 KiB of the cache.
+constexpr uint32_t kKv4Start = 12;
+__device__ __forceinline__ uint32_t kv4_cost(int tiles) { return tiles ? (uint32_t)tiles + kKv4Start : 0u; }
 struct Kv4Cut {
-    int64_t total, ctas;
-    __device__ __forceinline__ int64_t begin(int64_t cta) const { return total * cta / ctas; }
-    __device__ __forceinline__ int64_t cta_of(int64_t tile) const {       // the range that a tile is in
-        int64_t c = tile * ctas / total;
-        while (begin(c + 1) <= tile) ++c;
-        while (begin(c) > tile) --c;
-        return c;
+    uint32_t ctas, per, extra;
+    __device__ __forceinline__ uint32_t begin(uint32_t cta) const { return cta * per + min(cta, extra); }
+    __device__ __forceinline__ uint32_t cta_of(uint32_t at) const {       // the range that a unit is in
+        return at < extra * (per + 1) ? at / (per + 1) : extra + (at - extra * (per + 1)) / per;
     }
 };
-__device__ __forceinline__ Kv4Cut kv4_cut(const AttnKv4Params &p, const int32_t *pos, int64_t most_ctas, int lane) {
-    int64_t sum = 0;
-    for (int r0 = 0; r0 < p.rows; r0 += 32) sum += __reduce_add_sync(0xFFFFFFFFu, r0 + lane < p.rows ? kv4_tiles(kv4_context(p, pos, r0 + lane)) : 0);
+__device__ __forceinline__ Kv4Cut kv4_cut(const AttnKv4Params &p, const int32_t *pos, uint32_t most_ctas, int lane) {
+    uint32_t sum = 0;
+    for (int r0 = 0; r0 < p.rows; r0 += 32) sum += __reduce_add_sync(0xFFFFFFFFu, r0 + lane < p.rows ? kv4_cost(kv4_tiles(kv4_context(p, pos, r0 + lane))) : 0u);
+    sum *= (uint32_t)(p.hkv * p.blocks);
     Kv4Cut c;
-    c.total = sum * p.hkv * p.blocks;
-    c.ctas = min(most_ctas, max((c.total + kKv4Warps - 1) / kKv4Warps, (int64_t)1));
+    c.ctas = min(most_ctas, max(sum / (kKv4Start + kKv4Warps / 2), 1u));
+    c.per = sum / c.ctas, c.extra = sum - c.per * c.ctas;
     return c;
 }
 
@@ -159,12 +161,13 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
     __syncwarp();
     pdl_wait_prior_grids();
     const int32_t *pos = after_wait(p.pos);
-    const int heads = p.hkv * p.blocks;              // of a row, in the order of the cut
-    int64_t at = 0, end = 0;
+    const uint32_t heads = (uint32_t)(p.hkv * p.blocks);      // of a row, in the order of the cut
+    uint32_t at = 0, end = 0;
     if (!WHOLE) {
         const Kv4Cut cut = kv4_cut(p, pos, gridDim.x, lane);
-        if (blockIdx.x >= cut.ctas || cut.total == 0) return;
+        if (blockIdx.x >= cut.ctas) return;
         at = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
+        if (at >= end) return;
     }
     RingPos ring_pos = {0, 0u};
     bool ok = true;
@@ -177,33 +180,34 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             if (context == 0 && pos[row] != -1 && tid == 0) atomicExch(p.status, kStatusPosition);
             t0 = 0, t1 = tiles = kv4_tiles(context);
         } else {
-            int64_t before = 0;
+            uint32_t before = 0;
             row = 0;
             tiles = 0;
             for (int r0 = 0; r0 < p.rows; r0 += 32) {
-                const int mine = r0 + lane < p.rows ? kv4_tiles(kv4_context(p, pos, r0 + lane)) : 0;
-                int upto = mine;
+                const int here = r0 + lane < p.rows ? kv4_tiles(kv4_context(p, pos, r0 + lane)) : 0;
+                uint32_t upto = kv4_cost(here);
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
-                    const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                    const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
                     if (lane >= o) upto += v;
                 }
                 const unsigned hit = __ballot_sync(0xFFFFFFFFu, (before + upto) * heads > at);
                 if (hit) {
                     const int from = __ffs(hit) - 1;
                     row = r0 + from;
-                    tiles = __shfl_sync(0xFFFFFFFFu, mine, from);
-                    before += __shfl_sync(0xFFFFFFFFu, upto - mine, from);
+                    tiles = __shfl_sync(0xFFFFFFFFu, here, from);
+                    before += __shfl_sync(0xFFFFFFFFu, upto - kv4_cost(here), from);
                     break;
                 }
                 before += __shfl_sync(0xFFFFFFFFu, upto, 31);
             }
-            const int64_t in_row = at - before * heads;
-            head = (int)(in_row / tiles);
-            t0 = (int)(in_row - (int64_t)head * tiles);
-            t1 = (int)min((int64_t)tiles, t0 + (end - at));
+            const uint32_t cost = kv4_cost(tiles), in_row = at - before * heads;
+            head = (int)(in_row / cost);
+            const uint32_t off = in_row - (uint32_t)head * cost, off_end = min(cost, off + (end - at));
+            t0 = (int)max(off, kKv4Start) - (int)kKv4Start, t1 = (int)max(off_end, kKv4Start) - (int)kKv4Start;
             context = kv4_context(p, pos, row);
-            at += t1 - t0;
+            at += off_end - off;
+            if (t0 == t1) continue;                  // the range ends in front of the first tile
         }
         const int kvh = head / p.blocks, first = (head - kvh * p.blocks) * 8, in_block = min(8, p.group - first), q_head = kvh * p.group + first;
         const int64_t cache_at = ((int64_t)row * p.hkv + kvh) * p.max_pos;
@@ -413,7 +417,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                 for (int i = 0; i < 4; ++i) sum[i] = context ? sum[i] / den : 0.f;
                 kv4_store(p, row, q_head + warp, lane, sum);
             } else {
-                const int64_t slot = (2 * (int64_t)blockIdx.x + (t0 == 0 ? 1 : 0)) * 8 + warp;
+                const uint32_t slot = (2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * 8 + warp;
                 p.part[slot * 32 + lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
                 if (lane == 0) p.part_ml[slot] = make_float2(mx, den);
             }
@@ -425,7 +429,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
 }
 
 // A CTA per row and q head: joins the parts that ranges have left of it, and writes the zeros of a row without positions.
-__global__ void __launch_bounds__(512) attn_kv4_join_kernel(const AttnKv4Params p, int64_t most_ctas) {
+__global__ void __launch_bounds__(512) attn_kv4_join_kernel(const AttnKv4Params p, uint32_t most_ctas) {
     __shared__ float4 sums[16][32];
     __shared__ float dens[16];
     pdl_allow_next_grid();
@@ -441,21 +445,21 @@ __global__ void __launch_bounds__(512) attn_kv4_join_kernel(const AttnKv4Params 
         return;
     }
     const Kv4Cut cut = kv4_cut(p, pos, most_ctas, lane);
-    int64_t before = 0;
-    for (int r0 = 0; r0 < row; r0 += 32) before += __reduce_add_sync(0xFFFFFFFFu, r0 + lane < row ? kv4_tiles(kv4_context(p, pos, r0 + lane)) : 0);
-    const int64_t begin = before * p.hkv * p.blocks + (int64_t)head * tiles;
-    const int64_t c0 = cut.cta_of(begin), c1 = cut.cta_of(begin + tiles - 1);
+    uint32_t before = 0;
+    for (int r0 = 0; r0 < row; r0 += 32) before += __reduce_add_sync(0xFFFFFFFFu, r0 + lane < row ? kv4_cost(kv4_tiles(kv4_context(p, pos, r0 + lane))) : 0u);
+    const uint32_t first_tile = before * (uint32_t)(p.hkv * p.blocks) + (uint32_t)head * kv4_cost(tiles) + kKv4Start;
+    const int c0 = (int)cut.cta_of(first_tile), c1 = (int)cut.cta_of(first_tile + tiles - 1);
     if (c0 == c1) return;                            // one range had it all
     const float4 *part = after_wait(p.part);
     const float2 *part_ml = after_wait(p.part_ml);
     float mx = -INFINITY, den = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int64_t c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, __ldcg(part_ml + (2 * c + (c == c0 ? 1 : 0)) * 8 + (in_group & 7)).x);
+    for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, __ldcg(part_ml + (2 * c + (c == c0 ? 1 : 0)) * 8 + (in_group & 7)).x);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
 #pragma unroll 4
-    for (int64_t c = c0 + warp; c <= c1; c += 16) {
-        const int64_t slot = (2 * c + (c == c0 ? 1 : 0)) * 8 + (in_group & 7);
+    for (int c = c0 + warp; c <= c1; c += 16) {
+        const int slot = (2 * c + (c == c0 ? 1 : 0)) * 8 + (in_group & 7);
         const float2 ml = __ldcg(part_ml + slot);
         const float4 x = __ldcg(part + slot * 32 + lane);
         const float f = ex2(ml.x - mx);
@@ -528,5 +532,5 @@ extern "C" int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *
     static SmemOptIn opted;
     if (int e = allow_max_smem(attn_kv4_kernel<false>, opted)) return e;
     if (int e = launch(attn_kv4_kernel<false>, dim3((unsigned)ctas), dim3(32 * kKv4Warps), kKv4Smem, s, p)) return e;
-    return launch(attn_kv4_join_kernel, dim3((unsigned)heads, (unsigned)p.rows), dim3(512), 0, s, p, ctas);
+    return launch(attn_kv4_join_kernel, dim3((unsigned)heads, (unsigned)p.rows), dim3(512), 0, s, p, (uint32_t)ctas);
 }
