@@ -3,15 +3,15 @@
 //   s_j = scale q . k_j,  o = sum_j p_j v_j / sum_j p_j,  p_j = exp(s_j - m);   k = min + scale_g * code in groups g of 32 values, v alike
 //
 // The cache is read once, 160 bytes per position and kv head, for up to eight q heads of its group at a time.  A warp takes tiles of 32 positions through a
-// private ring of bulk copies and multiplies the codes as they are on mma.sync (m16n8k16, fp32 accumulation):
+// private ring of asynchronous copies and multiplies the codes as they are on mma.sync (m16n8k16, fp32 accumulation):
 //   scores   A = codes of 16 positions x 16 dims, B = q (column = q head).  A nibble put into the low bits of an fp16 is the number code * 2^-24, exactly, and one
 //            four bits higher 16 times that: two masks and half a shift per register, and q's values in the odd places are divided by 16 beforehand (q is first brought to
 //            at most 2 by a power of two, so that this loses nothing above 2^-25 of its largest value).  A group's sum is then scaled in fp32:
 //            s = sum_g scale_g sum_g(q code) + min_g sum_g(q), the second sum as one more product, of the stored (scale, minimum) pairs with (0, sum_g(q)) in two
 //            fp16 parts.
-//   output   A = codes of 16 dims x 16 positions, B = p_j * scale_g in fp16 (one set per group; transposed from the scores' layout by movmatrix), and the same
-//            weights against a constant -8:  sum p scale (code - 8) + sum p (min + 8 scale).  Codes counted from the middle, so that what the weights' rounding
-//            (2^-11, as that of P in any 16-bit product) is multiplied with is not larger than the values; the second sum is in fp32.
+//   output   A = codes - 8 of 16 dims x 16 positions, B = p_j * scale_g in fp16 (one set per group; transposed from the scores' layout by movmatrix):
+//            sum p scale (code - 8) + sum p (min + 8 scale).  Codes counted from the middle, so that what the weights' rounding (2^-11, as that of P in any 16-bit
+//            product) is multiplied with is not larger than the values; the second sum is in fp32.  (-8 by a product with a constant operand: 173 us where this takes 160.)
 // Weights refer to a running maximum of s + log2(a tile's largest scale): the products p * scale then fit fp16 whatever the scales are (2^11 where the reference was set, and
 // it moves only when they may pass 2^15, which their sum shows: no maximum is looked for otherwise; what falls below 2^-14 is 2^-25 of the largest).
 // Bound: HBM.  About 290 warp instructions per 16 positions (2560 bytes), two thirds of the issue slots at the measured copy rate.
@@ -21,13 +21,12 @@
 
 #include "fwht.cuh"
 #include "kv4.cuh"
-#include "tc_ptx.cuh"
 
 namespace rptc {
 
 constexpr int kKv4Warps = 8, kKv4Tile = 32, kKv4Stages = 2;
 constexpr uint32_t kKv4StageBytes = 2 * kKv4Tile * (kKv4Codes + kKv4Scales);
-constexpr uint32_t kKv4Ring = kKv4Warps * kKv4Stages * kKv4StageBytes, kKv4Merge = kKv4Warps * 8 * 128 * 4, kKv4Smem = kKv4Ring + kKv4Merge + kKv4Warps * 8 * 8 + 256;
+constexpr uint32_t kKv4Ring = kKv4Warps * kKv4Stages * kKv4StageBytes, kKv4Merge = kKv4Warps * 8 * 128 * 4, kKv4Smem = kKv4Ring + kKv4Merge + kKv4Warps * 8 * 8;
 constexpr int kKv4CtasPerSm = 2;
 constexpr int64_t kKv4Whole = 1024;
 constexpr float kKv4Bias = 11.f;
@@ -122,6 +121,10 @@ __device__ __forceinline__ float lg2(float x) {
     return y;
 }
 
+// A pair of codes less 8 as fp16, in units of 2^-24: those in the low nibbles of the two halves, and 16 times those in the next ones.  Exact.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return half2_as_u32(__hadd2(u32_as_half2(w & 0x000F000Fu), u32_as_half2(0x80088008u))); }
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return half2_as_u32(__hadd2(u32_as_half2(w & 0x00F000F0u), u32_as_half2(0x80808080u))); }
+
 // Four neighbouring values of 128 per lane -> the same of the output, after the output projection's input transform where that is asked for.
 __device__ __forceinline__ void kv4_store(const AttnKv4Params &p, int row, int head, int lane, float (&o)[4]) {
     if (p.signs_in) {
@@ -152,13 +155,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
     const uint32_t ring = smem_addr(smem) + (uint32_t)warp * kKv4Stages * kKv4StageBytes;
     float *merge = reinterpret_cast<float *>(smem + kKv4Ring);
     float2 *merge_ml = reinterpret_cast<float2 *>(smem + kKv4Ring + kKv4Merge);
-    const uint32_t bars = smem_addr(smem) + kKv4Ring + kKv4Merge + kKv4Warps * 8 * 8 + 8u * kKv4Stages * warp;
     pdl_allow_next_grid();
-    if (lane == 0) {
-        for (int i = 0; i < kKv4Stages; ++i) mbar_init(bars + 8 * i, 1);
-        mbar_fence_init();
-    }
-    __syncwarp();
     pdl_wait_prior_grids();
     const int32_t *pos = after_wait(p.pos);
     const uint32_t heads = (uint32_t)(p.hkv * p.blocks);      // of a row, in the order of the cut
@@ -169,8 +166,6 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
         at = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
         if (at >= end) return;
     }
-    RingPos ring_pos = {0, 0u};
-    bool ok = true;
     do {
         // ---- a row's head, its tiles t0 .. t1 - 1 ----
         int row, head, context, t0, t1, tiles;
@@ -213,21 +208,39 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
         const int64_t cache_at = ((int64_t)row * p.hkv + kvh) * p.max_pos;
         const uint8_t *k = after_wait(p.k) + cache_at * kKv4Codes, *v = after_wait(p.v) + cache_at * kKv4Codes;
         const __half2 *ks = after_wait(p.k_scales) + cache_at * 4, *vs = after_wait(p.v_scales) + cache_at * 4;
-        // Lanes 0 .. 3 copy the four pieces of a tile: codes and scales of k, of v.
-        const char *from = reinterpret_cast<const char *>(lane == 0 ? (const void *)k : lane == 1 ? (const void *)ks : lane == 2 ? (const void *)v : (const void *)vs);
-        const uint32_t size = (lane & 1) ? kKv4Scales : kKv4Codes;
-        const uint32_t piece = ring + (lane & 1) * kKv4Tile * kKv4Codes + ((lane >> 1) & 1) * kKv4Tile * (kKv4Codes + kKv4Scales);
+        // A tile is 320 pieces of 16 bytes, ten of them a lane's.  (Bulk copies by four lanes took about 70 instructions a tile more: they are issued lane by lane.)
+        const uint8_t *k_from = k + 16 * lane, *v_from = v + 16 * lane;
+        const char *ks_from = reinterpret_cast<const char *>(ks) + 16 * lane, *vs_from = reinterpret_cast<const char *>(vs) + 16 * lane;
         auto fetch = [&](int tile, int stage) {
-            const uint32_t n = (uint32_t)min(kKv4Tile, context - tile * kKv4Tile), bar = bars + 8u * stage;
-            if (lane == 0) mbar_expect_tx(bar, 2 * n * (kKv4Codes + kKv4Scales));
-            __syncwarp();
-            if (lane < 4) bulk_g2s(piece + (uint32_t)stage * kKv4StageBytes, from + (int64_t)tile * kKv4Tile * size, n * size, bar);
+            if (tile < t1) {
+                const uint32_t dst = ring + (uint32_t)stage * kKv4StageBytes + 16u * lane;
+                const int64_t c = (int64_t)tile * (kKv4Tile * kKv4Codes), s = (int64_t)tile * (kKv4Tile * kKv4Scales);
+                const int n = context - tile * kKv4Tile;
+                if (n >= kKv4Tile) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) cp_async16(dst + 512u * i, k_from + c + 512 * i);
+                    cp_async16(dst + kKv4Tile * kKv4Codes, ks_from + s);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) cp_async16(dst + kKv4Tile * (kKv4Codes + kKv4Scales) + 512u * i, v_from + c + 512 * i);
+                    cp_async16(dst + kKv4Tile * (2 * kKv4Codes + kKv4Scales), vs_from + s);
+                } else {                             // no further than the last position
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (8 * i + (lane >> 2) >= n) continue;
+                        cp_async16(dst + 512u * i, k_from + c + 512 * i);
+                        cp_async16(dst + kKv4Tile * (kKv4Codes + kKv4Scales) + 512u * i, v_from + c + 512 * i);
+                    }
+                    if (lane < n) {
+                        cp_async16(dst + kKv4Tile * kKv4Codes, ks_from + s);
+                        cp_async16(dst + kKv4Tile * (2 * kKv4Codes + kKv4Scales), vs_from + s);
+                    }
+                }
+            }
+            cp_async_commit();                       // an empty group when nothing is left keeps the count constant
         };
-        {
-            int s = ring_pos.s;
-            for (int i = 0; i < kKv4Stages; ++i, s = s + 1 == kKv4Stages ? 0 : s + 1)
-                if (t0 + warp + i * kKv4Warps < t1) fetch(t0 + warp + i * kKv4Warps, s);
-        }
+#pragma unroll
+        for (int i = 0; i < kKv4Stages; ++i) fetch(t0 + warp + i * kKv4Warps, i);
+        int stage_no = 0;
         // ---- q: this lane's operand values are those of q head g, dims 8 t .. 8 t + 7 of each group ----
         uint32_t qb[4][4], q_low[2];                 // q_low: (0, sum of q over group t) in two fp16 parts, against (scale, minimum) pairs
         float unit[2];                               // of the q heads 2 t and 2 t + 1, whose scores this lane gets
@@ -270,13 +283,14 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
         // ---- this warp's tiles ----
         float o[8][4] = {}, low[4][2] = {}, l[2] = {0.f, 0.f}, m[2] = {-INFINITY, -INFINITY};
         const int my_row = (g >> 1) + 4 * (g & 1);   // the position of an operand's row g, so that the V operand's rows t and t + 4 are neighbours in the product
-        constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u, kMinus8Low = 0x80088008u, kMinus8High = 0x80808080u;
+        constexpr uint32_t kLow = 0x000F000Fu, kHigh = 0x00F000F0u;
         constexpr uint32_t kC = kKv4Codes, kS = kKv4Scales, kKs = kKv4Tile * kC, kV = kKs + kKv4Tile * kS, kVs = kV + kKv4Tile * kC;      // in a stage
         const uint32_t k_lane = ring + my_row * kC + 16 * t, s_lane = ring + my_row * kS, v_lane = ring + t * kC + 8 * g;
 #pragma unroll 1
-        for (int tile = t0 + warp; tile < t1 && ok; tile += kKv4Warps) {
-            const uint32_t stage = (uint32_t)ring_pos.s * kKv4StageBytes, k_src = k_lane + stage, s_src = s_lane + stage, v_src = v_lane + stage;
-            ok = __all_sync(0xFFFFFFFFu, mbar_wait(bars + 8u * ring_pos.s, ring_pos.phase, p.status));
+        for (int tile = t0 + warp; tile < t1; tile += kKv4Warps) {
+            const uint32_t stage = (uint32_t)stage_no * kKv4StageBytes, k_src = k_lane + stage, s_src = s_lane + stage, v_src = v_lane + stage;
+            cp_async_wait<kKv4Stages - 1>();
+            __syncwarp();                            // the other lanes' pieces
             const int left = context - tile * kKv4Tile;
             float s[2][4];
             auto scores = [&](auto half) {           // of sixteen positions
@@ -362,10 +376,8 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                     const uint32_t b0 = transpose8(half2_as_u32(__floats2half2_rn(pa0 * fa.x, pa1 * fa.x)));
                     const uint32_t b1 = transpose8(half2_as_u32(__floats2half2_rn(pb0 * fb.x, pb1 * fb.x)));
                     const uint32_t w0 = j < 2 ? prmt(v0.x, v1.x, sel) : prmt(v0.y, v1.y, sel), w1 = j < 2 ? prmt(v2.x, v3.x, sel) : prmt(v2.y, v3.y, sel);
-                    mma_16816(o[2 * j], w0 & kLow, w0 & kHigh, w1 & kLow, w1 & kHigh, b0, b1);
-                    mma_16816(o[2 * j + 1], (w0 >> 8) & kLow, (w0 >> 8) & kHigh, (w1 >> 8) & kLow, (w1 >> 8) & kHigh, b0, b1);
-                    mma_16816(o[2 * j], kMinus8Low, kMinus8High, kMinus8Low, kMinus8High, b0, b1);
-                    mma_16816(o[2 * j + 1], kMinus8Low, kMinus8High, kMinus8Low, kMinus8High, b0, b1);
+                    mma_16816(o[2 * j], low_codes(w0), high_codes(w0), low_codes(w1), high_codes(w1), b0, b1);
+                    mma_16816(o[2 * j + 1], low_codes(w0 >> 8), high_codes(w0 >> 8), low_codes(w1 >> 8), high_codes(w1 >> 8), b0, b1);
                     const float mid_a = fmaf(8.f, fa.x, fa.y), mid_b = fmaf(8.f, fb.x, fb.y);
                     low[j][0] = fmaf(pa0, mid_a, fmaf(pb0, mid_b, low[j][0]));
                     low[j][1] = fmaf(pa1, mid_a, fmaf(pb1, mid_b, low[j][1]));
@@ -374,8 +386,8 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             values(std::integral_constant<int, 0>());
             values(std::integral_constant<int, 1>());
             __syncwarp();                            // the stage is free
-            if (ok && tile + kKv4Stages * kKv4Warps < t1) fetch(tile + kKv4Stages * kKv4Warps, ring_pos.s);
-            ring_pos.advance(kKv4Stages);
+            fetch(tile + kKv4Stages * kKv4Warps, stage_no);
+            stage_no = stage_no + 1 == kKv4Stages ? 0 : stage_no + 1;
         }
         // ---- the warps' sums into one ----
 #pragma unroll
@@ -422,10 +434,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                 if (lane == 0) p.part_ml[slot] = make_float2(mx, den);
             }
         }
-    } while (!WHOLE && at < end && ok);
-    if (!ok) {                                       // copies in flight land before the CTA leaves
-        for (int i = 0; i < kKv4Stages; ++i, ring_pos.advance(kKv4Stages)) mbar_wait(bars + 8u * ring_pos.s, ring_pos.phase, p.status);
-    }
+    } while (!WHOLE && at < end);
 }
 
 // A CTA per row and q head: joins the parts that ranges have left of it, and writes the zeros of a row without positions.
@@ -532,5 +541,10 @@ extern "C" int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *
     static SmemOptIn opted;
     if (int e = allow_max_smem(attn_kv4_kernel<false>, opted)) return e;
     if (int e = launch(attn_kv4_kernel<false>, dim3((unsigned)ctas), dim3(32 * kKv4Warps), kKv4Smem, s, p)) return e;
-    return launch(attn_kv4_join_kernel, dim3((unsigned)heads, (unsigned)p.rows), dim3(512), 0, s, p, (uint32_t)ctas);
+    // the second kernel starts early and waits for the first one's sums itself
+    const bool before = pdl_enabled();
+    rptc_set_pdl(1);
+    const int e = launch(attn_kv4_join_kernel, dim3((unsigned)heads, (unsigned)p.rows), dim3(512), 0, s, p, (uint32_t)ctas);
+    rptc_set_pdl(before ? 1 : 0);
+    return e;
 }
