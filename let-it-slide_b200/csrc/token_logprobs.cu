@@ -1,9 +1,23 @@
 // Log probabilities of given tokens, the entropy and the largest entries of rows of logits.  No reference counterpart.
+//
+//   with M = max x:  z = sum exp(x - M),  w = sum exp(x - M) (x - M);   logprob = (x_t - M) - log z,   entropy = log z - w / z
+//
+// One pass over the row: a thread keeps M, z and w of its own entries, and they meet at the end.  (x - M first and then its multiple of log2(e): x log2(e) would leave
+// fp32's range at the lowest values that masks are made of.)  The largest entries need no second pass either: a thread knows its largest entry, the k-th largest of
+// those is a lower bound of the k-th largest entry, and only the (at most k, but for ties) threads that reach it look at their entries again.  What they find is ranked by
+// (value, index).  Where more is found than there is room for, as in a row of equal entries, the k largest are taken one by one, a pass over the row each.
+// Few rows: a cluster of CTAs shares a row, and each one's sums and k largest meet in the first one's shared memory.
+// Bound: HBM, with the special-function unit (an exponential per entry) next: 2048 x 32000 in fp16 20.0 us of traffic, 14.6 of exponentials.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
 #include "common.cuh"
 
 namespace rptc {
+
+namespace cg = cooperative_groups;
+
+constexpr int kLogprobThreads = 256, kLogprobRoom = 512, kLogprobTop = 32, kLogprobUnroll = 4, kLogprobMaxCluster = 8;
 
 struct LogprobParams {
     const void *logits;
@@ -22,40 +36,63 @@ __device__ __forceinline__ float logit(const void *row, int64_t i) {
     if (DTYPE == 1) return __bfloat162float(static_cast<const __nv_bfloat16 *>(row)[i]);
     return static_cast<const float *>(row)[i];
 }
-
-// The order of the largest entries as whole numbers: larger logits first, equal ones (0 and -0 too) by their index, NaN in front of all.
-__device__ __forceinline__ uint64_t order_key(float x, uint32_t i) {
-    const uint32_t b = __float_as_uint(x + 0.f);             // -0 + 0 is 0
-    const uint32_t up = x != x ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
-    return (uint64_t)up << 32 | (0xFFFFFFFFu - i);
+// The entries of sixteen bytes.
+template <int DTYPE, int N>
+__device__ __forceinline__ void logits_of(const uint4 &v, float (&x)[N]) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (DTYPE == 0) {
+            const float2 f = __half22float2(u32_as_half2(w[i]));
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        } else if (DTYPE == 1) {
+            x[2 * i] = __uint_as_float(w[i] << 16), x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        } else {
+            x[i] = __uint_as_float(w[i]);
+        }
+    }
 }
+
+// The order of the largest entries as whole numbers: larger logits first, equal ones (0 and -0 too) by their index, NaN in front of all.  Never 0.
+__device__ __forceinline__ uint32_t order_of(float x) {
+    const uint32_t b = __float_as_uint(x + 0.f);             // -0 + 0 is 0
+    return x != x ? 0xFFFFFFFFu : (b & 0x80000000u) ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ uint64_t order_key(float x, uint32_t i) { return (uint64_t)order_of(x) << 32 | (0xFFFFFFFFu - i); }
 __device__ __forceinline__ float key_logit(uint64_t key) {
     const uint32_t up = (uint32_t)(key >> 32);
     return up == 0xFFFFFFFFu ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float((up & 0x80000000u) ? up & 0x7FFFFFFFu : ~up);
 }
 
-// Running maximum m, z = sum exp(x - m) and w = sum exp(x - m) (x - m).  A forbidden token (-inf) adds nothing; with NaN or +inf z and w become NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {      // NaN if either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float ex2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLeast = -200.f;      // exp(-200) is 0 in 32 bits, and 0 * -200 is 0: what a forbidden token (-inf) adds
+
+// M, z and w of some entries; NaN among them (or +inf) makes all three NaN, -inf alone leaves M at -inf.
 struct Tally {
-    float m = -INFINITY, z = 0.f, w = 0.f;
-    __device__ __forceinline__ void move(float to) {
-        if (to == m || m == -INFINITY) {
-            m = to;
+    float M, z, w;
+    __device__ __forceinline__ void move(float to) {         // to >= M, or NaN
+        if (M == -INFINITY) {
+            M = to;
             return;
         }
-        const float d = m - to, f = __expf(d);
-        w = f * fmaf(z, f == 0.f ? 0.f : d, w);              // where f is 0, d may be too large for a product
+        const float d = max_nan(M - to, kLeast), f = ex2_fast(d * kLog2e);
+        w = f * fmaf(z, d, w);
         z *= f;
-        m = to;
-    }
-    __device__ __forceinline__ void add(float x) {
-        if (x == -INFINITY) return;
-        if (x > m) move(x);
-        const float d = x - m, e = __expf(d);
-        z += e;
-        w = fmaf(e, e == 0.f ? 0.f : d, w);
+        M = to;
     }
     __device__ __forceinline__ void join(Tally o) {
-        const float to = fmaxf(m, o.m);
+        const float to = max_nan(M, o.M);
+        if (to == -INFINITY) return;
         move(to);
         o.move(to);
         z += o.z;
@@ -63,62 +100,276 @@ struct Tally {
     }
 };
 
+// A CTA's share of a row: sixteen-byte vectors first .. last - 1, and for the first and last CTA the entries in front of and behind the vectors, one to a thread.
 template <int DTYPE>
-__global__ void __launch_bounds__(256) token_logprobs_kernel(const LogprobParams p) {
-    __shared__ Tally tallies[8];
-    __shared__ uint64_t keys[8];
+struct Share {
+    static constexpr int kPer = DTYPE == 2 ? 4 : 8;
+    const char *row, *vectors;
+    int64_t n;
+    int32_t head, tail, first, last;                         // entries in front of and behind all vectors
+    bool has_head, has_tail;
+    __device__ __forceinline__ Share(const void *logits, int64_t r, const LogprobParams &p, int rank, int ranks) {
+        constexpr int kSize = DTYPE == 2 ? 4 : 2;
+        row = static_cast<const char *>(logits) + r * p.ld * kSize;
+        n = p.n;
+        const int lead = (int)((0 - reinterpret_cast<uintptr_t>(row)) & 15) / kSize;
+        head = (int)min((int64_t)lead, n);
+        const int all = (int)((n - head) / kPer);
+        tail = (int)(n - head) - all * kPer;
+        vectors = row + head * kSize;
+        first = (int)((int64_t)all * rank / ranks), last = (int)((int64_t)all * (rank + 1) / ranks);
+        has_head = rank == 0, has_tail = rank == ranks - 1;
+    }
+    __device__ __forceinline__ uint4 vector(int v) const { return __ldg(reinterpret_cast<const uint4 *>(vectors) + v); }
+    // the entry outside the vectors that thread t has, or -1
+    __device__ __forceinline__ int64_t single(int t) const {
+        if (has_head && t < head) return t;
+        if (has_tail && t >= 32 && t - 32 < tail) return n - tail + (t - 32);
+        return -1;
+    }
+    __device__ __forceinline__ uint32_t index(int v, int e) const { return (uint32_t)(head + v * kPer + e); }
+};
+
+constexpr int kLogprobWarps = kLogprobThreads / 32;
+struct LogprobShared {
+    Tally tallies[kLogprobWarps];
+    uint32_t sample[kLogprobWarps * 32];                     // the largest of every warp's threads' largest, in the order of the numbers
+    uint32_t bound;
+    int found, chosen;
+    int who[kLogprobThreads];
+    uint64_t keys[kLogprobRoom], best[kLogprobTop], merged[kLogprobMaxCluster * kLogprobTop], round[kLogprobWarps];
+    Tally tally;
+};
+
+// The k largest of the CTA's share, in order (0 where there are fewer), in sh.best.  All threads.
+template <int DTYPE>
+__device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, float mine, int k) {
+    constexpr int kPer = Share<DTYPE>::kPer;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    // A bound that at least k threads' largest entries reach: the k-th of a few of every warp, a few more than its part of k, so that it is seldom lower than the k-th of all.
+    const int few = min(32, (k + kLogprobWarps - 1) / kLogprobWarps + 2), samples = few * kLogprobWarps;
+    const uint32_t own = order_of(mine);
+    uint32_t left = own;
+    for (int j = 0; j < few; ++j) {
+        const uint32_t b = __reduce_max_sync(0xFFFFFFFFu, left);
+        if (lane == __ffs(__ballot_sync(0xFFFFFFFFu, left == b)) - 1) {
+            left = 0;
+            sh.sample[warp * few + j] = b;
+        }
+    }
+    if (t == 0) sh.found = sh.chosen = 0;
+    if (t < k) sh.best[t] = 0;
+    __syncthreads();
+    if (t < samples) {
+        const uint32_t x = sh.sample[t];
+        int before = 0;
+        for (int j = 0; j < samples; ++j) {
+            const uint32_t y = sh.sample[j];
+            before += y > x || (y == x && j < t);
+        }
+        if (before == k - 1) sh.bound = x;
+    }
+    __syncthreads();
+    const uint32_t bound = sh.bound;
+    if (own >= bound) sh.who[atomicAdd(&sh.chosen, 1)] = t;
+    auto offer = [&](float x, uint32_t i) {
+        if (order_of(x) < bound) return;
+        const int at = atomicAdd(&sh.found, 1);
+        if (at < kLogprobRoom) sh.keys[at] = order_key(x, i);
+    };
+    if (own >= bound)
+        if (const int64_t s = share.single(t); s >= 0) offer(logit<DTYPE>(share.row, s), (uint32_t)s);
+    __syncthreads();
+    // all threads look at the vectors of those that reach it
+    const int chosen = sh.chosen, each = (share.last - share.first + kLogprobThreads - 1) / kLogprobThreads;
+    for (int i = t; i < chosen * each; i += kLogprobThreads) {
+        const int q = i / each, v = share.first + sh.who[q] + (i - q * each) * kLogprobThreads;
+        if (v >= share.last) continue;
+        float x[kPer];
+        logits_of<DTYPE>(share.vector(v), x);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) offer(x[e], share.index(v, e));
+    }
+    __syncthreads();
+    const int found = sh.found;
+    if (found <= kLogprobRoom) {
+        for (int i = t; i < found; i += kLogprobThreads) {
+            const uint64_t key = sh.keys[i];
+            int rank = 0;
+            for (int j = 0; j < found && rank < k; ++j) rank += sh.keys[j] > key;
+            if (rank < k) sh.best[rank] = key;
+        }
+    } else {
+        uint64_t last = ~0ull;
+        for (int j = 0; j < k; ++j) {                        // one after the other
+            uint64_t best = 0;
+            auto look = [&](float x, uint32_t i) {
+                const uint64_t key = order_key(x, i);
+                if (key < last && key > best) best = key;
+            };
+            for (int v = share.first + t; v < share.last; v += kLogprobThreads) {
+                float x[kPer];
+                logits_of<DTYPE>(share.vector(v), x);
+#pragma unroll
+                for (int e = 0; e < kPer; ++e) look(x[e], share.index(v, e));
+            }
+            const int64_t s = share.single(t);
+            if (s >= 0) look(logit<DTYPE>(share.row, s), (uint32_t)s);
+            for (int o = 16; o > 0; o >>= 1) {
+                const uint64_t b = __shfl_xor_sync(0xFFFFFFFFu, best, o);
+                best = b > best ? b : best;
+            }
+            __syncthreads();
+            if (lane == 0) sh.round[warp] = best;
+            __syncthreads();
+            for (int i = 0; i < kLogprobThreads / 32; ++i) best = sh.round[i] > best ? sh.round[i] : best;
+            last = best;
+            if (t == 0) sh.best[j] = best;
+        }
+    }
+    __syncthreads();
+}
+
+template <int DTYPE, bool CLUSTER>
+__global__ void __launch_bounds__(kLogprobThreads, 4) token_logprobs_kernel(const LogprobParams p) {
+    constexpr int kPer = Share<DTYPE>::kPer, U = kLogprobUnroll;
+    __shared__ LogprobShared sh;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
+    int rank = 0, ranks = 1;
+    int64_t r = blockIdx.x;
+    if (CLUSTER) {
+        ranks = (int)cg::this_cluster().num_blocks(), rank = (int)cg::this_cluster().block_rank();
+        r = blockIdx.x / ranks;
+    }
     pdl_allow_next_grid();
     pdl_wait_prior_grids();
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
-    const int64_t r = blockIdx.x;
-    const char *row = static_cast<const char *>(after_wait(p.logits)) + r * p.ld * (DTYPE == 2 ? 4 : 2);
-    Tally a;
-    for (int64_t i = t; i < p.n; i += 256) a.add(logit<DTYPE>(row, i));
+    const Share<DTYPE> share(after_wait(p.logits), r, p, rank, ranks);
+    Tally a = {-INFINITY, 0.f, 0.f};
+    float largest = -INFINITY;                               // of this thread's entries; NaN if any is
+    auto add = [&](const float (&x)[kPer], f32x2 &z, f32x2 &w) {
+        const f32x2 unit = pack2(kLog2e, kLog2e), from = pack2(-a.M, -a.M);
+#pragma unroll
+        for (int e = 0; e < kPer; e += 2) {
+            float lo, hi;
+            unpack2(add2(pack2(x[e], x[e + 1]), from), lo, hi);
+            const f32x2 d = pack2(max_nan(lo, kLeast), max_nan(hi, kLeast));
+            unpack2(mul2(d, unit), lo, hi);
+            const f32x2 q = pack2(ex2_fast(lo), ex2_fast(hi));
+            z = add2(z, q);
+            w = fma2(q, d, w);
+        }
+    };
+    for (int v0 = share.first + t; v0 < share.last; v0 += U * kLogprobThreads) {
+        uint4 raw[U];
+        // a vector that is not there is one of forbidden tokens
+        const uint32_t none = DTYPE == 0 ? 0xFC00FC00u : DTYPE == 1 ? 0xFF80FF80u : 0xFF800000u;
+#pragma unroll
+        for (int u = 0; u < U; ++u) raw[u] = v0 + u * kLogprobThreads < share.last ? share.vector(v0 + u * kLogprobThreads) : make_uint4(none, none, none, none);
+        float top = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float x[kPer];
+            logits_of<DTYPE>(raw[u], x);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) top = max_nan(top, x[e]);
+        }
+        if (top == -INFINITY) continue;
+        if (!(top <= largest)) {
+            largest = max_nan(top, largest);
+            a.move(largest);
+        }
+        f32x2 z = pack2(a.z, 0.f), w = pack2(a.w, 0.f);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            float x[kPer];
+            logits_of<DTYPE>(raw[u], x);
+            add(x, z, w);
+        }
+        float lo, hi;
+        unpack2(z, lo, hi), a.z = lo + hi;
+        unpack2(w, lo, hi), a.w = lo + hi;
+    }
+    if (const int64_t s = share.single(t); s >= 0) {
+        const float x = logit<DTYPE>(share.row, s);
+        if (!(x == -INFINITY)) {
+            if (!(x <= largest)) {
+                largest = max_nan(x, largest);
+                a.move(largest);
+            }
+            const float d = max_nan(x - a.M, kLeast), e = ex2_fast(d * kLog2e);
+            a.z += e;
+            a.w = fmaf(e, d, a.w);
+        }
+    }
+    const float mine = largest;
     for (int o = 16; o > 0; o >>= 1) {
         Tally b;
-        b.m = __shfl_xor_sync(0xFFFFFFFFu, a.m, o), b.z = __shfl_xor_sync(0xFFFFFFFFu, a.z, o), b.w = __shfl_xor_sync(0xFFFFFFFFu, a.w, o);
+        b.M = __shfl_xor_sync(0xFFFFFFFFu, a.M, o), b.z = __shfl_xor_sync(0xFFFFFFFFu, a.z, o), b.w = __shfl_xor_sync(0xFFFFFFFFu, a.w, o);
         a.join(b);
     }
-    if (lane == 0) tallies[warp] = a;
-    __syncthreads();
-    a = tallies[0];
-    for (int i = 1; i < 8; ++i) a.join(tallies[i]);
-    const float log_z = logf(a.z);
+    if (lane == 0) sh.tallies[warp] = a;
+    if (p.k > 0) largest_entries<DTYPE>(sh, share, mine, p.k);
+    else __syncthreads();
     if (t == 0) {
-        if (p.entropy) p.entropy[r] = log_z - a.w / a.z;
-        if (p.targets) {
-            const int64_t at = after_wait(p.targets)[r];
-            float lp = 0.f;
-            if (at >= 0 && at < p.n) {
-                lp = (logit<DTYPE>(row, at) - a.m) - log_z;
-            } else if (at != -1) {
-                lp = __uint_as_float(0x7FFFFFFFu);
-                atomicExch(p.status, kStatusPosition);
+        a = sh.tallies[0];
+        for (int i = 1; i < kLogprobThreads / 32; ++i) a.join(sh.tallies[i]);
+        sh.tally = a;
+    }
+    if (CLUSTER) {
+        cg::this_cluster().sync();
+        if (rank == 0) {                                     // the others' sums and largest entries
+            for (int i = t; i < ranks * p.k; i += kLogprobThreads) sh.merged[i] = cg::this_cluster().map_shared_rank(sh.best, i / p.k)[i % p.k];
+            if (t == 0)
+                for (int i = 1; i < ranks; ++i) a.join(*cg::this_cluster().map_shared_rank(&sh.tally, i)), sh.tally = a;
+            __syncthreads();
+            if (const int i = t; i < ranks * p.k && sh.merged[i]) {
+                int at = 0;
+                for (int j = 0; j < ranks * p.k; ++j) at += sh.merged[j] > sh.merged[i];
+                if (at < p.k) sh.keys[at] = sh.merged[i];
             }
-            p.logprob[r] = lp;
         }
-    }
-    uint64_t last = ~0ull;
-    for (int j = 0; j < p.k; ++j) {
-        uint64_t best = 0;
-        for (int64_t i = t; i < p.n; i += 256) {
-            const uint64_t key = order_key(logit<DTYPE>(row, i), (uint32_t)i);
-            if (key < last && key > best) best = key;
-        }
-        for (int o = 16; o > 0; o >>= 1) {
-            const uint64_t b = __shfl_xor_sync(0xFFFFFFFFu, best, o);
-            best = b > best ? b : best;
-        }
+        cg::this_cluster().sync();                           // nobody leaves before its shared memory has been read
+        if (rank) return;
+    } else {
         __syncthreads();
-        if (lane == 0) keys[warp] = best;
-        __syncthreads();
-        for (int i = 0; i < 8; ++i) best = keys[i] > best ? keys[i] : best;
-        last = best;
-        if (t == 0) {
-            p.top[r * p.k + j] = (key_logit(best) - a.m) - log_z;
-            p.ids[r * p.k + j] = 0xFFFFFFFFu - (uint32_t)best;
-        }
     }
+    const float M = sh.tally.M, log_z = logf(sh.tally.z);
+    auto logprob = [&](float x) { return (x - M) - log_z; };
+    if (t < p.k) {
+        const uint64_t key = CLUSTER ? sh.keys[t] : sh.best[t];
+        p.top[r * p.k + t] = logprob(key_logit(key));
+        p.ids[r * p.k + t] = 0xFFFFFFFFu - (uint32_t)key;
+    }
+    if (t == 32 && p.entropy) p.entropy[r] = log_z - sh.tally.w / sh.tally.z;
+    if (t == 64 && p.targets) {
+        const int64_t at = after_wait(p.targets)[r];
+        float lp = 0.f;
+        if (at >= 0 && at < p.n) {
+            lp = logprob(logit<DTYPE>(share.row, at));
+        } else if (at != -1) {
+            lp = __uint_as_float(0x7FFFFFFFu);
+            atomicExch(p.status, kStatusPosition);
+        }
+        p.logprob[r] = lp;
+    }
+}
+
+template <int DTYPE>
+static int launch_logprobs(const LogprobParams &p, int64_t rows, int cluster, cudaStream_t s) {
+    if (cluster == 1) return launch(token_logprobs_kernel<DTYPE, false>, dim3((unsigned)rows), dim3(kLogprobThreads), 0, s, p);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * cluster));
+    cfg.blockDim = dim3(kLogprobThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)cluster, 1, 1};
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = pdl_enabled() ? 2 : 1;
+    RPTC_CUDA(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<DTYPE, true>, p));
+    return RPTC_OK;
 }
 
 }  // namespace rptc
@@ -145,8 +396,8 @@ extern "C" int rptc_token_logprobs(const void *logits, int dtype, int64_t ld, co
     LogprobParams p = {logits, ld, targets, logprob, entropy, top_logprobs, top_ids, n, top, device_status_word()};
     if (!p.status) return RPTC_ERR_CUDA;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const dim3 grid((unsigned)rows);
-    return dtype == 0 ? launch(token_logprobs_kernel<0>, grid, dim3(256), 0, s, p)
-           : dtype == 1 ? launch(token_logprobs_kernel<1>, grid, dim3(256), 0, s, p)
-                        : launch(token_logprobs_kernel<2>, grid, dim3(256), 0, s, p);
+    // Few rows: up to eight CTAs share one, as long as each has 8 KiB of it.
+    int cluster = 1;
+    while (cluster < kLogprobMaxCluster && rows * cluster * 2 <= 2 * num_sms() && n * (dtype == 2 ? 4 : 2) >= cluster * 2 * 8192) cluster *= 2;
+    return dtype == 0 ? launch_logprobs<0>(p, rows, cluster, s) : dtype == 1 ? launch_logprobs<1>(p, rows, cluster, s) : launch_logprobs<2>(p, rows, cluster, s);
 }
