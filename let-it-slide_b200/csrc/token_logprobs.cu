@@ -69,6 +69,13 @@ __device__ __forceinline__ float max_nan(float a, float b) {      // NaN if eith
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
+template <int DTYPE>
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+    uint32_t d;
+    if (DTYPE == 0) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
 __device__ __forceinline__ float ex2_fast(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -99,6 +106,12 @@ struct Tally {
         w += o.w;
     }
 };
+
+__device__ __forceinline__ float warp_max_nan(float x) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) x = max_nan(x, __shfl_xor_sync(0xFFFFFFFFu, x, o));
+    return x;
+}
 
 // A CTA's share of a row: sixteen-byte vectors first .. last - 1, and for the first and last CTA the entries in front of and behind the vectors, one to a thread.
 template <int DTYPE>
@@ -133,8 +146,7 @@ struct Share {
 constexpr int kLogprobWarps = kLogprobThreads / 32;
 struct LogprobShared {
     Tally tallies[kLogprobWarps];
-    uint32_t sample[kLogprobWarps * 32];                     // the largest of every warp's threads' largest, in the order of the numbers
-    uint32_t bound;
+    alignas(16) uint32_t sample[kLogprobWarps * 32 + 4];     // the largest of every warp's threads' largest, in the order of the numbers
     int found, chosen;
     int who[kLogprobThreads];
     uint64_t keys[kLogprobRoom], best[kLogprobTop], merged[kLogprobMaxCluster * kLogprobTop], round[kLogprobWarps];
@@ -159,36 +171,52 @@ __device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, fl
     }
     if (t == 0) sh.found = sh.chosen = 0;
     if (t < k) sh.best[t] = 0;
+    if (t >= samples && t < samples + 4) sh.sample[t] = 0;      // to whole loads
     __syncthreads();
-    if (t < samples) {
-        const uint32_t x = sh.sample[t];
+    uint32_t bound = 0;                                      // every warp finds it for itself
+    for (int i = lane; i < samples; i += 32) {
+        const uint32_t x = sh.sample[i];
         int before = 0;
-        for (int j = 0; j < samples; ++j) {
-            const uint32_t y = sh.sample[j];
-            before += y > x || (y == x && j < t);
+        for (int j = 0; j < samples; j += 4) {
+            const uint4 y = *reinterpret_cast<const uint4 *>(sh.sample + j);
+            before += (y.x > x) + (y.y > x) + (y.z > x) + (y.w > x);
         }
-        if (before == k - 1) sh.bound = x;
+        if (before < k) bound = bound ? min(bound, x) : x;   // the smallest that fewer than k pass
     }
-    __syncthreads();
-    const uint32_t bound = sh.bound;
-    if (own >= bound) sh.who[atomicAdd(&sh.chosen, 1)] = t;
+    bound = __reduce_min_sync(0xFFFFFFFFu, bound ? bound : 0xFFFFFFFFu);
     auto offer = [&](float x, uint32_t i) {
         if (order_of(x) < bound) return;
         const int at = atomicAdd(&sh.found, 1);
         if (at < kLogprobRoom) sh.keys[at] = order_key(x, i);
     };
-    if (own >= bound)
+    const bool reaches = own >= bound;
+    if (reaches)
         if (const int64_t s = share.single(t); s >= 0) offer(logit<DTYPE>(share.row, s), (uint32_t)s);
+    if (reaches) sh.who[atomicAdd(&sh.chosen, 1)] = t;
     __syncthreads();
-    // all threads look at the vectors of those that reach it
+    // all threads look at the vectors of those that reach the bound, a few at a time
     const int chosen = sh.chosen, each = (share.last - share.first + kLogprobThreads - 1) / kLogprobThreads;
-    for (int i = t; i < chosen * each; i += kLogprobThreads) {
-        const int q = i / each, v = share.first + sh.who[q] + (i - q * each) * kLogprobThreads;
-        if (v >= share.last) continue;
-        float x[kPer];
-        logits_of<DTYPE>(share.vector(v), x);
+    for (int i0 = t; i0 < chosen * each; i0 += 2 * kLogprobThreads) {
+        uint4 raw[2];
+        int v[2];
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) offer(x[e], share.index(v, e));
+        for (int u = 0; u < 2; ++u) {
+            const int i = i0 + u * kLogprobThreads, q = i / each;
+            v[u] = i < chosen * each ? share.first + sh.who[q] + (i - q * each) * kLogprobThreads : share.last;
+            if (v[u] < share.last) raw[u] = share.vector(v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            if (v[u] >= share.last) continue;
+            float x[kPer];
+            logits_of<DTYPE>(raw[u], x);
+            float top = x[0];
+#pragma unroll
+            for (int e = 1; e < kPer; ++e) top = max_nan(top, x[e]);
+            if (order_of(top) < bound) continue;             // most have nothing
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) offer(x[e], share.index(v[u], e));
+        }
     }
     __syncthreads();
     const int found = sh.found;
@@ -231,7 +259,7 @@ __device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, fl
 }
 
 template <int DTYPE, bool CLUSTER>
-__global__ void __launch_bounds__(kLogprobThreads, 4) token_logprobs_kernel(const LogprobParams p) {
+__global__ void __launch_bounds__(kLogprobThreads, 5) token_logprobs_kernel(const LogprobParams p) {
     constexpr int kPer = Share<DTYPE>::kPer, U = kLogprobUnroll;
     __shared__ LogprobShared sh;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
@@ -244,6 +272,12 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) token_logprobs_kernel(cons
     pdl_allow_next_grid();
     pdl_wait_prior_grids();
     const Share<DTYPE> share(after_wait(p.logits), r, p, rank, ranks);
+    int64_t target = -1;
+    float target_logit = 0.f;
+    if (t == 64 && rank == 0 && p.targets) {                 // its trip to memory under the others'
+        target = after_wait(p.targets)[r];
+        if (target >= 0 && target < p.n) target_logit = logit<DTYPE>(share.row, target);
+    }
     Tally a = {-INFINITY, 0.f, 0.f};
     float largest = -INFINITY;                               // of this thread's entries; NaN if any is
     auto add = [&](const float (&x)[kPer], f32x2 &z, f32x2 &w) {
@@ -266,12 +300,20 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) token_logprobs_kernel(cons
 #pragma unroll
         for (int u = 0; u < U; ++u) raw[u] = v0 + u * kLogprobThreads < share.last ? share.vector(v0 + u * kLogprobThreads) : make_uint4(none, none, none, none);
         float top = -INFINITY;
+        if (DTYPE == 2) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            float x[kPer];
-            logits_of<DTYPE>(raw[u], x);
+            for (int u = 0; u < U; ++u) {
+                float x[kPer];
+                logits_of<DTYPE>(raw[u], x);
 #pragma unroll
-            for (int e = 0; e < kPer; ++e) top = max_nan(top, x[e]);
+                for (int e = 0; e < kPer; ++e) top = max_nan(top, x[e]);
+            }
+        } else {
+            uint32_t m = raw[0].x;                           // pairs
+#pragma unroll
+            for (int u = 0; u < U; ++u) m = max_pair<DTYPE>(max_pair<DTYPE>(m, max_pair<DTYPE>(raw[u].x, raw[u].y)), max_pair<DTYPE>(raw[u].z, raw[u].w));
+            top = DTYPE == 0 ? max_nan(__low2float(u32_as_half2(m)), __high2float(u32_as_half2(m)))
+                             : max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
         }
         if (top == -INFINITY) continue;
         if (!(top <= largest)) {
@@ -302,18 +344,21 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) token_logprobs_kernel(cons
         }
     }
     const float mine = largest;
-    for (int o = 16; o > 0; o >>= 1) {
-        Tally b;
-        b.M = __shfl_xor_sync(0xFFFFFFFFu, a.M, o), b.z = __shfl_xor_sync(0xFFFFFFFFu, a.z, o), b.w = __shfl_xor_sync(0xFFFFFFFFu, a.w, o);
-        a.join(b);
-    }
+    const float warp_top = warp_max_nan(a.M);
+    if (!(warp_top == -INFINITY)) a.move(warp_top);
+    for (int o = 16; o > 0; o >>= 1) a.z += __shfl_xor_sync(0xFFFFFFFFu, a.z, o), a.w += __shfl_xor_sync(0xFFFFFFFFu, a.w, o);
     if (lane == 0) sh.tallies[warp] = a;
     if (p.k > 0) largest_entries<DTYPE>(sh, share, mine, p.k);
     else __syncthreads();
-    if (t == 0) {
-        a = sh.tallies[0];
-        for (int i = 1; i < kLogprobThreads / 32; ++i) a.join(sh.tallies[i]);
-        sh.tally = a;
+    if (warp == 0) {
+        a = sh.tallies[lane % kLogprobWarps];
+#pragma unroll
+        for (int o = 1; o < kLogprobWarps; o <<= 1) {
+            Tally b;
+            b.M = __shfl_xor_sync(0xFFFFFFFFu, a.M, o), b.z = __shfl_xor_sync(0xFFFFFFFFu, a.z, o), b.w = __shfl_xor_sync(0xFFFFFFFFu, a.w, o);
+            a.join(b);
+        }
+        if (lane == 0) sh.tally = a;
     }
     if (CLUSTER) {
         cg::this_cluster().sync();
@@ -322,7 +367,8 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) token_logprobs_kernel(cons
             if (t == 0)
                 for (int i = 1; i < ranks; ++i) a.join(*cg::this_cluster().map_shared_rank(&sh.tally, i)), sh.tally = a;
             __syncthreads();
-            if (const int i = t; i < ranks * p.k && sh.merged[i]) {
+            for (int i = t; i < ranks * p.k; i += kLogprobThreads) {
+                if (sh.merged[i] == 0) continue;
                 int at = 0;
                 for (int j = 0; j < ranks * p.k; ++j) at += sh.merged[j] > sh.merged[i];
                 if (at < p.k) sh.keys[at] = sh.merged[i];
@@ -342,11 +388,10 @@ __global__ void __launch_bounds__(kLogprobThreads, 4) token_logprobs_kernel(cons
     }
     if (t == 32 && p.entropy) p.entropy[r] = log_z - sh.tally.w / sh.tally.z;
     if (t == 64 && p.targets) {
-        const int64_t at = after_wait(p.targets)[r];
         float lp = 0.f;
-        if (at >= 0 && at < p.n) {
-            lp = logprob(logit<DTYPE>(share.row, at));
-        } else if (at != -1) {
+        if (target >= 0 && target < p.n) {
+            lp = logprob(target_logit);
+        } else if (target != -1) {
             lp = __uint_as_float(0x7FFFFFFFu);
             atomicExch(p.status, kStatusPosition);
         }
