@@ -19,25 +19,27 @@ inline int check_kv_cache(const rptc_kv_cache &c) {
 
 #ifdef __CUDACC__
 // Eight neighbouring values of a thread, whose group of 32 is that of four neighbouring lanes -> the thread's eight codes (nibbles, first value lowest) and the
-// group's scale and minimum.  The difference, its fifteenth and the quotient are rounded to 32 bits each, the scale then to fp16: what is stored is
-// what the codes are counted in.  A quotient differs from a half-way point by 2^-17 of itself at least (fp16 numbers over an fp16 number), which 32 bits hold.
+// group's scale and minimum.  The difference and its fifteenth are rounded to 32 bits each, the scale then to fp16: what is stored is what the codes are counted in.
+// Quotients by Markstein's correction (an estimate times the reciprocal, its exact remainder by a fused multiply-add, and the remainder's quotient added): one that is
+// half-way between two codes comes out exactly; any other differs from half-way by 2^-17 of itself at least (fp16 numbers over an fp16 number), far more than the estimate is off.
 __device__ __forceinline__ uint32_t kv4_quantise(const float (&v)[8], __half2 &scale_min) {
-    float lo = v[0], hi = v[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) lo = fminf(lo, v[i]), hi = fmaxf(hi, v[i]);
+    float lo = fminf(fminf(fminf(v[0], v[1]), fminf(v[2], v[3])), fminf(fminf(v[4], v[5]), fminf(v[6], v[7])));
+    float hi = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
     }
-    const __half scale = __float2half_rn(__fdiv_rn(hi - lo, 15.f));
+    const float range = hi - lo, part = range * (1.f / 15.f);
+    const __half scale = __float2half_rn(fmaf(fmaf(-part, 15.f, range), 1.f / 15.f, part));      // the rounded fifteenth, for every significand
     scale_min = __halves2half2(scale, __float2half_rn(lo));
-    const float step = __half2float(scale);
+    const float step = __half2float(scale), inv = step > 0.f ? __frcp_rn(step) : 0.f;      // scale 0: codes 0
     uint32_t codes = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float c = step > 0.f ? fminf(rintf(__fdiv_rn(v[i] - lo, step)), 15.f) : 0.f;
-        codes |= (uint32_t)c << (4 * i);
+        const float d = v[i] - lo, q0 = d * inv, q = fmaf(fmaf(-q0, step, d), inv, q0);
+        const uint32_t c = __float_as_uint(fminf(q, 15.f) + 12582912.f) & 15u;             // 1.5 * 2^23: rounds to the nearest whole number, half to even
+        codes |= c << (4 * i);
     }
     return codes;
 }

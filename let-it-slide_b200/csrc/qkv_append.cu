@@ -17,87 +17,149 @@ struct AppendParams {
     __half2 *k_scales, *v_scales;
     int64_t rows, max_pos;
     int32_t hq, hkv, clear, out_kv;
-    int32_t chunk, chunks;           // heads of a warp (even), warps of a token
+    int32_t chunk, chunks_q, chunks_kv, chunks;      // heads of a warp (even); warps of a token: for q, for k (and v), all
     float scale;                     // includes 1 / sqrt(128) with the transform
     unsigned int *status;
 };
 
-// A warp takes `chunk` heads of a token, two at a time: a half-warp holds a head, a lane eight neighbouring values of it.  The
-// rotation's partner (64 values on) is the lane 8 on, a group of 32 values is four lanes.  Rotation with every product rounded, as elementary operations
-// round it: which of two codes a value next to a border gets does not depend on what the compiler fuses.
+// A warp takes `chunk` heads of q, k or v of a token, two at a time: a half-warp holds a head, a lane eight neighbouring values of it, the next pair of heads under way.
+// The transform's stages of 8, 16, 32 and 64 and the rotation's partner (64 values on, the lane 8 on) are shuffles; a group of 32 values is four lanes.  Rotation with every
+// product rounded, as elementary operations round it: which of two codes a value next to a border gets does not depend on what the compiler fuses.
+template <bool F32>
+struct EightRaw {
+    float4 a, b;                     // fp16: a alone
+    uint4 signs;
+};
 template <bool F32, bool TRANSFORM, int BITS>
 __global__ void __launch_bounds__(256) qkv_append_kernel(const AppendParams p) {
     pdl_allow_next_grid();
     const int lane = threadIdx.x & 31, half = lane >> 4, dl = lane & 15;
-    const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    const int64_t token = w / p.chunks;
-    const int first = (int)(w - token * p.chunks) * p.chunk, heads = p.hq + 2 * p.hkv;
+    const int64_t token = blockIdx.x;
+    int part = __shfl_sync(0xFFFFFFFFu, blockIdx.y * 8 + (threadIdx.x >> 5), 0);      // the same in all lanes, and known to be
+    if (part >= p.chunks) return;
+    const bool is_q = part < p.chunks_q, is_v = part >= p.chunks_q + p.chunks_kv;
+    part -= is_q ? 0 : is_v ? p.chunks_q + p.chunks_kv : p.chunks_q;
+    const int heads = is_q ? p.hq : p.hkv, base = is_q ? 0 : is_v ? p.hq + p.hkv : p.hq, first = part * p.chunk, end = min(first + p.chunk, heads);
     pdl_wait_prior_grids();
-    if (token >= p.tokens) return;                           // of a whole warp
     const int32_t *pos_p = after_wait(p.pos), *slot_p = after_wait(p.slots);
     const int pos = __ldg(pos_p + token);
     const int64_t slot = slot_p ? __ldg(slot_p + token) : token;
-    const bool takes = pos >= 0 && pos < p.max_pos && slot >= 0 && slot < p.rows;
+    const bool takes = __any_sync(0xFFFFFFFFu, pos >= 0 && pos < p.max_pos && slot >= 0 && slot < p.rows);
     if (!takes && pos != -1 && lane == 0) atomicExch(p.status, kStatusPosition);
-    float cs[8], sn[8];
-    if (takes) {
+    // Everything advances by two heads.  Of an odd number the last is taken by both halves of the warp, which read it before either writes.
+    int head = min(first + half, end - 1);
+    const char *x = reinterpret_cast<const char *>(p.x) + (token * p.ld_x + (base + head) * 128 + 8 * dl) * (F32 ? 4 : 2);
+    const __half *signs = p.signs + (base + head) * 128 + 8 * dl;
+    const bool writes = is_q || p.out_kv;
+    __half *out = p.out + token * p.ld_out + (base + head) * 128 + 8 * dl;
+    auto fetch = [&]() {
+        EightRaw<F32> r;
+        r.a = reinterpret_cast<const float4 *>(x)[0];
+        if (F32) r.b = reinterpret_cast<const float4 *>(x)[1];
+        r.signs = make_uint4(0u, 0u, 0u, 0u);
+        if (TRANSFORM && p.signs) r.signs = __ldg(reinterpret_cast<const uint4 *>(signs));
+        return r;
+    };
+    EightRaw<F32> next = fetch();
+    f32x2 cs[4], sn[4];                                      // sn: minus the sine where the partner is subtracted
+    if (takes && !is_v) {
         const float4 *a = reinterpret_cast<const float4 *>(p.angles + (int64_t)pos * 64 + 8 * (dl & 7));
+        const float sign = dl < 8 ? -1.f : 1.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const float4 v = __ldg(a + i);
-            cs[2 * i] = v.x, sn[2 * i] = v.y, cs[2 * i + 1] = v.z, sn[2 * i + 1] = v.w;
+            cs[i] = pack2(v.x, v.z), sn[i] = pack2(sign * v.y, sign * v.w);
         }
     }
-#pragma unroll 2
-    for (int h0 = first; h0 < min(first + p.chunk, heads); h0 += 2) {
-        const int head = h0 + half;
-        const bool there = head < heads;
-        float v[8] = {};
-        if (F32) {
-            if (there) load8_f32(const_cast<float *>(static_cast<const float *>(p.x)) + token * p.ld_x + head * 128 + 8 * dl, v, p.clear);
-        } else {
-            if (there) load8_f16(static_cast<const __half *>(p.x) + token * p.ld_x + head * 128 + 8 * dl, v);
+    f32x2 side[4];                                           // +-1: what this lane's value counts in the stages of the transform that are shuffles
+#pragma unroll
+    for (int m = 0; m < 4; ++m) side[m] = (dl >> m) & 1 ? pack2(-1.f, -1.f) : pack2(1.f, 1.f);
+    const int64_t at = BITS == 4 ? (slot * p.hkv + head) * p.max_pos + pos : (slot * p.max_pos + pos) * p.hkv + head;
+    uint8_t *cache = (is_v ? p.v : p.k) + (BITS == 4 ? at * kKv4Codes + 4 * (4 * (dl & 3)) + 2 * (dl >> 2) : at * 256 + 16 * dl);
+    __half2 *scales = BITS == 4 ? (is_v ? p.v_scales : p.k_scales) + at * 4 + (dl >> 2) : nullptr;
+#pragma unroll 1
+    for (int left = end - first; left > 0; left -= 2) {
+        const EightRaw<F32> raw = next;
+        if (F32 && p.clear) {
+            float4 *src = reinterpret_cast<float4 *>(const_cast<char *>(x));
+            src[0] = src[1] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
+        const int step = min(head + 2, end - 1) - head;
+        head += step;
+        x += step * 128 * (F32 ? 4 : 2);
+        signs += step * 128;
+        if (left > 2) next = fetch();
         if (!takes) continue;
-        if (TRANSFORM) {
-            float s[8];
-            unpack8(raw8_or_ones(p.signs && there ? p.signs + head * 128 + 8 * dl : nullptr), s);
-            fwht8(v, 128, nullptr);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __half2float(__float2half_rn(__fmul_rn(v[i] * p.scale, s[i])));
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __half2float(__float2half_rn(v[i] * p.scale));
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float o = __shfl_xor_sync(0xFFFFFFFFu, v[i], 8);
-            const float turned = dl < 8 ? __fsub_rn(__fmul_rn(v[i], cs[i]), __fmul_rn(o, sn[i])) : __fadd_rn(__fmul_rn(v[i], cs[i]), __fmul_rn(o, sn[i]));
-            if (head < p.hq + p.hkv) v[i] = __half2float(__float2half_rn(turned));
-        }
-        if (there && (head < p.hq || p.out_kv)) store8_f16(p.out + token * p.ld_out + head * 128 + 8 * dl, v);
-        const bool is_v = head >= p.hq + p.hkv, cached = there && head >= p.hq;
-        const int kvh = head - p.hq - (is_v ? p.hkv : 0);
-        if (BITS == 16) {
-            if (cached) store8_f16(reinterpret_cast<__half *>(is_v ? p.v : p.k) + ((slot * p.max_pos + pos) * p.hkv + kvh) * 128 + 8 * dl, v);
-        } else {
-            __half2 sm;
-            const uint32_t codes = kv4_quantise(v, sm);      // all lanes take part
-            if (cached) {
-                const int64_t at = (slot * p.hkv + kvh) * p.max_pos + pos;
-                const int group = dl >> 2, piece = 2 * (dl & 3);
-                unsigned short *c = reinterpret_cast<unsigned short *>((is_v ? p.v : p.k) + at * kKv4Codes) + 4 * piece + group;
-                c[0] = (unsigned short)codes;
-                c[4] = (unsigned short)(codes >> 16);
-                if ((dl & 3) == 0) (is_v ? p.v_scales : p.k_scales)[at * 4 + group] = sm;
+        f32x2 y[4];
+        {
+            float v[8];
+            if (F32) {
+                v[0] = raw.a.x, v[1] = raw.a.y, v[2] = raw.a.z, v[3] = raw.a.w, v[4] = raw.b.x, v[5] = raw.b.y, v[6] = raw.b.z, v[7] = raw.b.w;
+            } else {
+                unpack8(*reinterpret_cast<const uint4 *>(&raw.a), v);
             }
+            if (TRANSFORM) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const float a = v[i], b = v[i + 1];
+                    y[i / 2] = pack2(a + b, a - b);
+                }
+                const f32x2 a = add2(y[0], y[1]), b = sub2(y[0], y[1]), c = add2(y[2], y[3]), d = sub2(y[2], y[3]);
+                y[0] = add2(a, c), y[1] = add2(b, d), y[2] = sub2(a, c), y[3] = sub2(b, d);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = pack2(v[2 * i], v[2 * i + 1]);
+            }
+        }
+        if (TRANSFORM) {
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float a, b;
+                    unpack2(y[i], a, b);
+                    y[i] = fma2(y[i], side[m], pack2(__shfl_xor_sync(0xFFFFFFFFu, a, 1 << m), __shfl_xor_sync(0xFFFFFFFFu, b, 1 << m)));
+                }
+        }
+        const uint32_t bits[4] = {raw.signs.x, raw.signs.y, raw.signs.z, raw.signs.w}, scale = __float_as_uint(p.scale);
+        uint32_t o16[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {                        // the layer's fp16 output, then the rotation of q and k
+            float a, b;
+            unpack2(mul2(y[i], TRANSFORM ? pack2(__uint_as_float(scale ^ ((bits[i] << 16) & 0x80000000u)), __uint_as_float(scale ^ (bits[i] & 0x80000000u)))
+                                         : pack2(p.scale, p.scale)), a, b);
+            o16[i] = half2_as_u32(__floats2half2_rn(a, b));
+            if (!is_v) {
+                const float2 f = __half22float2(u32_as_half2(o16[i])), o = __half22float2(u32_as_half2(__shfl_xor_sync(0xFFFFFFFFu, o16[i], 8)));
+                unpack2(add2(mul2(pack2(f.x, f.y), cs[i]), mul2(pack2(o.x, o.y), sn[i])), a, b);
+                o16[i] = half2_as_u32(__floats2half2_rn(a, b));
+            }
+        }
+        const uint4 whole = make_uint4(o16[0], o16[1], o16[2], o16[3]);
+        if (writes) *reinterpret_cast<uint4 *>(out) = whole;
+        out += step * 128;
+        if (is_q) continue;
+        if (BITS == 16) {
+            *reinterpret_cast<uint4 *>(cache) = whole;
+            cache += step * 256;
+        } else {
+            float v[8];
+            __half2 sm;
+            unpack8(whole, v);
+            const uint32_t codes = kv4_quantise(v, sm);      // all lanes take part
+            unsigned short *c = reinterpret_cast<unsigned short *>(cache);          // pieces 2 (dl % 4) and the next
+            c[0] = (unsigned short)codes;
+            c[4] = (unsigned short)(codes >> 16);
+            if ((dl & 3) == 0) *scales = sm;
+            cache += step * p.max_pos * kKv4Codes;
+            scales += step * p.max_pos * 4;
         }
     }
 }
 
 template <bool F32, bool TRANSFORM>
 static int launch_append(const AppendParams &p, int bits, cudaStream_t s) {
-    const dim3 grid((unsigned)((p.tokens * p.chunks + 7) / 8));
+    const dim3 grid((unsigned)p.tokens, (unsigned)((p.chunks + 7) / 8));
     return bits == 4 ? launch(qkv_append_kernel<F32, TRANSFORM, 4>, grid, dim3(256), 0, s, p) : launch(qkv_append_kernel<F32, TRANSFORM, 16>, grid, dim3(256), 0, s, p);
 }
 
@@ -165,8 +227,12 @@ extern "C" int rptc_qkv_append(const rptc_append *a, rptc_stream_t stream) {
     p.k_scales = static_cast<__half2 *>(c.k_scales), p.v_scales = static_cast<__half2 *>(c.v_scales);
     p.rows = c.rows, p.max_pos = c.max_pos;
     p.hq = a->heads, p.hkv = c.kv_heads, p.clear = a->clear, p.out_kv = a->out_kv;
-    p.chunk = 2;
-    p.chunks = (p.hq + 2 * p.hkv + p.chunk - 1) / p.chunk;
+    // A warp's heads share their token's angles and place; where there are few tokens more warps are worth more (2048 tokens of 96 heads: two heads a warp 77.8 us, eight
+    // 51.0; 16 tokens 2.9 and 5.3).
+    const int64_t pairs = a->tokens * ((p.hq + 1) / 2 + 2 * ((p.hkv + 1) / 2));
+    p.chunk = pairs >= 4 * 24 * (int64_t)num_sms() ? 8 : pairs >= 2 * 24 * (int64_t)num_sms() ? 4 : 2;
+    p.chunks_q = (p.hq + p.chunk - 1) / p.chunk, p.chunks_kv = (p.hkv + p.chunk - 1) / p.chunk;
+    p.chunks = p.chunks_q + 2 * p.chunks_kv;
     p.scale = a->transform ? (float)((double)a->scale * 0.08838834764831845) : a->scale;
     p.status = device_status_word();
     if (!p.status) return RPTC_ERR_CUDA;
