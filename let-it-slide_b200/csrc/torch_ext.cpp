@@ -11,6 +11,9 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <algorithm>
+#include <cmath>
+#include <cstring>
 #include <exception>
 #include <optional>
 #include <string>
@@ -29,6 +32,13 @@ struct {
     decltype(&rptc_gemv_timed) gemv_timed;
     decltype(&rptc_dequantize) dequantize;
     decltype(&rptc_decompress) decompress;
+    decltype(&rptc_attn_prompt) attn_prompt;
+    decltype(&rptc_qkv_append) qkv_append;
+    decltype(&rptc_kv4_values) kv4_values;
+    decltype(&rptc_attn_decode_kv4_workspace_bytes) attn_decode_kv4_workspace_bytes;
+    decltype(&rptc_attn_decode_kv4) attn_decode_kv4;
+    decltype(&rptc_token_logprobs_workspace_bytes) token_logprobs_workspace_bytes;
+    decltype(&rptc_token_logprobs) token_logprobs;
 } g_lib;
 
 #define RPTC_NAMES(X) X(in_features) X(out_features) X(block_in) X(block_out) X(scale) X(fmt) X(_buffers) X(codes) X(lut) X(carry_in) \
@@ -315,32 +325,261 @@ PyObject *decompress(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     });
 }
 
-// bind(linear_workspace_bytes, linear_forward, packed_workspace_bytes, packed_forward, gemv_timed, dequantize, decompress): addresses
+// ---- the serving operators.  None for what is not as the kernels read it: the caller refuses it, and says why. ----
+const at::Tensor *tensor_or_null(PyObject *o) { return THPVariable_Check(o) ? &THPVariable_Unpack(o) : nullptr; }
+// A tensor on `device` of `type`, contiguous in `shape`.
+bool is(const at::Tensor *t, c10::Device device, at::ScalarType type, at::IntArrayRef shape) {
+    return t && t->device() == device && t->scalar_type() == type && t->sizes() == shape && t->is_contiguous();
+}
+// Rows of at least `width` values with unit column stride; `ld` what is between them.
+bool is_rows(const at::Tensor *t, c10::Device device, int64_t rows, int64_t width, int64_t &ld) {
+    if (!t || t->device() != device || t->dim() != 2 || t->size(0) != rows || t->size(1) < width || (t->stride(1) != 1 && t->size(1) > 1)) return false;
+    ld = rows > 1 ? t->stride(0) : std::max(t->size(1), t->stride(0));
+    return true;
+}
+bool whole(PyObject *o, int64_t &v) {
+    if (!PyLong_Check(o)) return false;
+    v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw PyError();
+    return true;
+}
+bool number(PyObject *o, double none, float &v) {
+    const double d = o == Py_None ? none : PyFloat_AsDouble(o);
+    if (d == -1.0 && PyErr_Occurred()) throw PyError();
+    v = (float)d;
+    return true;
+}
+// (k, v) in fp16, or (k codes, k scales, v codes, v scales).
+bool cache_of(PyObject *o, rptc_kv_cache &c, const at::Tensor *(&t)[4]) {
+    if (!PyTuple_Check(o)) return false;
+    const Py_ssize_t n = PyTuple_GET_SIZE(o);
+    if (n != 2 && n != 4) return false;
+    for (Py_ssize_t i = 0; i < n; ++i)
+        if (!(t[i] = tensor_or_null(PyTuple_GET_ITEM(o, i)))) return false;
+    const at::Tensor &k = *t[0];
+    if (!k.is_cuda() || k.dim() != 4 || k.numel() == 0) return false;
+    if (n == 2) {
+        if (k.size(3) != 128 || !is(t[0], k.device(), at::kHalf, k.sizes()) || !is(t[1], k.device(), at::kHalf, k.sizes())) return false;
+        c = {t[0]->data_ptr(), nullptr, t[1]->data_ptr(), nullptr, k.size(0), k.size(1), (int32_t)k.size(2), 16};
+        return true;
+    }
+    const int64_t shape[5] = {k.size(0), k.size(1), k.size(2), 4, 2};
+    if (k.size(3) != 64) return false;
+    for (int i = 0; i < 4; ++i)
+        if (i % 2 ? !is(t[i], k.device(), at::kHalf, at::IntArrayRef(shape, 5)) : !is(t[i], k.device(), at::kByte, k.sizes())) return false;
+    c = {t[0]->data_ptr(), t[1]->data_ptr(), t[2]->data_ptr(), t[3]->data_ptr(), k.size(0), k.size(2), (int32_t)k.size(1), 4};
+    return true;
+}
+
+// attn_prompt(q, k, v, starts, kv_first, kv_len, out, scale)
+PyObject *attn_prompt(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject * {
+        if (nargs != 8) fail("attn_prompt(q, k, v, starts, kv_first, kv_len, out, scale)");
+        const at::Tensor *q = tensor_or_null(args[0]), *k = tensor_or_null(args[1]), *v = tensor_or_null(args[2]), *starts = tensor_or_null(args[3]);
+        if (!q || !k || !v || !starts || !q->is_cuda() || q->dim() != 3 || k->dim() != 3 || v->sizes() != k->sizes() || k->size(2) != q->size(2) ||
+            q->size(0) == 0 || k->size(0) == 0 || q->stride(2) != 1 || k->stride(2) != 1 || v->stride(2) != 1)
+            Py_RETURN_NONE;
+        const at::ScalarType type = q->scalar_type();
+        const c10::Device device = q->device();
+        if ((type != at::kHalf && type != at::kBFloat16) || k->scalar_type() != type || v->scalar_type() != type || k->device() != device || v->device() != device) Py_RETURN_NONE;
+        if (starts->dim() != 1 || starts->size(0) < 2 || !is(starts, device, at::kInt, starts->sizes())) Py_RETURN_NONE;
+        rptc_prompt_attention a = {};
+        a.sequences = starts->size(0) - 1;
+        a.starts = static_cast<const int32_t *>(starts->data_ptr());
+        if ((args[4] == Py_None) != (args[5] == Py_None)) Py_RETURN_NONE;
+        if (args[4] != Py_None) {
+            const at::Tensor *first = tensor_or_null(args[4]), *count = tensor_or_null(args[5]);
+            if (!is(first, device, at::kInt, {a.sequences}) || !is(count, device, at::kInt, {a.sequences})) Py_RETURN_NONE;
+            a.kv_first = static_cast<const int32_t *>(first->data_ptr()), a.kv_len = static_cast<const int32_t *>(count->data_ptr());
+        }
+        const at::Tensor *given = args[6] == Py_None ? nullptr : tensor_or_null(args[6]);
+        if (args[6] != Py_None && (!given || given->device() != device || given->scalar_type() != type || given->sizes() != q->sizes() || given->stride(2) != 1)) Py_RETURN_NONE;
+        a.tokens = q->size(0), a.kv_tokens = k->size(0), a.heads = (int32_t)q->size(1), a.kv_heads = (int32_t)k->size(1), a.d = (int32_t)q->size(2);
+        a.dtype = type == at::kBFloat16;
+        if (!number(args[7], 1.0 / std::sqrt((double)std::max(a.d, 1)), a.scale)) Py_RETURN_NONE;
+        const c10::cuda::OptionalCUDAGuard guard(device);
+        at::Tensor out = given ? *given : at::empty(q->sizes(), at::TensorOptions().dtype(type).device(device));
+        const auto strides = [&](const at::Tensor &t, int64_t &row, int64_t &head) {      // of an axis of one element any
+            row = t.size(0) > 1 ? t.stride(0) : t.size(1) * a.d, head = t.size(1) > 1 ? t.stride(1) : a.d;
+        };
+        strides(*q, a.q_row, a.q_head), strides(*k, a.k_row, a.k_head), strides(*v, a.v_row, a.v_head), strides(out, a.out_row, a.out_head);
+        a.q = q->data_ptr(), a.k = k->data_ptr(), a.v = v->data_ptr(), a.out = out.data_ptr();
+        const cudaStream_t s = current_stream(*q);
+        int status;
+        Py_BEGIN_ALLOW_THREADS
+        status = g_lib.attn_prompt(&a, s);
+        Py_END_ALLOW_THREADS
+        return status == RPTC_OK ? THPVariable_Wrap(std::move(out)) : PyLong_FromLong(status);
+    });
+}
+
+// qkv_append(x, pos, angles, cache, heads, kv_heads, slots, signs_out, scale, transform, out, clear)
+PyObject *qkv_append(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject * {
+        if (nargs != 12) fail("qkv_append(x, pos, angles, cache, heads, kv_heads, slots, signs_out, scale, transform, out, clear)");
+        rptc_append a = {};
+        const at::Tensor *held[4], *x = tensor_or_null(args[0]), *angles = tensor_or_null(args[2]);
+        int64_t heads, kv_heads;
+        if (!x || !x->is_cuda() || x->dim() != 2 || x->size(0) == 0 || !cache_of(args[3], a.cache, held) || !whole(args[4], heads) || !whole(args[5], kv_heads)) Py_RETURN_NONE;
+        const c10::Device device = x->device();
+        if (held[0]->device() != device || heads <= 0 || heads > 4096 || kv_heads != a.cache.kv_heads) Py_RETURN_NONE;
+        const int64_t width = (heads + 2 * kv_heads) * 128;
+        a.tokens = x->size(0), a.heads = (int32_t)heads;
+        a.x_is_f32 = x->scalar_type() == at::kFloat;
+        if ((!a.x_is_f32 && x->scalar_type() != at::kHalf) || !is_rows(x, device, a.tokens, width, a.ld_x)) Py_RETURN_NONE;
+        const at::Tensor *pos = tensor_or_null(args[1]);
+        if (!is(pos, device, at::kInt, {a.tokens}) || !angles || angles->dim() != 3 || angles->size(0) < a.cache.max_pos ||
+            !is(angles, device, at::kFloat, {angles->size(0), 64, 2}))
+            Py_RETURN_NONE;
+        a.pos = static_cast<const int32_t *>(pos->data_ptr()), a.angles = static_cast<const float *>(angles->data_ptr());
+        if (args[6] != Py_None) {
+            const at::Tensor *slots = tensor_or_null(args[6]);
+            if (!is(slots, device, at::kInt, {a.tokens})) Py_RETURN_NONE;
+            a.slots = static_cast<const int32_t *>(slots->data_ptr());
+        }
+        if (args[7] != Py_None) {
+            const at::Tensor *signs = tensor_or_null(args[7]);
+            if (!is(signs, device, at::kHalf, {width})) Py_RETURN_NONE;
+            a.signs_out = signs->data_ptr();
+        }
+        if (!number(args[8], 1.0, a.scale)) Py_RETURN_NONE;
+        const int transform = PyObject_IsTrue(args[9]), clear = PyObject_IsTrue(args[11]);
+        if (transform < 0 || clear < 0) throw PyError();
+        a.transform = transform, a.clear = clear;
+        const at::Tensor *given = args[10] == Py_None ? nullptr : tensor_or_null(args[10]);
+        if (args[10] != Py_None && (!given || given->scalar_type() != at::kHalf || !is_rows(given, device, a.tokens, heads * 128, a.ld_out))) Py_RETURN_NONE;
+        const c10::cuda::OptionalCUDAGuard guard(device);
+        at::Tensor out = given ? *given : at::empty({a.tokens, width}, at::TensorOptions().dtype(at::kHalf).device(device));
+        if (!given) a.ld_out = width;
+        a.out_kv = out.size(1) >= width;
+        a.x = x->data_ptr(), a.out = out.data_ptr();
+        const cudaStream_t s = current_stream(*x);
+        int status;
+        Py_BEGIN_ALLOW_THREADS
+        status = g_lib.qkv_append(&a, s);
+        Py_END_ALLOW_THREADS
+        return status == RPTC_OK ? THPVariable_Wrap(std::move(out)) : PyLong_FromLong(status);
+    });
+}
+
+// kv4_values(cache, count, out): (k, v)
+PyObject *kv4_values(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject * {
+        if (nargs != 3) fail("kv4_values(cache, count, out)");
+        rptc_kv_cache c;
+        const at::Tensor *held[4], *count = tensor_or_null(args[1]);
+        if (!cache_of(args[0], c, held) || c.bits != 4) Py_RETURN_NONE;
+        const c10::Device device = held[0]->device();
+        if (!is(count, device, at::kInt, {c.rows})) Py_RETURN_NONE;
+        const int64_t shape[4] = {c.rows, c.max_pos, c.kv_heads, 128};
+        at::Tensor out[2];
+        const c10::cuda::OptionalCUDAGuard guard(device);
+        for (int i = 0; i < 2; ++i) {
+            if (args[2] == Py_None) {
+                out[i] = at::empty(at::IntArrayRef(shape, 4), at::TensorOptions().dtype(at::kHalf).device(device));
+            } else {
+                if (!PyTuple_Check(args[2]) || PyTuple_GET_SIZE(args[2]) != 2) Py_RETURN_NONE;
+                const at::Tensor *t = tensor_or_null(PyTuple_GET_ITEM(args[2], i));
+                if (!is(t, device, at::kHalf, at::IntArrayRef(shape, 4))) Py_RETURN_NONE;
+                out[i] = *t;
+            }
+        }
+        const cudaStream_t s = current_stream(*held[0]);
+        int status;
+        Py_BEGIN_ALLOW_THREADS
+        status = g_lib.kv4_values(&c, static_cast<const int32_t *>(count->data_ptr()), out[0].data_ptr(), out[1].data_ptr(), s);
+        Py_END_ALLOW_THREADS
+        if (status != RPTC_OK) return PyLong_FromLong(status);
+        return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(out[0])), THPVariable_Wrap(std::move(out[1])));
+    });
+}
+
+// attn_decode_kv4(q, pos, cache, heads, out, scale, signs_in)
+PyObject *attn_decode_kv4(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject * {
+        if (nargs != 7) fail("attn_decode_kv4(q, pos, cache, heads, out, scale, signs_in)");
+        rptc_kv_cache c;
+        const at::Tensor *held[4], *q = tensor_or_null(args[0]), *pos = tensor_or_null(args[1]);
+        int64_t heads, ld_q, ld_out = 0;
+        if (!cache_of(args[2], c, held) || c.bits != 4 || !whole(args[3], heads) || heads <= 0 || heads > 4096) Py_RETURN_NONE;
+        const c10::Device device = held[0]->device();
+        if (!is_rows(q, device, c.rows, heads * 128, ld_q) || q->scalar_type() != at::kHalf || !is(pos, device, at::kInt, {c.rows})) Py_RETURN_NONE;
+        const at::Tensor *given = args[4] == Py_None ? nullptr : tensor_or_null(args[4]), *signs = args[6] == Py_None ? nullptr : tensor_or_null(args[6]);
+        if (args[4] != Py_None && (!given || given->scalar_type() != at::kHalf || !is_rows(given, device, c.rows, heads * 128, ld_out))) Py_RETURN_NONE;
+        if (args[6] != Py_None && !is(signs, device, at::kHalf, {heads * 128})) Py_RETURN_NONE;
+        float scale;
+        if (!number(args[5], 0.08838834764831845, scale)) Py_RETURN_NONE;
+        const c10::cuda::OptionalCUDAGuard guard(device);
+        at::Tensor out = given ? *given : at::empty({c.rows, heads * 128}, at::TensorOptions().dtype(at::kHalf).device(device));
+        if (!given) ld_out = heads * 128;
+        const int64_t need = g_lib.attn_decode_kv4_workspace_bytes(&c, (int)heads);
+        at::Tensor ws;
+        if (need > 0) ws = at::empty({need}, at::TensorOptions().dtype(at::kByte).device(device));
+        const cudaStream_t s = current_stream(*q);
+        int status;
+        Py_BEGIN_ALLOW_THREADS
+        status = g_lib.attn_decode_kv4(q->data_ptr(), ld_q, static_cast<const int32_t *>(pos->data_ptr()), &c, out.data_ptr(), ld_out, (int)heads, scale,
+                                       signs ? signs->data_ptr() : nullptr, need > 0 ? ws.data_ptr() : nullptr, need, s);
+        Py_END_ALLOW_THREADS
+        return status == RPTC_OK ? THPVariable_Wrap(std::move(out)) : PyLong_FromLong(status);
+    });
+}
+
+// token_logprobs(logits, targets, top): (logprob or None, entropy, top_logprobs, top_ids)
+PyObject *token_logprobs(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
+    return guarded([&]() -> PyObject * {
+        if (nargs != 3) fail("token_logprobs(logits, targets, top)");
+        const at::Tensor *x = tensor_or_null(args[0]), *targets = args[1] == Py_None ? nullptr : tensor_or_null(args[1]);
+        int64_t top, ld;
+        if (!x || !x->is_cuda() || x->dim() != 2 || x->size(0) == 0 || x->size(1) == 0 || !whole(args[2], top)) Py_RETURN_NONE;
+        const c10::Device device = x->device();
+        const int64_t rows = x->size(0), n = x->size(1);
+        const at::ScalarType type = x->scalar_type();
+        const int dtype = type == at::kHalf ? 0 : type == at::kBFloat16 ? 1 : type == at::kFloat ? 2 : -1;
+        if (dtype < 0 || top < 0 || top > 32 || top > n || !is_rows(x, device, rows, n, ld) || (args[1] != Py_None && !is(targets, device, at::kLong, {rows}))) Py_RETURN_NONE;
+        const c10::cuda::OptionalCUDAGuard guard(device);
+        const auto f32 = at::TensorOptions().dtype(at::kFloat).device(device);
+        at::Tensor logprob, entropy = at::empty({rows}, f32), best = at::empty({rows, top}, f32), ids = at::empty({rows, top}, f32.dtype(at::kLong)), ws;
+        if (targets) logprob = at::empty({rows}, f32);
+        const int64_t need = g_lib.token_logprobs_workspace_bytes(rows, n, (int)top);
+        if (need > 0) ws = at::empty({need}, f32.dtype(at::kByte));
+        const cudaStream_t s = current_stream(*x);
+        int status;
+        Py_BEGIN_ALLOW_THREADS
+        status = g_lib.token_logprobs(x->data_ptr(), dtype, ld, targets ? static_cast<const int64_t *>(targets->data_ptr()) : nullptr,
+                                      targets ? static_cast<float *>(logprob.data_ptr()) : nullptr, static_cast<float *>(entropy.data_ptr()),
+                                      top ? static_cast<float *>(best.data_ptr()) : nullptr, top ? static_cast<int64_t *>(ids.data_ptr()) : nullptr, rows, n, (int)top,
+                                      need > 0 ? ws.data_ptr() : nullptr, need, s);
+        Py_END_ALLOW_THREADS
+        if (status != RPTC_OK) return PyLong_FromLong(status);
+        PyObject *first = targets ? THPVariable_Wrap(std::move(logprob)) : Py_NewRef(Py_None);
+        return Py_BuildValue("(NNNN)", first, THPVariable_Wrap(std::move(entropy)), THPVariable_Wrap(std::move(best)), THPVariable_Wrap(std::move(ids)));
+    });
+}
+
+// bind(addresses of the entry points, in the order of g_lib)
 PyObject *bind(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
     return guarded([&]() -> PyObject * {
-        if (nargs != 7) fail("bind(seven addresses)");
-        void *p[7];
-        for (int i = 0; i < 7; ++i) {
+        constexpr Py_ssize_t kEntries = sizeof(g_lib) / sizeof(void *);
+        if (nargs != kEntries) fail("bind(an address per entry point)");
+        void *p[kEntries];
+        for (Py_ssize_t i = 0; i < kEntries; ++i) {
             p[i] = PyLong_AsVoidPtr(args[i]);
             if (!p[i]) {
                 if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, "null address");
                 throw PyError();
             }
         }
-        g_lib.linear_workspace_bytes = reinterpret_cast<decltype(g_lib.linear_workspace_bytes)>(p[0]);
-        g_lib.linear_forward = reinterpret_cast<decltype(g_lib.linear_forward)>(p[1]);
-        g_lib.packed_workspace_bytes = reinterpret_cast<decltype(g_lib.packed_workspace_bytes)>(p[2]);
-        g_lib.packed_forward = reinterpret_cast<decltype(g_lib.packed_forward)>(p[3]);
-        g_lib.gemv_timed = reinterpret_cast<decltype(g_lib.gemv_timed)>(p[4]);
-        g_lib.dequantize = reinterpret_cast<decltype(g_lib.dequantize)>(p[5]);
-        g_lib.decompress = reinterpret_cast<decltype(g_lib.decompress)>(p[6]);
+        static_assert(sizeof(g_lib) == sizeof(p), "addresses alone");
+        memcpy(&g_lib, p, sizeof(p));
         Py_RETURN_NONE;
     });
 }
 
 #define RPTC_METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {RPTC_METHOD(bind), RPTC_METHOD(linear_forward), RPTC_METHOD(packed_forward), RPTC_METHOD(gemv_timed),
-                           RPTC_METHOD(dequantize), RPTC_METHOD(decompress), {nullptr, nullptr, 0, nullptr}};
+                           RPTC_METHOD(dequantize), RPTC_METHOD(decompress), RPTC_METHOD(attn_prompt), RPTC_METHOD(qkv_append), RPTC_METHOD(kv4_values),
+                           RPTC_METHOD(attn_decode_kv4), RPTC_METHOD(token_logprobs), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_native", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -256,7 +256,8 @@ def native():
         L = lib()
         ext.bind(*[ctypes.cast(getattr(L, "rptc_" + name), ctypes.c_void_p).value for name in (
             "linear_workspace_bytes", "linear_forward", "packed_workspace_bytes", "packed_forward", "gemv_timed",
-            "dequantize", "decompress")])
+            "dequantize", "decompress", "attn_prompt", "qkv_append", "kv4_values", "attn_decode_kv4_workspace_bytes", "attn_decode_kv4",
+            "token_logprobs_workspace_bytes", "token_logprobs")])
         _native = ext
     return _native
 

@@ -366,6 +366,13 @@ def _on(device: torch.device, name: str, t: torch.Tensor, dtype, shape: tuple | 
         raise RuntimeError(f"{name} must be contiguous {list(shape)}, got {list(t.shape)}")
 
 
+def _answer(result, where: str):
+    """What a native call gave: None where something is not as the kernels read it (checked and refused below the call)."""
+    if type(result) is int:
+        check(result, where)
+    return result
+
+
 def kv4_cache(rows: int, max_pos: int, kv_heads: int, device="cuda") -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """A layer's KV cache in 4 bits for 128-wide heads, empty: codes of k, (scale, minimum) of its groups of 32 values, the same
     for v (rptc_kv_cache); 160 bytes per position and kv head, where fp16 takes 512."""
@@ -405,6 +412,9 @@ def qkv_append(x: torch.Tensor, pos: torch.Tensor, angles: torch.Tensor, cache, 
     position, k and v appended to `cache` (fp16 pair or `kv4_cache`) at [slots[t], pos[t]] (slots None: row t; pos -1: a token of no
     sequence, nothing is written).  Returns fp16 [tokens, (heads + 2 kv_heads) * 128] with q, k and v as finished; an `out` of fewer columns
     takes q alone.  `clear` zeroes an fp32 x.  `out` may be x itself; otherwise the two do not overlap."""
+    done = _answer(native().qkv_append(x, pos, angles, cache, heads, kv_heads, slots, signs_out, scale, transform, out, clear), "rptc_qkv_append")
+    if done is not None:
+        return done
     device, width = x.device, (heads + 2 * kv_heads) * 128
     c = _kv_cache(cache, device)
     if heads <= 0 or kv_heads != c.kv_heads:
@@ -435,6 +445,9 @@ def qkv_append(x: torch.Tensor, pos: torch.Tensor, angles: torch.Tensor, cache, 
 def kv4_values(cache, count: torch.Tensor, out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The values that the first count[r] (int32 [rows]) positions of row r of a 4-bit cache stand for, fp16 k and v [rows, max_pos, kv_heads,
     128]; other positions are left as they are (rptc_kv4_values)."""
+    done = _answer(native().kv4_values(cache, count, out), "rptc_kv4_values")
+    if done is not None:
+        return done
     device = cache[0].device
     c = _kv_cache(cache, device)
     if c.bits != 4:
@@ -453,6 +466,9 @@ def attn_decode_kv4(q: torch.Tensor, pos: torch.Tensor, cache, heads: int, out: 
     """Single-query attention over positions 0 .. pos[r] of row r of a 4-bit cache (rptc_attn_decode_kv4): q fp16 [rows, >= heads * 128] ->
     fp16 [rows, heads * 128].  pos -1: a row of no sequence, zeros.  signs_in: each head's output also goes through the 128-wide input
     transform of the output projection."""
+    done = _answer(native().attn_decode_kv4(q, pos, cache, heads, out, scale, signs_in), "rptc_attn_decode_kv4")
+    if done is not None:
+        return done
     device = cache[0].device
     c = _kv_cache(cache, device)
     _rows_of("q", q, device, torch.float16, c.rows, heads * 128)
@@ -477,6 +493,9 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch
     bf16, d 64 or 128, unit stride along d -> out [tokens, heads, d].  Sequence s has the queries starts[s] .. starts[s + 1] - 1 (int32
     [sequences + 1]) and, for prompts that continue a cached context, the keys kv_first[s] .. kv_first[s] + kv_len[s] - 1 (int32 [sequences]; None:
     its keys lie where its queries do); its last query sees all of them.  Rows of `out` behind the last sequence are left as they are."""
+    done = _answer(native().attn_prompt(q, k, v, starts, kv_first, kv_len, out, scale), "rptc_attn_prompt")
+    if done is not None:
+        return done
     device = q.device
     for name, t in (("q", q), ("k", k), ("v", v)):
         _on(device, name, t, (torch.float16, torch.bfloat16))
@@ -520,6 +539,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     """Log probabilities of given tokens, with entropy and alternatives (rptc_token_logprobs): logits fp16, bf16 or fp32 [rows, n], targets int64
     [rows] (-1: no token, 0) -> (logprob fp32 [rows] or None, entropy fp32 [rows], top_logprobs fp32 [rows, top], top_ids int64 [rows, top], the
     largest first, equal ones by their index).  -inf is a forbidden token."""
+    done = _answer(native().token_logprobs(logits, targets, top), "rptc_token_logprobs")
+    if done is not None:
+        return done
     device = logits.device
     _on(device, "logits", logits, tuple(_LOGIT_TYPES))
     if logits.dim() != 2 or logits.shape[1] < 1 or (logits.stride(1) != 1 and logits.shape[1] > 1):
