@@ -78,8 +78,10 @@ class RPTCLlama:
     """Random-init Llama-shape model with all block linears RPTC-quantised; batch-`rows` decode."""
 
     def __init__(self, cfg: LlamaConfig, fmt: Format | None = None, rows: int = 1, seed: int = 0, device="cuda",
-                 incoherent: bool = True, tp_world: int = 1, tp_rank: int = 0, tp_group=None, peer_allreduce: bool = False):
-        """tp_world > 1: this object is rank `tp_rank`'s shard of a tensor-parallel model; the partial
+                 incoherent: bool = True, tp_world: int = 1, tp_rank: int = 0, tp_group=None, peer_allreduce: bool = False, kv_bits: int = 16):
+        """kv_bits: 16 keeps keys and values in fp16, 4 in 4 bits (`ops.kv4_cache`; 160 bytes per position and kv head instead of 512, heads of 128).
+
+        tp_world > 1: this object is rank `tp_rank`'s shard of a tensor-parallel model; the partial
         outputs of the row-parallel layers (o, down) are summed over `tp_group` with an NCCL all-reduce.
         Embedding, norms and output head are replicated (same seed on every rank)."""
         self.cfg, self.rows, self.device = cfg, rows, torch.device(device)
@@ -96,8 +98,16 @@ class RPTCLlama:
         self.heads_l, self.kv_heads_l, self.ffn_l = cfg.heads // tp_world, cfg.kv_heads // tp_world, cfg.ffn // tp_world
         q, kv = self.heads_l * cfg.head_dim, self.kv_heads_l * cfg.head_dim
         f16 = dict(dtype=torch.float16, device=device)
-        self.kcache = [torch.zeros((rows, cfg.max_pos, self.kv_heads_l, cfg.head_dim), **f16) for _ in range(cfg.layers)]
-        self.vcache = [torch.zeros((rows, cfg.max_pos, self.kv_heads_l, cfg.head_dim), **f16) for _ in range(cfg.layers)]
+        if kv_bits not in (4, 16) or (kv_bits == 4 and cfg.head_dim != 128):
+            raise ValueError("kv_bits must be 16, or 4 with heads of 128")
+        self.kv_bits = kv_bits
+        self.kcache = self.vcache = self.kv4 = None
+        if kv_bits == 16:
+            self.kcache = [torch.zeros((rows, cfg.max_pos, self.kv_heads_l, cfg.head_dim), **f16) for _ in range(cfg.layers)]
+            self.vcache = [torch.zeros((rows, cfg.max_pos, self.kv_heads_l, cfg.head_dim), **f16) for _ in range(cfg.layers)]
+        else:
+            self.kv4 = [ops.kv4_cache(rows, cfg.max_pos, self.kv_heads_l, self.device) for _ in range(cfg.layers)]
+        self._angles: torch.Tensor | None = None       # see _rope_table
         # step workspace (fixed addresses, so that the step can live in a CUDA graph)
         self.ids = torch.zeros(rows, dtype=torch.int32, device=device)
         self.pos = torch.zeros(rows, dtype=torch.int32, device=device)
@@ -171,7 +181,11 @@ class RPTCLlama:
 
     def _extra_launches(self) -> int:
         """Launches beyond one per matvec: the output head takes up to sixteen activation rows per launch."""
-        return (self.rows - 1) // 16
+        return (self.rows - 1) // 16 + self._join_launches()
+
+    def _join_launches(self) -> int:
+        """Attention over long 4-bit caches joins the parts of a context in a launch of its own."""
+        return len(self.blocks) if self.kv_bits == 4 and self.cfg.max_pos > 1024 else 0
 
     def step_eager(self) -> None:
         if self._glueable():
@@ -182,6 +196,29 @@ class RPTCLlama:
             self._step_fused()
         else:
             self._step_unfused()
+
+    def _rope_table(self) -> torch.Tensor:
+        """Cosines and sines of all positions, made once (before a capture: `capture` runs a step first)."""
+        if self._angles is None:
+            self._angles = ops.rope_angles(self.cfg.max_pos, self.cfg.rope_theta, self.device)
+        return self._angles
+
+    def _cache(self, i: int) -> tuple:
+        return self.kv4[i] if self.kv_bits == 4 else (self.kcache[i], self.vcache[i])
+
+    def _attend(self, i: int, b: "Block") -> None:
+        """One token per row, from the qkv layer's accumulator to the attention's output behind the output projection's per-head input
+        transform: q, k, v finished, rotated, k and v appended to the cache, attention over it."""
+        cfg = self.cfg
+        if self.kv_bits == 4:
+            ops.qkv_append(self.acc_qkv, self.pos, self._rope_table(), self.kv4[i], self.heads_l, self.kv_heads_l, signs_out=b.qkv.signs_out, scale=b.qkv.scale,
+                           transform=True, out=self.qkv_out[:, : self.heads_l * cfg.head_dim], clear=True)
+            ops.attn_decode_kv4(self.qkv_out, self.pos, self.kv4[i], self.heads_l, out=self.attn, signs_in=b.o.signs_in)
+            return
+        ops.qkv_finish(self.acc_qkv, b.qkv.signs_out, b.qkv.scale, self.qkv_out, self.kcache[i], self.vcache[i], self.pos,
+                       self.heads_l, self.kv_heads_l, b.qkv.block_out, cfg.rope_theta)
+        ops.attn_decode(self.qkv_out, self.pos, self.kcache[i], self.vcache[i], self.attn, self.heads_l, self.kv_heads_l,
+                        cfg.head_dim, signs_in=b.o.signs_in)
 
     def _embed_ids(self) -> None:
         if self.mailbox is not None:
@@ -208,15 +245,12 @@ class RPTCLlama:
                      and self.fmt.K in (2, 4))
         for i, b in enumerate(self.blocks):
             b.qkv.matvec_acc(xt, self.acc_qkv)
-            if self.fuse_attention and self.heads_l == self.kv_heads_l and b.qkv.block_out == 128:
+            if self.fuse_attention and self.kv_bits == 16 and self.heads_l == self.kv_heads_l and b.qkv.block_out == 128:
                 ops.qkv_attn_decode(self.acc_qkv, b.qkv.signs_out, b.qkv.scale, self.pos, self.kcache[i], self.vcache[i], self.attn,
                                     self.heads_l, self.kv_heads_l, cfg.rope_theta, b.o.signs_in)
                 n_launch -= 1
             else:
-                ops.qkv_finish(self.acc_qkv, b.qkv.signs_out, b.qkv.scale, self.qkv_out, self.kcache[i], self.vcache[i], self.pos,
-                               self.heads_l, self.kv_heads_l, b.qkv.block_out, cfg.rope_theta)
-                ops.attn_decode(self.qkv_out, self.pos, self.kcache[i], self.vcache[i], self.attn, self.heads_l, self.kv_heads_l,
-                                cfg.head_dim, signs_in=b.o.signs_in)
+                self._attend(i, b)
             b.o.matvec_acc(self.attn, self.acc_h)
             ops.finish_norm_hadamard(self.acc_h, b.o.signs_out, b.o.scale, self.h, b.norm2, cfg.rms_eps, b.gate_up.signs_in, True, xt)
             if mlp_glued:
@@ -253,7 +287,7 @@ class RPTCLlama:
         cfg, r = self.cfg, self.rows
         self._embed_ids()
         mlp_glued = self._mlp_glueable()
-        mha = self.fuse_attention and self.blocks[0].qkv.block_out == 128 and cfg.head_dim == 128
+        mha = self.fuse_attention and self.kv_bits == 16 and self.blocks[0].qkv.block_out == 128 and cfg.head_dim == 128
         gqa = self.heads_l != self.kv_heads_l
         # the launch that opens a block zeroes what the block before it left: acc_o always, acc_gu too when the down
         # projection reads it in every CTA
@@ -267,10 +301,7 @@ class RPTCLlama:
                 ops.qkv_attn_decode(self.acc_qkv, b.qkv.signs_out, b.qkv.scale, self.pos, self.kcache[i], self.vcache[i], self.attn,
                                     self.heads_l, self.kv_heads_l, cfg.rope_theta, b.o.signs_in)
             else:
-                ops.qkv_finish(self.acc_qkv, b.qkv.signs_out, b.qkv.scale, self.qkv_out, self.kcache[i], self.vcache[i], self.pos,
-                               self.heads_l, self.kv_heads_l, b.qkv.block_out, cfg.rope_theta)
-                ops.attn_decode(self.qkv_out, self.pos, self.kcache[i], self.vcache[i], self.attn, self.heads_l, self.kv_heads_l,
-                                cfg.head_dim, signs_in=b.o.signs_in)
+                self._attend(i, b)
             b.o.matvec_acc(self.attn, self.acc_o)
             # acc_h was consumed by this block's first launch; with grouped-query attention acc_qkv is zeroed here too
             stale_h = self._acc_pool2 if (mha and gqa) else (self.acc_h if i else None)
@@ -289,7 +320,7 @@ class RPTCLlama:
         ops.finish_norm_hadamard(self.acc_h, last.signs_out, last.scale, self.h, self.norm_f, cfg.rms_eps, None, False, self.xn)
         ops.dense_gemv(self.head, self.xn, out=self.logits)
         self._next_token()
-        self.launches_per_step = ((5 if mlp_glued else 6) + (0 if mha else 1)) * len(self.blocks) + 4
+        self.launches_per_step = ((5 if mlp_glued else 6) + (0 if mha else 1)) * len(self.blocks) + 4 + self._join_launches()
 
     def _step_fused_tp(self) -> None:
         """Tensor-parallel decode step with the glue fused as far as the all-reduce allows: RMSNorm + input transform in
@@ -314,10 +345,7 @@ class RPTCLlama:
         ops.finish_norm_hadamard(None, None, 1.0, self.h, b0.norm1, cfg.rms_eps, b0.qkv.signs_in, True, xt)
         for i, b in enumerate(self.blocks):
             b.qkv.matvec_acc(xt, self.acc_qkv)
-            ops.qkv_finish(self.acc_qkv, b.qkv.signs_out, b.qkv.scale, self.qkv_out, self.kcache[i], self.vcache[i], self.pos,
-                           self.heads_l, self.kv_heads_l, b.qkv.block_out, cfg.rope_theta)
-            ops.attn_decode(self.qkv_out, self.pos, self.kcache[i], self.vcache[i], self.attn, self.heads_l, self.kv_heads_l,
-                            cfg.head_dim, signs_in=b.o.signs_in)
+            self._attend(i, b)
             b.o.matvec_acc(self.attn, self.acc_h)
             self._finish_row_parallel(b.o)
             ops.finish_norm_hadamard(None, None, 1.0, self.h, b.norm2, cfg.rms_eps, b.gate_up.signs_in, True, xt)
@@ -349,7 +377,7 @@ class RPTCLlama:
         """The tensor-parallel chain with the norms inside the matvecs: qkv* -> attention (q/k/v finish inside or in
         front) -> o -> all-reduce -> gate-up* -> down (SwiGLU inside or in front) -> all-reduce."""
         cfg = self.cfg
-        fused_attn = self.fuse_attention and self.blocks[0].qkv.block_out == 128 and cfg.head_dim == 128
+        fused_attn = self.fuse_attention and self.kv_bits == 16 and self.blocks[0].qkv.block_out == 128 and cfg.head_dim == 128
         # grouped-query attention: the fused attention kernel leaves acc_qkv as it is and the gate-up launch zeroes it
         stale_qkv = self.acc_qkv if (fused_attn and self.heads_l != self.kv_heads_l) else None
         for i, b in enumerate(self.blocks):
@@ -358,10 +386,7 @@ class RPTCLlama:
                 ops.qkv_attn_decode(self.acc_qkv, b.qkv.signs_out, b.qkv.scale, self.pos, self.kcache[i], self.vcache[i], self.attn,
                                     self.heads_l, self.kv_heads_l, cfg.rope_theta, b.o.signs_in)
             else:
-                ops.qkv_finish(self.acc_qkv, b.qkv.signs_out, b.qkv.scale, self.qkv_out, self.kcache[i], self.vcache[i], self.pos,
-                               self.heads_l, self.kv_heads_l, b.qkv.block_out, cfg.rope_theta)
-                ops.attn_decode(self.qkv_out, self.pos, self.kcache[i], self.vcache[i], self.attn, self.heads_l, self.kv_heads_l,
-                                cfg.head_dim, signs_in=b.o.signs_in)
+                self._attend(i, b)
             b.o.matvec_acc(self.attn, self.acc_h)
             self._finish_row_parallel(b.o)
             if mlp_glued:
@@ -379,7 +404,7 @@ class RPTCLlama:
         ops.finish_norm_hadamard(None, None, 1.0, self.h, self.norm_f, cfg.rms_eps, None, False, self.xn)
         ops.dense_gemv(self.head, self.xn, out=self.logits)
         self._next_token()
-        self.launches_per_step = ((6 if mlp_glued else 7) - (1 if fused_attn else 0) + 2 * per_reduce) * len(self.blocks) + 4
+        self.launches_per_step = ((6 if mlp_glued else 7) - (1 if fused_attn else 0) + 2 * per_reduce) * len(self.blocks) + 4 + self._join_launches()
 
     def _step_unfused(self) -> None:
         cfg, r = self.cfg, self.rows
@@ -391,10 +416,14 @@ class RPTCLlama:
             xt = b.qkv.transform_in(self.xn, out=self.xt[:, : cfg.hidden])
             b.qkv.matvec_acc(xt, self.acc_qkv)
             b.qkv.finish(self.acc_qkv, out=self.qkv_out)
-            ops.rope_cache(self.qkv_out, self.pos, self.kcache[i], self.vcache[i], self.heads_l, self.kv_heads_l, cfg.head_dim,
-                           cfg.rope_theta)
-            ops.attn_decode(self.qkv_out, self.pos, self.kcache[i], self.vcache[i], self.attn, self.heads_l, self.kv_heads_l,
-                            cfg.head_dim)
+            if self.kv_bits == 4:
+                ops.qkv_append(self.qkv_out, self.pos, self._rope_table(), self.kv4[i], self.heads_l, self.kv_heads_l, out=self.qkv_out)
+                ops.attn_decode_kv4(self.qkv_out, self.pos, self.kv4[i], self.heads_l, out=self.attn)
+            else:
+                ops.rope_cache(self.qkv_out, self.pos, self.kcache[i], self.vcache[i], self.heads_l, self.kv_heads_l, cfg.head_dim,
+                               cfg.rope_theta)
+                ops.attn_decode(self.qkv_out, self.pos, self.kcache[i], self.vcache[i], self.attn, self.heads_l, self.kv_heads_l,
+                                cfg.head_dim)
             xt = b.o.transform_in(self.attn, out=self.xt[:, : self.attn.shape[1]])
             b.o.matvec_acc(xt, self.acc_h)
             self._finish_row_parallel(b.o)
@@ -509,10 +538,10 @@ class RPTCLlama:
         cfg = self.cfg
         packed = cfg.quantised_weights() * self.fmt.K // 8 // self.tp_world
         head = cfg.vocab * cfg.hidden * 2
-        kv = 2 * cfg.layers * context * self.kv_heads_l * cfg.head_dim * 2
+        kv = cfg.layers * context * self.kv_heads_l * (160 if self.kv_bits == 4 else 4 * cfg.head_dim)
         return {"packed": packed, "head": head, "kv": kv}
 
-    # -- dense fp32 reference of the same model (decode weights with the GPU's bit-exact decompress) --------
+    # -- prompts ---------------------------------------------------------------------------------------------
     @torch.no_grad()
     def prefill(self, tokens: torch.Tensor) -> torch.Tensor:
         """Pushes a whole prompt `tokens` [rows, T] through the network in one pass: every block linear runs as the
@@ -520,13 +549,124 @@ class RPTCLlama:
         0..T-1, `pos` is set to T and `ids` to the greedy choice after the last prompt token.  Returns the logits of
         the last position, fp16 [rows, vocab].  Attention over the prompt is torch's scaled_dot_product_attention;
         norms, transforms, RoPE + cache writes, residual adds and the gated-MLP middle are this library's glue
-        kernels; decoding continues with `step`."""
+        kernels; decoding continues with `step`.  With a 4-bit cache it is `prefill_packed` of equally long prompts."""
         cfg = self.cfg
         R, T = tokens.shape
         if R != self.rows or T > cfg.max_pos:
             raise ValueError("tokens must be [rows, T] with T <= max_pos")
-        D = cfg.head_dim
+        if self.kv_bits == 4:
+            return self.prefill_packed(list(tokens))
         h = self.embed[tokens.long()].reshape(R * T, cfg.hidden)                     # fp16 residual stream
+        D = cfg.head_dim
+        heads_of_128 = D == 128 and self.blocks[0].qkv.block_out == 128
+        angles = ops.rope_angles(T, cfg.rope_theta, h.device) if heads_of_128 else None
+
+        def attend(i, b, qkv, finished):
+            if not finished and heads_of_128:
+                ops.prompt_qkv(qkv, b.qkv.signs_out, b.qkv.scale, R, T, self.kcache[i], self.vcache[i], self.heads_l, self.kv_heads_l, angles)
+            else:
+                qkv = qkv if finished else b.qkv.finish_t(qkv)
+                ops.rope_cache_prompt(qkv, R, T, self.kcache[i], self.vcache[i], self.heads_l, self.kv_heads_l, D, cfg.rope_theta)
+            return self._prompt_attention(qkv, i, R, T)
+
+        last = self._prompt_blocks(h, attend, lambda t: t.view(R, T, -1)[:, -1].contiguous())
+        self.pos.fill_(T - 1)
+        self._pos_hi = T
+        return self._greedy(last)
+
+    def _greedy(self, last: torch.Tensor) -> torch.Tensor:
+        """Logits of the residual stream `last` [rows, hidden]; pos moves on by one, ids are the greedy choice."""
+        ops.rmsnorm(last, self.norm_f, self.xn, self.cfg.rms_eps)
+        ops.dense_gemv(self.head, self.xn, out=self.logits)
+        ops.next_token(self.logits, self.next_ids, self.ids, self.pos, None)
+        return self.logits
+
+    @torch.no_grad()
+    def prefill_packed(self, prompts: list[torch.Tensor]) -> torch.Tensor:
+        """`prefill` for prompts of different lengths: prompts[r] (whole numbers, at least one) goes into row r from position 0 on.  All tokens go
+        through the network packed, one prompt behind the other (`ops.attn_prompt`), so that nothing is padded.  Returns the logits behind each
+        prompt's last token, fp16 [rows, vocab]; `pos` is set to the lengths and `ids` to the greedy choices; decoding continues with `step`."""
+        self.reset()
+        return self._greedy(self._push(prompts, whole=False))
+
+    @torch.no_grad()
+    def extend(self, prompts: list[torch.Tensor]) -> torch.Tensor:
+        """`prefill_packed` behind what the rows hold already: row r continues at `pos[r]` (a further turn of a conversation).  The new
+        tokens attend over the cached positions as the cache holds them, their own among them."""
+        return self._greedy(self._push(prompts, whole=False))
+
+    @torch.no_grad()
+    def score(self, prompts: list[torch.Tensor], top: int = 0) -> list[tuple]:
+        """How probable the model finds given texts: for each prompt (any number of them) (logprob, entropy, top_logprobs, top_ids), entry t about token
+        t + 1 given the tokens up to t (`ops.token_logprobs`; one entry less than tokens).  The perplexity of a text is exp of minus the mean of
+        logprob.  Uses the rows' caches: the model is reset before and after."""
+        found = []
+        for p0 in range(0, len(prompts), self.rows):
+            group = [torch.as_tensor(p, device=self.device) for p in prompts[p0:p0 + self.rows]]
+            self.reset()
+            h = self._push(group, whole=True)
+            targets = torch.cat([torch.cat((p[1:].long(), p.new_full((1,), -1).long())) for p in group])
+            xn, outs = torch.empty_like(h), []
+            ops.rmsnorm(h, self.norm_f, xn, self.cfg.rms_eps)
+            for t0 in range(0, len(targets), 4096):              # the logits of so many tokens at a time
+                outs.append(ops.token_logprobs(xn[t0:t0 + 4096] @ self.head.t(), targets[t0:t0 + 4096], top))
+            columns = [torch.cat(c).split([len(p) for p in group]) for c in zip(*outs)]
+            found += [tuple(c[i][:-1] for c in columns) for i in range(len(group))]
+        self.reset()
+        return found
+
+    def _push(self, prompts: list[torch.Tensor], whole: bool) -> torch.Tensor:
+        """Tokens of prompts[r] behind what row r holds (the first len(prompts) rows), one packed pass.  Returns the residual stream behind the blocks, of
+        every token (`whole`) or of each prompt's last; `pos` is left at the last token's position."""
+        cfg, D = self.cfg, self.cfg.head_dim
+        prompts = [torch.as_tensor(p, device=self.device) for p in prompts]
+        lengths, n = [p.numel() for p in prompts], len(prompts)
+        if (n != self.rows and not (whole and 0 < n < self.rows)) or any(p.dim() != 1 or p.numel() == 0 or p.is_floating_point() for p in prompts):
+            raise ValueError("prompts must be one row of at least one token each, one for every row of the model")
+        if D != 128:
+            raise ValueError("packed prompts need heads of 128")
+        if self._pos_hi + max(lengths) > cfg.max_pos:
+            raise ValueError(f"{max(lengths)} tokens behind position {self._pos_hi}, but the KV caches hold max_pos = {cfg.max_pos} positions")
+        fresh = self._pos_hi == 0                                # no row holds anything
+        total = sum(lengths)
+        i32 = dict(dtype=torch.int32, device=self.device)
+        length = torch.tensor(lengths, **i32)
+        starts = torch.nn.functional.pad(length.cumsum(0, dtype=torch.int32), (1, 0))
+        slots = torch.arange(n, **i32).repeat_interleave(length, output_size=total)
+        past = self.pos[:n]
+        places = torch.arange(total, **i32) + (past - starts[:-1]).repeat_interleave(length, output_size=total)
+        kv_first, kv_len = torch.arange(n, **i32) * cfg.max_pos, past + length
+        angles = self._rope_table()
+        values = None
+        if not fresh and self.kv_bits == 4:                      # where the cached values are spelt out, layer by layer
+            values = tuple(torch.empty((self.rows, cfg.max_pos, self.kv_heads_l, D), dtype=torch.float16, device=self.device) for _ in range(2))
+            count = torch.nn.functional.pad(kv_len, (0, self.rows - n))
+        cut = (self.heads_l * D, self.kv_heads_l * D, self.kv_heads_l * D)
+
+        def attend(i, b, qkv, finished):
+            transform = not finished and b.qkv.block_out == 128
+            if not finished and not transform:
+                qkv, finished = b.qkv.finish_t(qkv), True
+            ops.qkv_append(qkv, places, angles, self._cache(i), self.heads_l, self.kv_heads_l, slots=slots, signs_out=b.qkv.signs_out if transform else None,
+                           scale=b.qkv.scale if transform else 1.0, transform=transform, out=qkv)
+            q, k, v = (s.unflatten(1, (-1, D)) for s in qkv.split(cut, dim=1))
+            if fresh:
+                return ops.attn_prompt(q, k, v, starts).flatten(1)
+            k, v = ops.kv4_values(self.kv4[i], count, values) if self.kv_bits == 4 else (self.kcache[i], self.vcache[i])
+            return ops.attn_prompt(q, k.flatten(0, 1), v.flatten(0, 1), starts, kv_first, kv_len).flatten(1)
+
+        h = self.embed[torch.cat([p.long() for p in prompts])]
+        last = (starts[1:] - 1).long()
+        out = self._prompt_blocks(h, attend, (lambda t: t) if whole else (lambda t: t[last]))
+        self.pos[:n] += length - 1
+        self._pos_hi += max(lengths)
+        return out
+
+    def _prompt_blocks(self, h: torch.Tensor, attend, pick) -> torch.Tensor:
+        """The blocks over the residual stream h [tokens, hidden] of any prompts.  attend(i, block, qkv, finished): the attention's output [tokens, q] from the
+        qkv layer's output, or (not finished) from its product before the output transform.  Returns pick(the residual stream behind the last block)."""
+        cfg = self.cfg
+        tokens = h.shape[0]
 
         def reduce(y):
             if self.tp_world > 1:
@@ -534,41 +674,29 @@ class RPTCLlama:
                 dist.all_reduce(y, group=self.tp_group)
             return y
 
-        b0 = self.blocks[0]
-        fused = b0.o.incoherent and R * T > 8 and self.tp_world == 1              # residuals, rotation and SwiGLU inside the glue kernels
-        last = None
-        if fused:
+        if self.blocks[0].o.incoherent and tokens > 8 and self.tp_world == 1:     # residuals, rotation and SwiGLU inside the glue kernels
             before = lib().rptc_pdl()
             lib().rptc_set_pdl(1)
             try:
-                last = self._prefill_blocks_fused(h, R, T)
+                return self._prompt_blocks_fused(h, attend, pick)
             finally:
                 lib().rptc_set_pdl(before)
-        else:
 
-            def apply(lin, x):
-                # like the fused path a row's results do not depend on the number of rows that go with it
-                if R * T > 8 and lin.out_features % 128 == 0:
-                    return lin.finish_t(lin.product_t(lin.transform_in(x)))
-                return lin(x)
+        def apply(lin, x):
+            # like the fused path a row's results do not depend on the number of rows that go with it
+            if tokens > 8 and lin.out_features % 128 == 0:
+                return lin.finish_t(lin.product_t(lin.transform_in(x)))
+            return lin(x)
 
-            xn = torch.empty_like(h)
-            for i, b in enumerate(self.blocks):
-                ops.rmsnorm(h, b.norm1, xn, cfg.rms_eps)
-                qkv = apply(b.qkv, xn)
-                ops.rope_cache_prompt(qkv, R, T, self.kcache[i], self.vcache[i], self.heads_l, self.kv_heads_l, D, cfg.rope_theta)
-                h = h + reduce(apply(b.o, self._prompt_attention(qkv, i, R, T)))
-                ops.rmsnorm(h, b.norm2, xn, cfg.rms_eps)
-                gu = apply(b.gate_up, xn)
-                mlp = torch.nn.functional.silu(gu[:, : self.ffn_l]).mul_(gu[:, self.ffn_l:])      # fp32 inside, fp16 in and out
-                h = h + reduce(apply(b.down, mlp))
-            last = h.reshape(R, T, cfg.hidden)[:, -1].contiguous()
-        ops.rmsnorm(last, self.norm_f, self.xn, cfg.rms_eps)
-        ops.dense_gemv(self.head, self.xn, out=self.logits)
-        self.pos.fill_(T - 1)
-        self._pos_hi = T
-        ops.next_token(self.logits, self.next_ids, self.ids, self.pos, None)        # pos -> T, ids -> greedy choice
-        return self.logits
+        xn = torch.empty_like(h)
+        for i, b in enumerate(self.blocks):
+            ops.rmsnorm(h, b.norm1, xn, cfg.rms_eps)
+            h = h + reduce(apply(b.o, attend(i, b, apply(b.qkv, xn), True)))
+            ops.rmsnorm(h, b.norm2, xn, cfg.rms_eps)
+            gu = apply(b.gate_up, xn)
+            mlp = torch.nn.functional.silu(gu[:, : self.ffn_l]).mul_(gu[:, self.ffn_l:])      # fp32 inside, fp16 in and out
+            h = h + reduce(apply(b.down, mlp))
+        return pick(h)
 
     def _prompt_attention(self, qkv: torch.Tensor, i: int, R: int, T: int) -> torch.Tensor:
         """Causal attention of a prompt whose rotated q sit in the first columns of qkv and whose k and v are in the caches."""
@@ -579,14 +707,11 @@ class RPTCLlama:
                                                                is_causal=True, enable_gqa=self.heads_l != self.kv_heads_l)
         return att.transpose(1, 2).reshape(R * T, q_dim)
 
-    def _prefill_blocks_fused(self, h: torch.Tensor, R: int, T: int) -> torch.Tensor:
-        """The blocks over a prompt's residual stream h [R * T, hidden] (updated in place), with everything between two
-        matrix products in one kernel each; returns the residual stream of every row's last position."""
+    def _prompt_blocks_fused(self, h: torch.Tensor, attend, pick) -> torch.Tensor:
+        """`_prompt_blocks` with everything between two matrix products in one kernel each; h is updated in place."""
         cfg = self.cfg
-        heads_of_128 = cfg.head_dim == 128 and self.blocks[0].qkv.block_out == 128
         whole_rows = 256 <= cfg.hidden <= 8192 and cfg.hidden & (cfg.hidden - 1) == 0      # the norm kernel's rows: a block, or two of 4096
-        xt, mlp = torch.empty_like(h), torch.empty((R * T, self.ffn_l), dtype=torch.float16, device=h.device)
-        angles = ops.rope_angles(T, cfg.rope_theta, h.device) if heads_of_128 else None
+        xt, mlp = torch.empty_like(h), torch.empty((h.shape[0], self.ffn_l), dtype=torch.float16, device=h.device)
         y, prev = None, None                                         # product whose output side is still to be added to h, its layer
 
         def norm_into(w_norm, lin):
@@ -599,21 +724,15 @@ class RPTCLlama:
             return lin.transform_in(xt, out=xt)
 
         for i, b in enumerate(self.blocks):
-            qkv = b.qkv.product_t(norm_into(b.norm1, b.qkv))
-            if heads_of_128:
-                ops.prompt_qkv(qkv, b.qkv.signs_out, b.qkv.scale, R, T, self.kcache[i], self.vcache[i], self.heads_l, self.kv_heads_l, angles)
-            else:
-                qkv = b.qkv.finish_t(qkv)
-                ops.rope_cache_prompt(qkv, R, T, self.kcache[i], self.vcache[i], self.heads_l, self.kv_heads_l, cfg.head_dim, cfg.rope_theta)
-            att = self._prompt_attention(qkv, i, R, T)
+            att = attend(i, b, b.qkv.product_t(norm_into(b.norm1, b.qkv)), False)
             y, prev = b.o.product_t(b.o.transform_in(att, out=att)), b.o
             gu = b.gate_up.product_t(norm_into(b.norm2, b.gate_up))
             ops.swiglu_hadamard_f16(gu, mlp, b.gate_up.signs_out, b.down.signs_in, self.ffn_l, b.down.block_in, b.gate_up.scale)
             y, prev = b.down.product_t(mlp), b.down
-        # only the last position of each row is read on
-        pick = lambda t: t.view(R, T, -1)[:, -1].contiguous()
         return prev.finish_t(pick(y), residual=pick(h))
 
+    # -- dense fp32 reference of the same model (decode weights with the GPU's bit-exact decompress) --------
+    @torch.no_grad()
     def reference_logits(self, tokens: torch.Tensor, act_dtype: torch.dtype | None = None) -> torch.Tensor:
         """fp32 torch forward of the same network on `tokens` [rows, T] -> logits [rows, T, vocab].
 
