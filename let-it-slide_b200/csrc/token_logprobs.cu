@@ -146,17 +146,18 @@ struct Share {
 constexpr int kLogprobWarps = kLogprobThreads / 32;
 struct LogprobShared {
     Tally tallies[kLogprobWarps];
-    alignas(16) uint32_t sample[kLogprobWarps * 32 + 4];     // the largest of every warp's threads' largest, in the order of the numbers
-    int found, chosen;
-    int who[kLogprobThreads];
-    uint64_t keys[kLogprobRoom], best[kLogprobTop], merged[kLogprobMaxCluster * kLogprobTop], round[kLogprobWarps];
+    alignas(16) uint32_t sample[kLogprobWarps * 32 + 16];     // the largest of every warp's threads' largest, in the order of the numbers
+    int found, chosen, again;
+    int at[kLogprobThreads], who[kLogprobThreads], whole[kLogprobThreads];
+    alignas(16) uint64_t keys[kLogprobRoom + 8];
+    uint64_t best[kLogprobTop], merged[kLogprobMaxCluster * kLogprobTop], round[kLogprobWarps];
     Tally tally;
 };
 
 // The k largest of the CTA's share, in order (0 where there are fewer), in sh.best.  All threads.
 template <int DTYPE>
-__device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, float mine, int k) {
-    constexpr int kPer = Share<DTYPE>::kPer;
+__device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, float mine, float second, int chunk, int k) {
+    constexpr int kPer = Share<DTYPE>::kPer, U = kLogprobUnroll;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     // A bound that at least k threads' largest entries reach: the k-th of a few of every warp, a few more than its part of k, so that it is seldom lower than the k-th of all.
     const int few = min(32, (k + kLogprobWarps - 1) / kLogprobWarps + 2), samples = few * kLogprobWarps;
@@ -169,17 +170,21 @@ __device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, fl
             sh.sample[warp * few + j] = b;
         }
     }
-    if (t == 0) sh.found = sh.chosen = 0;
+    if (t == 0) sh.found = sh.chosen = sh.again = 0;
+    sh.at[t] = chunk;
     if (t < k) sh.best[t] = 0;
-    if (t >= samples && t < samples + 4) sh.sample[t] = 0;      // to whole loads
+    if (t >= samples && t < samples + 16) sh.sample[t] = 0;     // to whole rounds of the loop below
     __syncthreads();
     uint32_t bound = 0;                                      // every warp finds it for itself
     for (int i = lane; i < samples; i += 32) {
         const uint32_t x = sh.sample[i];
         int before = 0;
-        for (int j = 0; j < samples; j += 4) {
-            const uint4 y = *reinterpret_cast<const uint4 *>(sh.sample + j);
-            before += (y.x > x) + (y.y > x) + (y.z > x) + (y.w > x);
+        for (int j = 0; j < samples; j += 16) {
+            uint4 y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const uint4 *>(sh.sample + j + 4 * e);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) before += (y[e].x > x) + (y[e].y > x) + (y[e].z > x) + (y[e].w > x);
         }
         if (before < k) bound = bound ? min(bound, x) : x;   // the smallest that fewer than k pass
     }
@@ -189,33 +194,34 @@ __device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, fl
         const int at = atomicAdd(&sh.found, 1);
         if (at < kLogprobRoom) sh.keys[at] = order_key(x, i);
     };
-    const bool reaches = own >= bound;
-    if (reaches)
+    if (own >= bound) {
         if (const int64_t s = share.single(t); s >= 0) offer(logit<DTYPE>(share.row, s), (uint32_t)s);
-    if (reaches) sh.who[atomicAdd(&sh.chosen, 1)] = t;
+        sh.who[atomicAdd(&sh.chosen, 1)] = t;
+        if (order_of(second) >= bound) sh.whole[atomicAdd(&sh.again, 1)] = t;
+    }
     __syncthreads();
-    // all threads look at the vectors of those that reach the bound, a few at a time
-    const int chosen = sh.chosen, each = (share.last - share.first + kLogprobThreads - 1) / kLogprobThreads;
-    for (int i0 = t; i0 < chosen * each; i0 += 2 * kLogprobThreads) {
-        uint4 raw[2];
-        int v[2];
+    auto look = [&](int v) {
+        float x[kPer];
+        logits_of<DTYPE>(share.vector(v), x);
+        float top = x[0];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int i = i0 + u * kLogprobThreads, q = i / each;
-            v[u] = i < chosen * each ? share.first + sh.who[q] + (i - q * each) * kLogprobThreads : share.last;
-            if (v[u] < share.last) raw[u] = share.vector(v[u]);
-        }
+        for (int e = 1; e < kPer; ++e) top = max_nan(top, x[e]);
+        if (order_of(top) < bound) return;                   // most have nothing
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            if (v[u] >= share.last) continue;
-            float x[kPer];
-            logits_of<DTYPE>(raw[u], x);
-            float top = x[0];
-#pragma unroll
-            for (int e = 1; e < kPer; ++e) top = max_nan(top, x[e]);
-            if (order_of(top) < bound) continue;             // most have nothing
-#pragma unroll
-            for (int e = 0; e < kPer; ++e) offer(x[e], share.index(v[u], e));
+        for (int e = 0; e < kPer; ++e) offer(x[e], share.index(v, e));
+    };
+    // All threads look at the vectors of those that reach the bound: the few that were read together with the largest
+    // entry, and all the others too where one of them reaches it as well.
+    const int chosen = sh.chosen, again = sh.again;
+    for (int i = t; i < chosen * U; i += kLogprobThreads) {
+        const int v = sh.at[sh.who[i / U]] + (i % U) * kLogprobThreads;
+        if (v < share.last) look(v);
+    }
+    if (again) {
+        const int each = (share.last - share.first + kLogprobThreads - 1) / kLogprobThreads;
+        for (int i = t; i < again * each; i += kLogprobThreads) {
+            const int q = i / each, who = sh.whole[q], v = share.first + who + (i - q * each) * kLogprobThreads, from = v - sh.at[who];
+            if (v < share.last && (from < 0 || from >= U * kLogprobThreads)) look(v);
         }
     }
     __syncthreads();
@@ -224,14 +230,20 @@ __device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, fl
         for (int i = t; i < found; i += kLogprobThreads) {
             const uint64_t key = sh.keys[i];
             int rank = 0;
-            for (int j = 0; j < found && rank < k; ++j) rank += sh.keys[j] > key;
+            for (int j = 0; j < found; j += 8) {
+                ulonglong2 y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = *reinterpret_cast<const ulonglong2 *>(sh.keys + j + 2 * e);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) rank += (j + 2 * e < found && y[e].x > key) + (j + 2 * e + 1 < found && y[e].y > key);
+            }
             if (rank < k) sh.best[rank] = key;
         }
     } else {
         uint64_t last = ~0ull;
         for (int j = 0; j < k; ++j) {                        // one after the other
             uint64_t best = 0;
-            auto look = [&](float x, uint32_t i) {
+            auto consider = [&](float x, uint32_t i) {
                 const uint64_t key = order_key(x, i);
                 if (key < last && key > best) best = key;
             };
@@ -239,10 +251,10 @@ __device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, fl
                 float x[kPer];
                 logits_of<DTYPE>(share.vector(v), x);
 #pragma unroll
-                for (int e = 0; e < kPer; ++e) look(x[e], share.index(v, e));
+                for (int e = 0; e < kPer; ++e) consider(x[e], share.index(v, e));
             }
             const int64_t s = share.single(t);
-            if (s >= 0) look(logit<DTYPE>(share.row, s), (uint32_t)s);
+            if (s >= 0) consider(logit<DTYPE>(share.row, s), (uint32_t)s);
             for (int o = 16; o > 0; o >>= 1) {
                 const uint64_t b = __shfl_xor_sync(0xFFFFFFFFu, best, o);
                 best = b > best ? b : best;
@@ -279,7 +291,8 @@ __global__ void __launch_bounds__(kLogprobThreads, 5) token_logprobs_kernel(cons
         if (target >= 0 && target < p.n) target_logit = logit<DTYPE>(share.row, target);
     }
     Tally a = {-INFINITY, 0.f, 0.f};
-    float largest = -INFINITY;                               // of this thread's entries; NaN if any is
+    float largest = -INFINITY, second = -INFINITY;           // of this thread's entries, and of those not read together with it; NaN if any is
+    int chunk = share.last;                                  // the first of the vectors read with the largest
     auto add = [&](const float (&x)[kPer], f32x2 &z, f32x2 &w) {
         const f32x2 unit = pack2(kLog2e, kLog2e), from = pack2(-a.M, -a.M);
 #pragma unroll
@@ -316,9 +329,13 @@ __global__ void __launch_bounds__(kLogprobThreads, 5) token_logprobs_kernel(cons
                              : max_nan(__uint_as_float(m << 16), __uint_as_float(m & 0xFFFF0000u));
         }
         if (top == -INFINITY) continue;
-        if (!(top <= largest)) {
-            largest = max_nan(top, largest);
-            a.move(largest);
+        if (!(top <= second)) {
+            if (!(top <= largest)) {
+                second = largest, largest = max_nan(top, largest), chunk = v0;
+                a.move(largest);
+            } else {
+                second = top;
+            }
         }
         f32x2 z = pack2(a.z, 0.f), w = pack2(a.w, 0.f);
 #pragma unroll
@@ -348,7 +365,7 @@ __global__ void __launch_bounds__(kLogprobThreads, 5) token_logprobs_kernel(cons
     if (!(warp_top == -INFINITY)) a.move(warp_top);
     for (int o = 16; o > 0; o >>= 1) a.z += __shfl_xor_sync(0xFFFFFFFFu, a.z, o), a.w += __shfl_xor_sync(0xFFFFFFFFu, a.w, o);
     if (lane == 0) sh.tallies[warp] = a;
-    if (p.k > 0) largest_entries<DTYPE>(sh, share, mine, p.k);
+    if (p.k > 0) largest_entries<DTYPE>(sh, share, mine, second, chunk, p.k);
     else __syncthreads();
     if (warp == 0) {
         a = sh.tallies[lane % kLogprobWarps];

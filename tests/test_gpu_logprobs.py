@@ -118,6 +118,31 @@ def test_large_and_close_values(n):
     check(ops.token_logprobs(x, targets, 32), *reference(x, targets, 32))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,n,top", [(3, 32000, 20), (400, 32000, 32), (400, 128001, 20)])
+def test_largest_entries_side_by_side(dtype, rows, n, top):
+    """The largest lie apart by lengths that the kernel's strides divide, or next to one another, or all but one are -inf."""
+    from rptc_b200 import ops
+    x, targets = rand(rows, n, dtype, 7 * rows + n)
+    for r in range(rows):
+        step = (1, 4, 8, 1024, 2048, 4096, 8192, 1000)[r % 8]
+        at = torch.arange(r, n, step, device="cuda")[:top + 3]
+        x[r, at] = 20 + torch.arange(len(at), device="cuda", dtype=dtype) / 8
+    x[0] = -math.inf
+    x[0, n // 3] = 1
+    targets[0] = n // 3
+    if rows > 8:
+        x[8, n // 2:] = -math.inf
+        x[9, 5] = x[9, 4096 + 5] = math.inf
+    out = ops.token_logprobs(x, targets, top)
+    want, tol = reference(x, targets, top)
+    if rows > 8:      # a row with +inf has no probabilities
+        assert out[0][9].isnan() and out[1][9].isnan() and out[2][9].isnan().all()
+    keep = torch.arange(rows, device="cuda") != 9
+    check([o[keep] for o in out], [w[keep] for w in want], [t[keep] for t in tol])
+    ops.device_status()
+
+
 def test_rows_without_numbers():
     from rptc_b200 import ops
     x, targets = rand(4, 2000, torch.float32, 6)
