@@ -14,9 +14,12 @@
 //            product) is multiplied with is not larger than the values; the second sum is in fp32.  (-8 by a product with a constant operand: 173 us where this takes 160.)
 // Weights refer to a running maximum of s + log2(a tile's largest scale): the products p * scale then fit fp16 whatever the scales are (2^11 where the reference was set, and
 // it moves only when they may pass 2^15, which their sum shows: no maximum is looked for otherwise; what falls below 2^-14 is 2^-25 of the largest).
-// Bound: HBM.  About 290 warp instructions per 16 positions (2560 bytes), two thirds of the issue slots at the measured copy rate.
+// Bound: HBM (160 bytes per position and kv head) with the issue slots close behind, about 350 warp instructions per 16 positions: four rows in flight per scheduler at 128
+// registers leave a quarter of the slots empty.  32 rows of 500 to 32768 positions, 8 kv heads: 140 us, 4.9 TB/s; one row of 131072: 45 us, 3.7 TB/s; one of 200: 4.6 us.
 // Long contexts: all tiles of all rows and heads, laid end to end, are cut into equal ranges for the CTAs of one wave, so that rows of different lengths balance; a range's
-// part of a row goes to the workspace (fp32) and a second kernel joins the parts.  Short caches (max_pos up to kKv4Whole) take one CTA per row and head and no second kernel.
+// part of a row goes to the workspace (fp32) and a second kernel joins the parts.  A warp's ring goes on into the range's next item: its first tiles and its q are on their
+// way while the item before is finished (32 rows as above 160 us without, and with a join that looked at every row's heads instead of the ranges' ends).
+// Short caches take one CTA per row and head and no second kernel (the rule is at kv4_whole).
 #include <type_traits>
 
 #include "fwht.cuh"
@@ -24,11 +27,10 @@
 
 namespace rptc {
 
-constexpr int kKv4Warps = 8, kKv4Tile = 32, kKv4Stages = 2;
+constexpr int kKv4Warps = 8, kKv4Tile = 32, kKv4Stages = 2, kKv4CtasPerSm = 2;
 constexpr uint32_t kKv4StageBytes = 2 * kKv4Tile * (kKv4Codes + kKv4Scales);
 constexpr uint32_t kKv4Ring = kKv4Warps * kKv4Stages * kKv4StageBytes, kKv4Merge = kKv4Warps * 8 * 128 * 4, kKv4Smem = kKv4Ring + kKv4Merge + kKv4Warps * 8 * 8;
-constexpr int kKv4CtasPerSm = 2;
-constexpr int64_t kKv4Whole = 1024;
+static_assert(kKv4Stages == 2, "a stage is the other one's next");
 constexpr float kKv4Bias = 11.f;
 
 struct AttnKv4Params {
@@ -53,10 +55,10 @@ __device__ __forceinline__ int kv4_context(const AttnKv4Params &p, const int32_t
 }
 __device__ __forceinline__ int kv4_tiles(int context) { return (context + kKv4Tile - 1) / kKv4Tile; }
 
-// How the work is cut: every row's heads laid end to end, each worth its tiles and kKv4Start for what a CTA does around them (q, the ring's first copies, the warps' sums: as
-// long as about twelve tiles; without it the CTAs that got the short rows took 365,000 clocks where the others took 270,000: 32 rows of 500 to 32768).  In numbers of 32
-// bits: a unit stands for a tile of 5 KiB of the cache.
-constexpr uint32_t kKv4Start = 12;
+// How the work is cut: every row's heads laid end to end, each worth its tiles and kKv4Start for what a CTA does around them (q, the warps' sums).  32 rows of 500 to 32768
+// took 158 us with 12 of those, 150 with 16, 145 with 24 and 146 with 32; kKv4Least is what a CTA is worth starting for.  In numbers of 32 bits: a unit stands for a tile of
+// 5 KiB of the cache.
+constexpr uint32_t kKv4Start = 24, kKv4Least = 16;
 __device__ __forceinline__ uint32_t kv4_cost(int tiles) { return tiles ? (uint32_t)tiles + kKv4Start : 0u; }
 struct Kv4Cut {
     uint32_t ctas, per, extra;
@@ -70,10 +72,44 @@ __device__ __forceinline__ Kv4Cut kv4_cut(const AttnKv4Params &p, const int32_t 
     for (int r0 = 0; r0 < p.rows; r0 += 32) sum += __reduce_add_sync(0xFFFFFFFFu, r0 + lane < p.rows ? kv4_cost(kv4_tiles(kv4_context(p, pos, r0 + lane))) : 0u);
     sum *= (uint32_t)(p.hkv * p.blocks);
     Kv4Cut c;
-    c.ctas = min(most_ctas, max(sum / (kKv4Start + kKv4Warps / 2), 1u));
+    c.ctas = min(most_ctas, max(sum / kKv4Least, 1u));
     c.per = sum / c.ctas, c.extra = sum - c.per * c.ctas;
     return c;
 }
+// The row, the head and the place in it that lie `at` units on.  A whole warp.
+struct Kv4Place {
+    int row, head, context;
+    uint32_t cost, off;
+};
+__device__ __forceinline__ Kv4Place kv4_place(const AttnKv4Params &p, const int32_t *pos, uint32_t at, int lane) {
+    const uint32_t heads = (uint32_t)(p.hkv * p.blocks);
+    uint32_t before = 0;
+    Kv4Place f = {};
+    for (int r0 = 0; r0 < p.rows; r0 += 32) {
+        const int here = r0 + lane < p.rows ? kv4_context(p, pos, r0 + lane) : 0;
+        const uint32_t cost = kv4_cost(kv4_tiles(here));
+        uint32_t upto = cost;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+            if (lane >= o) upto += v;
+        }
+        const unsigned hit = __ballot_sync(0xFFFFFFFFu, (before + upto) * heads > at);
+        if (hit) {
+            const int from = __ffs(hit) - 1;
+            f.row = r0 + from;
+            f.context = __shfl_sync(0xFFFFFFFFu, here, from);
+            f.cost = __shfl_sync(0xFFFFFFFFu, cost, from);
+            const uint32_t in_row = at - (before + __shfl_sync(0xFFFFFFFFu, upto - cost, from)) * heads;
+            f.head = (int)(in_row / f.cost), f.off = in_row - (uint32_t)f.head * f.cost;
+            break;
+        }
+        before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    return f;
+}
+// That many units of an item reach so far into its tiles.
+__device__ __forceinline__ int kv4_tile_of(uint32_t units) { return (int)max(units, kKv4Start) - (int)kKv4Start; }
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     uint32_t d;
@@ -155,102 +191,109 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
     const uint32_t ring = smem_addr(smem) + (uint32_t)warp * kKv4Stages * kKv4StageBytes;
     float *merge = reinterpret_cast<float *>(smem + kKv4Ring);
     float2 *merge_ml = reinterpret_cast<float2 *>(smem + kKv4Ring + kKv4Merge);
-    pdl_allow_next_grid();
     pdl_wait_prior_grids();
+    pdl_allow_next_grid();                           // not before: the join reads pos without waiting for this kernel's end
     const int32_t *pos = after_wait(p.pos);
-    const uint32_t heads = (uint32_t)(p.hkv * p.blocks);      // of a row, in the order of the cut
-    uint32_t at = 0, end = 0;
-    if (!WHOLE) {
+    const int heads = p.hkv * p.blocks;              // of a row, in the order of the cut
+    // ---- a row's head, its tiles t0 .. t1 - 1; `units` of the range are left behind them ----
+    int row, head, context, t0, t1;
+    uint32_t units = 0;
+    if (WHOLE) {
+        row = blockIdx.y, head = blockIdx.x;
+        context = kv4_context(p, pos, row);
+        if (context == 0 && pos[row] != -1 && tid == 0) atomicExch(p.status, kStatusPosition);
+        t0 = 0, t1 = kv4_tiles(context);
+    } else {
         const Kv4Cut cut = kv4_cut(p, pos, gridDim.x, lane);
         if (blockIdx.x >= cut.ctas) return;
-        at = cut.begin(blockIdx.x), end = cut.begin(blockIdx.x + 1);
-        if (at >= end) return;
+        const uint32_t at = cut.begin(blockIdx.x);
+        units = cut.begin(blockIdx.x + 1) - at;
+        if (units == 0) return;
+        const Kv4Place f = kv4_place(p, pos, at, lane);
+        row = f.row, head = f.head, context = f.context;
+        const uint32_t here = min(f.cost - f.off, units);
+        t0 = kv4_tile_of(f.off), t1 = kv4_tile_of(f.off + here);
+        units -= here;
+        if (t0 == t1) return;                        // the range ends in front of the first tile
     }
-    do {
-        // ---- a row's head, its tiles t0 .. t1 - 1 ----
-        int row, head, context, t0, t1, tiles;
-        if (WHOLE) {
-            row = blockIdx.y, head = blockIdx.x;
-            context = kv4_context(p, pos, row);
-            if (context == 0 && pos[row] != -1 && tid == 0) atomicExch(p.status, kStatusPosition);
-            t0 = 0, t1 = tiles = kv4_tiles(context);
-        } else {
-            uint32_t before = 0;
-            row = 0;
-            tiles = 0;
-            for (int r0 = 0; r0 < p.rows; r0 += 32) {
-                const int here = r0 + lane < p.rows ? kv4_tiles(kv4_context(p, pos, r0 + lane)) : 0;
-                uint32_t upto = kv4_cost(here);
+    auto cache_of = [&](int r, int h) { return ((uint32_t)r * p.hkv + h / p.blocks) * (uint32_t)p.max_pos; };      // in positions: as many as device memory holds
+    // q of a head's block, as the lanes use it: of head g the values 8 t .. 8 t + 7 of each group, or null
+    auto q_of = [&](int r, int h) -> const __half * {
+        const int kvh = h / p.blocks, first = (h - kvh * p.blocks) * 8;
+        return g < p.group - first ? p.q + (int64_t)r * p.ld_q + (kvh * p.group + first + g) * 128 + 8 * t : nullptr;
+    };
+    uint4 raw[4];
+    {
+        const __half *q = q_of(row, head);
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-                    if (lane >= o) upto += v;
-                }
-                const unsigned hit = __ballot_sync(0xFFFFFFFFu, (before + upto) * heads > at);
-                if (hit) {
-                    const int from = __ffs(hit) - 1;
-                    row = r0 + from;
-                    tiles = __shfl_sync(0xFFFFFFFFu, here, from);
-                    before += __shfl_sync(0xFFFFFFFFu, upto - kv4_cost(here), from);
-                    break;
-                }
-                before += __shfl_sync(0xFFFFFFFFu, upto, 31);
+        for (int j = 0; j < 4; ++j) raw[j] = q ? ld_ordered_u128(q + 32 * j) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    // The next item's comes by asynchronous copies into what only this warp reads of the merge buffer (a lane its own bytes); a plain load would wait behind all that the rings
+    // ask for, some 7000 clocks.
+    const uint32_t q_lane = smem_addr(merge) + 512u * warp + 16u * lane;      // its head of the first four warps' sums
+    int stage_no = 0;
+    for (bool started = false;; started = true) {
+        const uint32_t cache_at = cache_of(row, head);
+        // ---- what comes next in the range: it begins with an item's first tile, which is fetched under this one's last ----
+        int n_row = row, n_head = head + 1, n_context = context, n_t1 = 0;
+        if (!WHOLE && units) {
+            if (n_head == heads) {
+                n_head = 0;
+                do n_context = kv4_context(p, pos, ++n_row);
+                while (n_context == 0 && n_row + 1 < p.rows);
             }
-            const uint32_t cost = kv4_cost(tiles), in_row = at - before * heads;
-            head = (int)(in_row / cost);
-            const uint32_t off = in_row - (uint32_t)head * cost, off_end = min(cost, off + (end - at));
-            t0 = (int)max(off, kKv4Start) - (int)kKv4Start, t1 = (int)max(off_end, kKv4Start) - (int)kKv4Start;
-            context = kv4_context(p, pos, row);
-            at += off_end - off;
-            if (t0 == t1) continue;                  // the range ends in front of the first tile
+            n_t1 = kv4_tile_of(min(kv4_cost(kv4_tiles(n_context)), units));
         }
-        const int kvh = head / p.blocks, first = (head - kvh * p.blocks) * 8, in_block = min(8, p.group - first), q_head = kvh * p.group + first;
-        const int64_t cache_at = ((int64_t)row * p.hkv + kvh) * p.max_pos;
-        const uint8_t *k = after_wait(p.k) + cache_at * kKv4Codes, *v = after_wait(p.v) + cache_at * kKv4Codes;
-        const __half2 *ks = after_wait(p.k_scales) + cache_at * 4, *vs = after_wait(p.v_scales) + cache_at * 4;
+        const uint32_t n_cache_at = WHOLE ? 0u : cache_of(n_row, n_head);
         // A tile is 320 pieces of 16 bytes, ten of them a lane's.  (Bulk copies by four lanes took about 70 instructions a tile more: they are issued lane by lane.)
-        const uint8_t *k_from = k + 16 * lane, *v_from = v + 16 * lane;
-        const char *ks_from = reinterpret_cast<const char *>(ks) + 16 * lane, *vs_from = reinterpret_cast<const char *>(vs) + 16 * lane;
         auto fetch = [&](int tile, int stage) {
-            if (tile < t1) {
-                const uint32_t dst = ring + (uint32_t)stage * kKv4StageBytes + 16u * lane;
-                const int64_t c = (int64_t)tile * (kKv4Tile * kKv4Codes), s = (int64_t)tile * (kKv4Tile * kKv4Scales);
-                const int n = context - tile * kKv4Tile;
+            const bool next = !WHOLE && tile >= t1;
+            if (next) tile = warp + ((tile - t1) & ~(kKv4Warps - 1));
+            if (tile < (next ? n_t1 : t1)) {
+                const uint32_t dst = ring + (uint32_t)stage * kKv4StageBytes + 16u * lane, first = (uint32_t)tile * kKv4Tile;
+                const uint32_t place = (next ? n_cache_at : cache_at) + first;
+                const int n = (next ? n_context : context) - (int)first;
+                const uint64_t codes = (uint64_t)place * kKv4Codes + 16 * lane, scales = (uint64_t)(place + lane) * 4;
+                const uint8_t *kc = p.k + codes, *vc = p.v + codes;
+                const __half2 *ks = p.k_scales + scales, *vs = p.v_scales + scales;
                 if (n >= kKv4Tile) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) cp_async16(dst + 512u * i, k_from + c + 512 * i);
-                    cp_async16(dst + kKv4Tile * kKv4Codes, ks_from + s);
+                    for (int i = 0; i < 4; ++i) cp_async16(dst + 512u * i, kc + 512 * i);
+                    cp_async16(dst + kKv4Tile * kKv4Codes, ks);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) cp_async16(dst + kKv4Tile * (kKv4Codes + kKv4Scales) + 512u * i, v_from + c + 512 * i);
-                    cp_async16(dst + kKv4Tile * (2 * kKv4Codes + kKv4Scales), vs_from + s);
+                    for (int i = 0; i < 4; ++i) cp_async16(dst + kKv4Tile * (kKv4Codes + kKv4Scales) + 512u * i, vc + 512 * i);
+                    cp_async16(dst + kKv4Tile * (2 * kKv4Codes + kKv4Scales), vs);
                 } else {                             // no further than the last position
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if (8 * i + (lane >> 2) >= n) continue;
-                        cp_async16(dst + 512u * i, k_from + c + 512 * i);
-                        cp_async16(dst + kKv4Tile * (kKv4Codes + kKv4Scales) + 512u * i, v_from + c + 512 * i);
+                        cp_async16(dst + 512u * i, kc + 512 * i);
+                        cp_async16(dst + kKv4Tile * (kKv4Codes + kKv4Scales) + 512u * i, vc + 512 * i);
                     }
                     if (lane < n) {
-                        cp_async16(dst + kKv4Tile * kKv4Codes, ks_from + s);
-                        cp_async16(dst + kKv4Tile * (2 * kKv4Codes + kKv4Scales), vs_from + s);
+                        cp_async16(dst + kKv4Tile * kKv4Codes, ks);
+                        cp_async16(dst + kKv4Tile * (2 * kKv4Codes + kKv4Scales), vs);
                     }
                 }
             }
             cp_async_commit();                       // an empty group when nothing is left keeps the count constant
         };
+        if (n_t1) {
+            const __half *q = q_of(n_row, n_head);
 #pragma unroll
-        for (int i = 0; i < kKv4Stages; ++i) fetch(t0 + warp + i * kKv4Warps, i);
-        int stage_no = 0;
-        // ---- q: this lane's operand values are those of q head g, dims 8 t .. 8 t + 7 of each group ----
+            for (int j = 0; j < 4; ++j)
+                if (q) cp_async16(q_lane + 4096u * j, q + 32 * j);
+        }
+        // The ring's next stages: after the first item they are under way, but for those that a short one does not fill.  The second one asks for its tile after q.
+        if (!started || t0 + warp >= t1) fetch(t0 + warp, stage_no);
+        // ---- q ----
         uint32_t qb[4][4], q_low[2];                 // q_low: (0, sum of q over group t) in two fp16 parts, against (scale, minimum) pairs
         float unit[2];                               // of the q heads 2 t and 2 t + 1, whose scores this lane gets
         {
             float x[4][8], big = 0.f, mine = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-                if (g < in_block) raw = ld_ordered_u128(p.q + (int64_t)row * p.ld_q + (q_head + g) * 128 + 32 * j + 8 * t);
-                unpack8(raw, x[j]);
+                unpack8(raw[j], x[j]);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) big = fmaxf(big, fabsf(x[j][i]));
             }
@@ -280,6 +323,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             q_low[1] = half2_as_u32(__halves2half2(__float2half_rn(0.f), __float2half_rn(mine - __half2float(hi))));
             unit[0] = __shfl_sync(0xFFFFFFFFu, up, 8 * t), unit[1] = __shfl_sync(0xFFFFFFFFu, up, 8 * t + 4);
         }
+        if (!started || t0 + warp + kKv4Warps >= t1) fetch(t0 + warp + kKv4Warps, stage_no ^ 1);
         // ---- this warp's tiles ----
         float o[8][4] = {}, low[4][2] = {}, l[2] = {0.f, 0.f}, m[2] = {-INFINITY, -INFINITY};
         const int my_row = (g >> 1) + 4 * (g & 1);   // the position of an operand's row g, so that the V operand's rows t and t + 4 are neighbours in the product
@@ -387,7 +431,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             values(std::integral_constant<int, 1>());
             __syncwarp();                            // the stage is free
             fetch(tile + kKv4Stages * kKv4Warps, stage_no);
-            stage_no = stage_no + 1 == kKv4Stages ? 0 : stage_no + 1;
+            stage_no ^= 1;
         }
         // ---- the warps' sums into one ----
 #pragma unroll
@@ -399,7 +443,14 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                 for (int j = 0; j < 4; ++j) low[j][c] += __shfl_xor_sync(0xFFFFFFFFu, low[j][c], x);
             }
         }
-        __syncthreads();                             // the last segment's sums have been taken
+        if (n_t1) {
+            cp_async_wait<kKv4Stages - 1>();
+            const bool there = q_of(n_row, n_head);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) raw[j] = there ? lds128_at<0>(q_lane + 4096u * j) : make_uint4(0u, 0u, 0u, 0u);
+        }
+        const int kvh = head / p.blocks, first = (head - kvh * p.blocks) * 8, in_block = min(8, p.group - first), q_head = kvh * p.group + first;
+        __syncthreads();                             // the last item's sums have been taken
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             float *dst = merge + (warp * 8 + 2 * t + c) * 128 + 4 * g;
@@ -424,7 +475,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                 den = fmaf(ml[w].y, f, den);
                 sum[0] = fmaf(x.x, f, sum[0]), sum[1] = fmaf(x.y, f, sum[1]), sum[2] = fmaf(x.z, f, sum[2]), sum[3] = fmaf(x.w, f, sum[3]);
             }
-            if (WHOLE || (t0 == 0 && t1 == tiles)) {
+            if (WHOLE || (t0 == 0 && t1 == kv4_tiles(context))) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) sum[i] = context ? sum[i] / den : 0.f;
                 kv4_store(p, row, q_head + warp, lane, sum);
@@ -434,61 +485,71 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                 if (lane == 0) p.part_ml[slot] = make_float2(mx, den);
             }
         }
-    } while (!WHOLE && at < end);
+        if (n_t1 == 0) break;
+        units -= min(kv4_cost(kv4_tiles(n_context)), units);
+        row = n_row, head = n_head, context = n_context, t0 = 0, t1 = n_t1;
+    }
 }
 
-// A CTA per row and q head: joins the parts that ranges have left of it, and writes the zeros of a row without positions.
-__global__ void __launch_bounds__(512) attn_kv4_join_kernel(const AttnKv4Params p, uint32_t most_ctas) {
-    __shared__ float4 sums[16][32];
-    __shared__ float dens[16];
-    pdl_allow_next_grid();
+// Joins the parts that ranges have left of an item, a CTA per q head of it: of each item where there are few, else of the item that a range's end lies in (`by_item`).
+// Also writes the zeros of rows without positions.
+constexpr int kKv4JoinWarps = 8;
+__global__ void __launch_bounds__(32 * kKv4JoinWarps) attn_kv4_join_kernel(const AttnKv4Params p, uint32_t most_ctas, int by_item) {
+    __shared__ float4 sums[kKv4JoinWarps][32];
+    __shared__ float2 ml[kKv4JoinWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    pdl_wait_prior_grids();
+    // pos was there before the first kernel let this one start: where the parts lie is found while that one works.
     const int32_t *pos = after_wait(p.pos);
-    const int row = blockIdx.y, q_head = blockIdx.x, kvh = q_head / p.group, in_group = q_head - kvh * p.group, head = kvh * p.blocks + in_group / 8;
-    const int tiles = kv4_tiles(kv4_context(p, pos, row));
-    if (tiles == 0) {
-        if (q_head == 0 && threadIdx.x == 0 && pos[row] != -1) atomicExch(p.status, kStatusPosition);
-        float zero[4] = {0.f, 0.f, 0.f, 0.f};
-        if (warp == 0) kv4_store(p, row, q_head, lane, zero);
-        return;
-    }
+    const int heads = p.hkv * p.blocks;
     const Kv4Cut cut = kv4_cut(p, pos, most_ctas, lane);
-    uint32_t before = 0;
-    for (int r0 = 0; r0 < row; r0 += 32) before += __reduce_add_sync(0xFFFFFFFFu, r0 + lane < row ? kv4_cost(kv4_tiles(kv4_context(p, pos, r0 + lane))) : 0u);
-    const uint32_t first_tile = before * (uint32_t)(p.hkv * p.blocks) + (uint32_t)head * kv4_cost(tiles) + kKv4Start;
-    const int c0 = (int)cut.cta_of(first_tile), c1 = (int)cut.cta_of(first_tile + tiles - 1);
-    if (c0 == c1) return;                            // one range had it all
+    int row = 0, head = 0, tiles = 0;
+    uint32_t first_tile = 0;
+    if (by_item) {
+        row = blockIdx.x / heads, head = blockIdx.x % heads;
+        tiles = kv4_tiles(kv4_context(p, pos, row));
+        uint32_t before = 0;
+        for (int r0 = 0; r0 < row; r0 += 32) before += __reduce_add_sync(0xFFFFFFFFu, r0 + lane < row ? kv4_cost(kv4_tiles(kv4_context(p, pos, r0 + lane))) : 0u);
+        first_tile = before * (uint32_t)heads + (uint32_t)head * kv4_cost(tiles) + kKv4Start;
+    } else if (blockIdx.x + 1 < cut.ctas) {
+        const uint32_t at = cut.begin(blockIdx.x + 1);
+        const Kv4Place f = kv4_place(p, pos, at, lane);
+        if (f.off > kKv4Start) row = f.row, head = f.head, tiles = kv4_tiles(f.context), first_tile = at - f.off + kKv4Start;      // else it ends in front of a first tile
+    }
+    int c0 = 0, c1 = 0;
+    if (tiles) c0 = (int)cut.cta_of(first_tile), c1 = (int)cut.cta_of(first_tile + tiles - 1);
+    const int kvh = head / p.blocks, in_group = (head - kvh * p.blocks) * 8 + blockIdx.y, q_head = kvh * p.group + in_group;
+    pdl_wait_prior_grids();
+    pdl_allow_next_grid();
+    for (int r = blockIdx.x; r < p.rows; r += gridDim.x) {
+        if (kv4_context(p, pos, r)) continue;
+        if (blockIdx.y == 0 && threadIdx.x == 0 && pos[r] != -1) atomicExch(p.status, kStatusPosition);
+        float zero[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int h = blockIdx.y * kKv4JoinWarps + warp; h < p.hkv * p.group; h += gridDim.y * kKv4JoinWarps) kv4_store(p, r, h, lane, zero);
+    }
+    if (c0 == c1 || (!by_item && c0 != (int)blockIdx.x) || in_group >= p.group) return;      // one range had it all; another CTA has it
     const float4 *part = after_wait(p.part);
     const float2 *part_ml = after_wait(p.part_ml);
     float mx = -INFINITY, den = 0.f;
     float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = c0 + lane; c <= c1; c += 32) mx = fmaxf(mx, __ldcg(part_ml + (2 * c + (c == c0 ? 1 : 0)) * 8 + (in_group & 7)).x);
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xFFFFFFFFu, mx, o));
+    auto add = [&](float2 a, float4 x) {
+        const float to = fmaxf(mx, a.x), f = mx == -INFINITY ? 0.f : ex2(mx - to), g = ex2(a.x - to);
+        mx = to;
+        den = fmaf(a.y, g, den * f);
+        sum.x = fmaf(x.x, g, sum.x * f), sum.y = fmaf(x.y, g, sum.y * f), sum.z = fmaf(x.z, g, sum.z * f), sum.w = fmaf(x.w, g, sum.w * f);
+    };
 #pragma unroll 4
-    for (int c = c0 + warp; c <= c1; c += 16) {
+    for (int c = c0 + warp; c <= c1; c += kKv4JoinWarps) {
         const int slot = (2 * c + (c == c0 ? 1 : 0)) * 8 + (in_group & 7);
-        const float2 ml = __ldcg(part_ml + slot);
-        const float4 x = __ldcg(part + slot * 32 + lane);
-        const float f = ex2(ml.x - mx);
-        den = fmaf(ml.y, f, den);
-        sum.x = fmaf(x.x, f, sum.x), sum.y = fmaf(x.y, f, sum.y), sum.z = fmaf(x.z, f, sum.z), sum.w = fmaf(x.w, f, sum.w);
+        add(__ldcg(part_ml + slot), __ldcg(part + slot * 32 + lane));
     }
     sums[warp][lane] = sum;
-    if (lane == 0) dens[warp] = den;
+    if (lane == 0) ml[warp] = make_float2(mx, den);
     __syncthreads();
     if (warp) return;
-    float out[4] = {0.f, 0.f, 0.f, 0.f};
-    den = 0.f;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) {
-        const float4 x = sums[w][lane];
-        den += dens[w];
-        out[0] += x.x, out[1] += x.y, out[2] += x.z, out[3] += x.w;
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) out[i] /= den;
+    for (int w = 1; w < kKv4JoinWarps; ++w)
+        if (c0 + w <= c1) add(ml[w], sums[w][lane]);
+    float out[4] = {sum.x / den, sum.y / den, sum.z / den, sum.w / den};
     kv4_store(p, row, q_head, lane, out);
 }
 
@@ -496,8 +557,15 @@ __global__ void __launch_bounds__(512) attn_kv4_join_kernel(const AttnKv4Params 
 
 using namespace rptc;
 
+// A CTA per row and head, or ranges.  Measured on full caches of 8 kv heads: 1024 positions 9.1 against 9.9 us (one row), 9.3 and 16.7 (16), 51 and 87 (148); 2048 positions
+// 13.8 against 10.3 (one row), 14.0 and 13.8 (4), 13.9 and 20.8 (16), 83 and 95 (148).  Longer ones go by ranges whatever the rows are, as those may differ in length.
+static bool kv4_whole(const rptc_kv_cache &c, int heads) {
+    const int64_t items = (int64_t)c.rows * c.kv_heads * ((heads / c.kv_heads + 7) / 8);
+    return c.max_pos <= 1024 || (c.max_pos <= 2048 && 4 * items >= num_sms());
+}
+
 extern "C" int64_t rptc_attn_decode_kv4_workspace_bytes(const rptc_kv_cache *cache, int heads) {
-    if (!cache || check_kv_cache(*cache) || cache->bits != 4 || cache->max_pos <= kKv4Whole || heads <= 0) return 0;
+    if (!cache || check_kv_cache(*cache) || cache->bits != 4 || heads <= 0 || kv4_whole(*cache, heads)) return 0;
     return (int64_t)num_sms() * kKv4CtasPerSm * 2 * 8 * (128 * 4 + 8);
 }
 
@@ -530,7 +598,7 @@ extern "C" int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *
     if (!p.status) return RPTC_ERR_CUDA;
     p.part = nullptr, p.part_ml = nullptr;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (cache->max_pos <= kKv4Whole) {
+    if (kv4_whole(*cache, heads)) {
         static SmemOptIn opted;
         if (int e = allow_max_smem(attn_kv4_kernel<true>, opted)) return e;
         return launch(attn_kv4_kernel<true>, dim3((unsigned)(p.hkv * p.blocks), (unsigned)p.rows), dim3(32 * kKv4Warps), kKv4Smem, s, p);
@@ -544,7 +612,9 @@ extern "C" int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *
     // the second kernel starts early and waits for the first one's sums itself
     const bool before = pdl_enabled();
     rptc_set_pdl(1);
-    const int e = launch(attn_kv4_join_kernel, dim3((unsigned)heads, (unsigned)p.rows), dim3(512), 0, s, p, (uint32_t)ctas);
+    const int64_t items = (int64_t)p.rows * p.hkv * p.blocks;
+    const int e = launch(attn_kv4_join_kernel, dim3((unsigned)(items < ctas ? items : ctas), (unsigned)(p.group < 8 ? p.group : 8)), dim3(32 * kKv4JoinWarps), 0, s, p,
+                         (uint32_t)ctas, items < ctas ? 1 : 0);
     rptc_set_pdl(before ? 1 : 0);
     return e;
 }

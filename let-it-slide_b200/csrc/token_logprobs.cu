@@ -4,10 +4,12 @@
 //
 // One pass over the row: a thread keeps M, z and w of its own entries, and they meet at the end.  (x - M first and then its multiple of log2(e): x log2(e) would leave
 // fp32's range at the lowest values that masks are made of.)  The largest entries need no second pass either: a thread knows its largest entry, the k-th largest of
-// those is a lower bound of the k-th largest entry, and only the (at most k, but for ties) threads that reach it look at their entries again.  What they find is ranked by
+// those is a lower bound of the k-th largest entry, and only the (at most k, but for ties) threads that reach it have anything to look for: all threads look, at the few vectors
+// that such a thread had read together with its largest entry, and at all of its entries where another of them reaches the bound too.  What is found is ranked by
 // (value, index).  Where more is found than there is room for, as in a row of equal entries, the k largest are taken one by one, a pass over the row each.
 // Few rows: a cluster of CTAs shares a row, and each one's sums and k largest meet in the first one's shared memory.
-// Bound: HBM, with the special-function unit (an exponential per entry) next: 2048 x 32000 in fp16 20.0 us of traffic, 14.6 of exponentials.
+// Bound: HBM, with the special-function unit (an exponential per entry) next: 2048 x 32000 in fp16 20.0 us of traffic, 14.6 of exponentials; 27.5 us measured, 34 with the
+// largest entry, 43 with the 20 largest (the meetings of a row's threads, while the SM's other rows read on).  1500 x 128001 in fp32: 117 of traffic, 131, 137 and 146.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -458,8 +460,9 @@ extern "C" int rptc_token_logprobs(const void *logits, int dtype, int64_t ld, co
     LogprobParams p = {logits, ld, targets, logprob, entropy, top_logprobs, top_ids, n, top, device_status_word()};
     if (!p.status) return RPTC_ERR_CUDA;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // Few rows: up to eight CTAs share one, as long as each has 8 KiB of it.
+    // Few rows: up to eight CTAs share one, as long as each has 32 KiB of it (one row of 8192 in fp16: four CTAs 3.8 us, one 2.5; 32000 in fp16: 4.4 and 4.6; 128001 in
+    // fp32: eight 6.8, one 15.8; 148 rows of 32000: two 5.7, one 4.9).
     int cluster = 1;
-    while (cluster < kLogprobMaxCluster && rows * cluster * 2 <= 2 * num_sms() && n * (dtype == 2 ? 4 : 2) >= cluster * 2 * 8192) cluster *= 2;
+    while (cluster < kLogprobMaxCluster && rows * cluster * 2 <= 2 * num_sms() && n * (dtype == 2 ? 4 : 2) >= cluster * 2 * 32768) cluster *= 2;
     return dtype == 0 ? launch_logprobs<0>(p, rows, cluster, s) : dtype == 1 ? launch_logprobs<1>(p, rows, cluster, s) : launch_logprobs<2>(p, rows, cluster, s);
 }
