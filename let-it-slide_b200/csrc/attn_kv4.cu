@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
     }
     // The next item's comes by asynchronous copies into what only this warp reads of the merge buffer (a lane its own bytes); a plain load would wait behind all that the rings
     // ask for, some 7000 clocks.
-    const uint32_t q_lane = smem_addr(merge) + 512u * warp + 16u * lane;      // its head of the first four warps' sums
+    auto q_lane = [&](int j) { return smem_addr(merge) + 512u * (8 * j + warp) + 16u * lane; };      // its head of the first four warps' sums
     int stage_no = 0;
     for (bool started = false;; started = true) {
         const uint32_t cache_at = cache_of(row, head);
@@ -244,14 +244,13 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             }
             n_t1 = kv4_tile_of(min(kv4_cost(kv4_tiles(n_context)), units));
         }
-        const uint32_t n_cache_at = WHOLE ? 0u : cache_of(n_row, n_head);
         // A tile is 320 pieces of 16 bytes, ten of them a lane's.  (Bulk copies by four lanes took about 70 instructions a tile more: they are issued lane by lane.)
         auto fetch = [&](int tile, int stage) {
             const bool next = !WHOLE && tile >= t1;
             if (next) tile = warp + ((tile - t1) & ~(kKv4Warps - 1));
             if (tile < (next ? n_t1 : t1)) {
                 const uint32_t dst = ring + (uint32_t)stage * kKv4StageBytes + 16u * lane, first = (uint32_t)tile * kKv4Tile;
-                const uint32_t place = (next ? n_cache_at : cache_at) + first;
+                const uint32_t place = (next ? cache_of(n_row, n_head) : cache_at) + first;
                 const int n = (next ? n_context : context) - (int)first;
                 const uint64_t codes = (uint64_t)place * kKv4Codes + 16 * lane, scales = (uint64_t)(place + lane) * 4;
                 const uint8_t *kc = p.k + codes, *vc = p.v + codes;
@@ -282,7 +281,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             const __half *q = q_of(n_row, n_head);
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (q) cp_async16(q_lane + 4096u * j, q + 32 * j);
+                if (q) cp_async16(q_lane(j), q + 32 * j);
         }
         // The ring's next stages: after the first item they are under way, but for those that a short one does not fill.  The second one asks for its tile after q.
         if (!started || t0 + warp >= t1) fetch(t0 + warp, stage_no);
@@ -447,7 +446,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             cp_async_wait<kKv4Stages - 1>();
             const bool there = q_of(n_row, n_head);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) raw[j] = there ? lds128_at<0>(q_lane + 4096u * j) : make_uint4(0u, 0u, 0u, 0u);
+            for (int j = 0; j < 4; ++j) raw[j] = there ? lds128_at<0>(q_lane(j)) : make_uint4(0u, 0u, 0u, 0u);
         }
         const int kvh = head / p.blocks, first = (head - kvh * p.blocks) * 8, in_block = min(8, p.group - first), q_head = kvh * p.group + first;
         __syncthreads();                             // the last item's sums have been taken
