@@ -15,7 +15,7 @@
 // Weights refer to a running maximum of s + log2(a tile's largest scale): the products p * scale then fit fp16 whatever the scales are (2^11 where the reference was set, and
 // it moves only when they may pass 2^15, which their sum shows: no maximum is looked for otherwise; what falls below 2^-14 is 2^-25 of the largest).
 // Bound: HBM (160 bytes per position and kv head) with the issue slots close behind, about 350 warp instructions per 16 positions: four rows in flight per scheduler at 128
-// registers leave a quarter of the slots empty.  32 rows of 500 to 32768 positions, 8 kv heads: 140 us, 4.9 TB/s; one row of 131072: 45 us, 3.7 TB/s; one of 200: 4.6 us.
+// registers leave a quarter of the slots empty.  32 rows of 500 to 32768 positions, 8 kv heads: 142 us, 4.8 TB/s; one row of 131072: 45 us, 3.7 TB/s; one of 200: 4.6 us.
 // Long contexts: all tiles of all rows and heads, laid end to end, are cut into equal ranges for the CTAs of one wave, so that rows of different lengths balance; a range's
 // part of a row goes to the workspace (fp32) and a second kernel joins the parts.  A warp's ring goes on into the range's next item: its first tiles and its q are on their
 // way while the item before is finished (32 rows as above 160 us without, and with a join that looked at every row's heads instead of the ranges' ends).
@@ -56,7 +56,7 @@ __device__ __forceinline__ int kv4_context(const AttnKv4Params &p, const int32_t
 __device__ __forceinline__ int kv4_tiles(int context) { return (context + kKv4Tile - 1) / kKv4Tile; }
 
 // How the work is cut: every row's heads laid end to end, each worth its tiles and kKv4Start for what a CTA does around them (q, the warps' sums).  32 rows of 500 to 32768
-// took 158 us with 12 of those, 150 with 16, 145 with 24 and 146 with 32; kKv4Least is what a CTA is worth starting for.  In numbers of 32 bits: a unit stands for a tile of
+// take 143 us with 16 of those, 141.7 with 24, 143.5 with 32 and 147 with 48; kKv4Least is what a CTA is worth starting for.  In numbers of 32 bits: a unit stands for a tile of
 // 5 KiB of the cache.
 constexpr uint32_t kKv4Start = 24, kKv4Least = 16;
 __device__ __forceinline__ uint32_t kv4_cost(int tiles) { return tiles ? (uint32_t)tiles + kKv4Start : 0u; }

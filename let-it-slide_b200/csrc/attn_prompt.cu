@@ -16,6 +16,10 @@
 // lies there has to be 0.
 // Items go to CTAs longest first, there and back again (the longest of a round meets the shortest of the next): the order is worked out from
 // `starts` on the device, by counting items of at least a number of tiles.
+// Bound: the exponentials.  A tile of 128 keys and 256 rows takes 2770 to 3000 clocks: 2048 for its 32768 exponentials on the special-function unit (busy 69 % of the time at
+// 8192 tokens, as is the tensor pipe), 1024 for its products, the rest the softmax warps' other work.  One prompt of 2048 tokens, 32 heads of 128: 37.6 us (fp16, 0.91 PFLOP/s);
+// one of 8192, 64 heads over 8: 845 us (1.30 PFLOP/s, at the power cap).  A short prompt pays for its set-up too: first scores after some 7000 clocks, the last result 2200 after
+// the last product; 24 tokens take 6.6 us.  Sixteen sequences of 1 to 1024 tokens with `pack` heads together 80 us, with one head at a time 112.
 #include <cuda_bf16.h>
 
 #include "tc_ptx.cuh"
@@ -70,7 +74,8 @@ struct PromptItem {
     int32_t pad[2];
 };
 
-// The items in their order, by one warp.  A lane holds sequence number `lane`; those from 32 on are read again whenever they are counted.
+// The items in their order, by one warp.  A lane holds sequence number `lane`; those from 32 on are read again whenever they are counted.  Of one sequence alone, which all
+// lanes hold, the order is the reverse of its rows.
 struct ItemList {
     const PromptParams &p;
     int lane, shift, groups, most;                   // most: tiles of the longest item
@@ -79,6 +84,12 @@ struct ItemList {
     __device__ __forceinline__ ItemList(const PromptParams &params, int l) : p(params), lane(l) {
         shift = 8 - (31 - __clz(p.pack));
         groups = p.kv_heads * p.group / p.pack;
+        most = 1;
+        if (p.sequences == 1) {
+            mine = sequence(p, 0);
+            total = (uint32_t)items_of(mine, shift, 1) * groups;
+            return;
+        }
         mine = {0, 0, 0, 0};
         if (lane < p.sequences) mine = sequence(p, lane);
         most = mine.n > 0 ? (mine.m + kTileKeys - 1) / kTileKeys : 1;
@@ -94,45 +105,51 @@ struct ItemList {
     }
     __device__ __forceinline__ PromptItem item(uint32_t index) const {
         const int per_item = 1 << shift, rank = (int)(index / (uint32_t)groups), heads = (int)(index - (uint32_t)rank * groups);
-        int lo = 1, hi = most;                       // the largest c of which there are more than `rank`
-        while (lo < hi) {
-            const int mid = lo + (hi - lo + 1) / 2;
-            if (count(mid) > rank) lo = mid;
-            else hi = mid - 1;
-        }
-        int left = rank - count(lo + 1);
-        PromptItem it = {};
-        for (int s0 = 0; s0 < p.sequences; s0 += 32) {
-            Sequence q = mine;
-            if (s0 > 0) q = s0 + lane < p.sequences ? sequence(p, s0 + lane) : Sequence{0, 0, 0, 0};
-            const int from = items_of(q, shift, lo), here = from - items_of(q, shift, lo + 1);
-            int upto = here;
+        Sequence q = mine;
+        int j = items_of(mine, shift, 1) - 1 - rank, found = 1;
+        if (p.sequences > 1) {
+            found = 0;
+            int lo = 1, hi = most;                   // the largest c of which there are more than `rank`
+            while (lo < hi) {
+                const int mid = lo + (hi - lo + 1) / 2;
+                if (count(mid) > rank) lo = mid;
+                else hi = mid - 1;
+            }
+            int left = rank - count(lo + 1);
+            for (int s0 = 0; s0 < p.sequences; s0 += 32) {
+                if (s0 > 0) q = s0 + lane < p.sequences ? sequence(p, s0 + lane) : Sequence{0, 0, 0, 0};
+                const int from = items_of(q, shift, lo), here = from - items_of(q, shift, lo + 1);
+                int upto = here;
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
-                if (lane >= o) upto += v;
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int v = __shfl_up_sync(0xFFFFFFFFu, upto, o);
+                    if (lane >= o) upto += v;
+                }
+                const unsigned hit = __ballot_sync(0xFFFFFFFFu, left < upto);
+                if (hit == 0) {
+                    left -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+                    continue;
+                }
+                const int in = __ffs(hit) - 1;
+                j = __shfl_sync(0xFFFFFFFFu, ((q.n + per_item - 1) >> shift) - from + left - (upto - here), in);
+                q.q0 = __shfl_sync(0xFFFFFFFFu, q.q0, in), q.n = __shfl_sync(0xFFFFFFFFu, q.n, in);
+                q.k0 = __shfl_sync(0xFFFFFFFFu, q.k0, in), q.m = __shfl_sync(0xFFFFFFFFu, q.m, in);
+                found = 1;
+                break;
             }
-            const unsigned hit = __ballot_sync(0xFFFFFFFFu, left < upto);
-            if (hit == 0) {
-                left -= __shfl_sync(0xFFFFFFFFu, upto, 31);
-                continue;
-            }
-            const int in = __ffs(hit) - 1, j = __shfl_sync(0xFFFFFFFFu, ((q.n + per_item - 1) >> shift) - from + left - (upto - here), in);
-            q.q0 = __shfl_sync(0xFFFFFFFFu, q.q0, in), q.n = __shfl_sync(0xFFFFFFFFu, q.n, in);
-            q.k0 = __shfl_sync(0xFFFFFFFFu, q.k0, in), q.m = __shfl_sync(0xFFFFFFFFu, q.m, in);
-            const int splits = p.group / p.pack;
-            it.go = 1;
-            it.kv_head = heads / splits;
-            it.head = it.kv_head * p.group + (heads - it.kv_head * splits) * p.pack;
-            it.token = q.q0 + j * per_item;
-            it.tokens = min(per_item, q.n - j * per_item);
-            it.k0 = q.k0, it.keys = q.m;
-            it.seen = q.m - q.n + j * per_item;
-            const int last0 = it.seen + min(it.tokens, per_item / 2), last1 = it.seen + it.tokens;      // keys that a half's last query sees
-            it.tiles0 = max(0, (last0 + kTileKeys - 1) / kTileKeys);
-            it.tiles1 = it.tokens > per_item / 2 ? max(0, (last1 + kTileKeys - 1) / kTileKeys) : 0;
-            break;
         }
+        const int splits = p.group / p.pack;
+        PromptItem it = {};
+        it.go = found;
+        it.kv_head = heads / splits;
+        it.head = it.kv_head * p.group + (heads - it.kv_head * splits) * p.pack;
+        it.token = q.q0 + j * per_item;
+        it.tokens = min(per_item, q.n - j * per_item);
+        it.k0 = q.k0, it.keys = q.m;
+        it.seen = q.m - q.n + j * per_item;
+        const int last0 = it.seen + min(it.tokens, per_item / 2), last1 = it.seen + it.tokens;      // keys that a half's last query sees
+        it.tiles0 = max(0, (last0 + kTileKeys - 1) / kTileKeys);
+        it.tiles1 = it.tokens > per_item / 2 ? max(0, (last1 + kTileKeys - 1) / kTileKeys) : 0;
         return it;
     }
 };
