@@ -107,6 +107,7 @@ class RPTCLlama:
             self.vcache = [torch.zeros((rows, cfg.max_pos, self.kv_heads_l, cfg.head_dim), **f16) for _ in range(cfg.layers)]
         else:
             self.kv4 = [ops.kv4_cache(rows, cfg.max_pos, self.kv_heads_l, self.device) for _ in range(cfg.layers)]
+        self._kv4_joins = kv_bits == 4 and ops.attn_decode_kv4_joins(self.kv4[0], self.heads_l)
         self._angles: torch.Tensor | None = None       # see _rope_table
         # step workspace (fixed addresses, so that the step can live in a CUDA graph)
         self.ids = torch.zeros(rows, dtype=torch.int32, device=device)
@@ -149,6 +150,7 @@ class RPTCLlama:
         self.graph: torch.cuda.CUDAGraph | None = None
         self.launches_per_step = 0
         self._pos_hi = 0            # host-side upper bound of the positions on the device (see step)
+        self._behind = [0] * rows   # how far each row's position is below it
 
     # -- one token for every row ---------------------------------------------------------------------
     def _fusable(self) -> bool:
@@ -185,7 +187,7 @@ class RPTCLlama:
 
     def _join_launches(self) -> int:
         """Attention over long 4-bit caches joins the parts of a context in a launch of its own."""
-        return len(self.blocks) if self.kv_bits == 4 and self.cfg.max_pos > 1024 else 0
+        return len(self.blocks) if self._kv4_joins else 0
 
     def step_eager(self) -> None:
         if self._glueable():
@@ -508,7 +510,9 @@ class RPTCLlama:
 
     def sync_positions(self) -> None:
         """Re-reads the device-side positions after they were edited directly (`model.pos.copy_(...)`)."""
-        self._pos_hi = int(self.pos.max().item())
+        at = self.pos.tolist()
+        self._pos_hi = max(at)
+        self._behind = [self._pos_hi - p for p in at]
 
     def _claim_positions(self, n_steps: int) -> None:
         """The positions live on the device and advance with every replay of the captured step; the host keeps an upper
@@ -528,7 +532,7 @@ class RPTCLlama:
 
     def reset(self, ids: torch.Tensor | None = None) -> None:
         self.pos.zero_()
-        self._pos_hi = 0
+        self._pos_hi, self._behind = 0, [0] * self.rows
         self._acc_pool.zero_()      # the short chain leaves acc_o / acc_gu to the next token's first launch
         self.acc_gu2.zero_()
         if ids is not None:
@@ -571,7 +575,7 @@ class RPTCLlama:
 
         last = self._prompt_blocks(h, attend, lambda t: t.view(R, T, -1)[:, -1].contiguous())
         self.pos.fill_(T - 1)
-        self._pos_hi = T
+        self._pos_hi, self._behind = T, [0] * self.rows
         return self._greedy(last)
 
     def _greedy(self, last: torch.Tensor) -> torch.Tensor:
@@ -625,8 +629,12 @@ class RPTCLlama:
             raise ValueError("prompts must be one row of at least one token each, one for every row of the model")
         if D != 128:
             raise ValueError("packed prompts need heads of 128")
-        if self._pos_hi + max(lengths) > cfg.max_pos:
-            raise ValueError(f"{max(lengths)} tokens behind position {self._pos_hi}, but the KV caches hold max_pos = {cfg.max_pos} positions")
+        ends = [self._pos_hi - b + l for b, l in zip(self._behind, lengths + [0] * (self.rows - n))]
+        if max(ends) > cfg.max_pos:
+            raise ValueError(f"row {ends.index(max(ends))} would have {max(ends)} positions, but the KV caches hold max_pos = {cfg.max_pos}")
+        ids = torch.cat([p.long() for p in prompts])
+        if not bool(((ids >= 0) & (ids < cfg.vocab)).all()):
+            raise ValueError(f"token ids must be between 0 and {cfg.vocab - 1}")
         fresh = self._pos_hi == 0                                # no row holds anything
         total = sum(lengths)
         i32 = dict(dtype=torch.int32, device=self.device)
@@ -655,11 +663,12 @@ class RPTCLlama:
             k, v = ops.kv4_values(self.kv4[i], count, values) if self.kv_bits == 4 else (self.kcache[i], self.vcache[i])
             return ops.attn_prompt(q, k.flatten(0, 1), v.flatten(0, 1), starts, kv_first, kv_len).flatten(1)
 
-        h = self.embed[torch.cat([p.long() for p in prompts])]
+        h = self.embed[ids]
         last = (starts[1:] - 1).long()
         out = self._prompt_blocks(h, attend, (lambda t: t) if whole else (lambda t: t[last]))
         self.pos[:n] += length - 1
-        self._pos_hi += max(lengths)
+        self._pos_hi = max(ends)
+        self._behind = [self._pos_hi - e for e in ends]
         return out
 
     def _prompt_blocks(self, h: torch.Tensor, attend, pick) -> torch.Tensor:

@@ -487,6 +487,11 @@ def attn_decode_kv4(q: torch.Tensor, pos: torch.Tensor, cache, heads: int, out: 
     return out
 
 
+def attn_decode_kv4_joins(cache, heads: int) -> bool:
+    """Whether `attn_decode_kv4` over this cache takes a workspace, and a second launch that joins the parts of a row in it."""
+    return lib().rptc_attn_decode_kv4_workspace_bytes(ctypes.byref(_kv_cache(cache, cache[0].device)), heads) > 0
+
+
 def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, starts: torch.Tensor, kv_first: torch.Tensor | None = None,
                 kv_len: torch.Tensor | None = None, out: torch.Tensor | None = None, scale: float | None = None) -> torch.Tensor:
     """Causal attention of packed prompts of different lengths (rptc_attn_prompt): q [tokens, heads, d], k and v [kv_tokens, kv_heads, d], fp16 or

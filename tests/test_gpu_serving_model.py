@@ -148,6 +148,48 @@ def test_four_bits_in_every_chain(hidden, kv_heads, rows, max_pos):
                 close(model.logits[r], reference(model, tokens[r, :t + 1], 0, 4, r)[-1], 1e-2 if hidden < 4096 else 2e-2)
 
 
+@pytest.mark.parametrize("kv_bits", [16, 4])
+def test_rows_fill_their_caches_by_themselves(kv_bits):
+    """A row has the room behind its own position, wherever the others are."""
+    model = make(rows=2, kv_bits=kv_bits)
+    first, second = texts([90, 2]), texts([1, 60], seed=3)
+    model.prefill_packed(first)
+    logits = model.extend(second)
+    for r in range(2):
+        tokens = torch.cat((first[r], second[r]))
+        close(logits[r], reference(model, tokens, len(first[r]), kv_bits, r)[-1])
+    assert model.pos.tolist() == [91, 62] and model._pos_hi == 91 and model._behind == [0, 29]
+    for _ in range(5):
+        model.step()
+    with pytest.raises(RuntimeError):
+        model.step()
+    with pytest.raises(ValueError):
+        model.extend(texts([1, 1]))
+    model.pos.copy_(torch.tensor([10, 80], device="cuda"))
+    model.sync_positions()
+    with pytest.raises(ValueError):
+        model.extend(texts([1, 17]))
+    model.extend(texts([86, 16]))
+    assert model.pos.tolist() == [96, 96]
+
+
+def test_launches_of_long_four_bit_caches():
+    """A second launch where a workspace takes the parts of a row."""
+    import ctypes
+
+    from rptc_b200 import ops
+    from rptc_b200._lib import lib
+    for rows, max_pos in ((1, 1024), (1, 2048), (64, 2048), (64, 2049)):
+        cache = ops.kv4_cache(rows, max_pos, 2)
+        joins = ops.attn_decode_kv4_joins(cache, 4)
+        assert joins == (lib().rptc_attn_decode_kv4_workspace_bytes(ctypes.byref(ops._kv_cache(cache, cache[0].device)), 4) > 0)
+        assert joins == (max_pos > 2048 or (rows, max_pos) == (1, 2048))
+    long, short = make(rows=2, kv_bits=4, max_pos=1500), make(rows=2, kv_bits=4)
+    for model in (long, short):
+        model.step()
+    assert long.launches_per_step == short.launches_per_step + len(long.blocks)
+
+
 def test_scores_are_the_log_probabilities_of_the_next_tokens():
     model = make(rows=2)
     prompts = texts([30, 1, 9, 2, 50])
@@ -173,9 +215,14 @@ def test_what_is_refused():
             model.prefill_packed(bad)
     with pytest.raises(ValueError):
         model.prefill_packed([a, texts([97])[0]])
+    for bad in (-1, 1024):                                           # no such token
+        with pytest.raises(ValueError):
+            model.prefill_packed([a, torch.tensor([3, bad])])
+        with pytest.raises(ValueError):
+            model.score([torch.tensor([bad, 2])])
     model.prefill_packed(texts([90, 1]))
     with pytest.raises(ValueError):
-        model.extend([a, texts([7])[0]])
+        model.extend([texts([7])[0], a])
     with pytest.raises(ValueError):
         RPTCLlama(LlamaConfig(hidden=512, layers=1, heads=8, kv_heads=8, head_dim=64, ffn=1024, vocab=64), kv_bits=4)
     with pytest.raises(ValueError):
