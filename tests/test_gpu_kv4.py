@@ -255,6 +255,31 @@ def test_attention_over_long_contexts(heads, hkv, rows, context):
     check(ops.attn_decode_kv4(q, pos, cache, heads), q, pos, cache, heads)
 
 
+@pytest.mark.parametrize("heads,hkv,rows,max_pos,most", [(8, 8, 40, 2100, 2100), (64, 4, 40, 2100, 700), (2, 1, 300, 2049, 90), (3, 3, 100, 2304, 2304), (8, 8, 36, 2500, 40), (8, 2, 70, 4000, 1)])
+def test_attention_of_many_rows(heads, hkv, rows, max_pos, most):
+    """More items than ranges, and fewer: lengths of all sizes, rows of no sequence among them, a range's end at any place of an item."""
+    from rptc_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    cache = random_cache(g, rows, max_pos, hkv)
+    q = torch.randn(rows, heads * 128, generator=g, device="cuda").half()
+    pos = torch.randint(-1, most, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    pos[0], pos[rows - 1] = most - 1, -1
+    for r, n in enumerate(pos.tolist()):
+        for t in cache[1], cache[3]:
+            t[r, :, n + 1:] = math.nan
+    got = ops.attn_decode_kv4(q, pos, cache, heads)
+    check(got, q, pos, cache, heads)
+    assert (got[pos < 0] == 0).all()
+    for last in (0, rows // 2, rows - 1):                      # one row alone
+        alone = torch.full_like(pos, -1)
+        alone[last] = most - 1
+        for t in cache[1], cache[3]:
+            t[last].nan_to_num_(nan=0.5)
+        check(ops.attn_decode_kv4(q, alone, cache, heads), q, alone, cache, heads)
+    assert (ops.attn_decode_kv4(q, torch.full_like(pos, -1), cache, heads) == 0).all()
+    ops.device_status()
+
+
 @pytest.mark.parametrize("spread,offset,q_spread,scale", [(1e-4, 0, 1, None), (300, 0, 0.1, 1e-3), (1, 50, 1, None), (1, 0, 40, None), (1, 0, 1e-4, 1.0), (0.0, 2.0, 1, None),
                                                           (1, 0, 1000, 1e-2)])
 def test_values_of_all_sizes(spread, offset, q_spread, scale):
