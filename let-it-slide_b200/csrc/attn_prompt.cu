@@ -75,12 +75,13 @@ struct PromptItem {
 };
 
 // The items in their order, by one warp.  A lane holds sequence number `lane`; those from 32 on are read again whenever they are counted.  Of one sequence alone, which all
-// lanes hold, the order is the reverse of its rows.
+// lanes hold, the order is the reverse of its rows.  Items are asked for in rising order: a search goes on where the last one ended.
 struct ItemList {
     const PromptParams &p;
-    int lane, shift, groups, most;                   // most: tiles of the longest item
+    int lane, shift, groups, most, all = 0;          // most: tiles of the longest item; all: items of a group of heads
     uint32_t total;
     Sequence mine;
+    int c = 0, before = 0, end = 0, s0 = 0;          // items of c tiles end in front of `end`; `before` are in front of those of c tiles of sequence s0
     __device__ __forceinline__ ItemList(const PromptParams &params, int l) : p(params), lane(l) {
         shift = 8 - (31 - __clz(p.pack));
         groups = p.kv_heads * p.group / p.pack;
@@ -96,29 +97,33 @@ struct ItemList {
         for (int s = lane + 32; s < p.sequences; s += 32)
             if (const Sequence q = sequence(p, s); q.n > 0) most = max(most, (q.m + kTileKeys - 1) / kTileKeys);
         most = max(1, __reduce_max_sync(0xFFFFFFFFu, most));
-        total = (uint32_t)count(1) * groups;         // at most 2^28 for the rows and 2^28 for the sequences
+        all = count(1);
+        total = (uint32_t)all * groups;              // at most 2^28 for the rows and 2^28 for the sequences
     }
-    __device__ __forceinline__ int count(int c) const {
-        int n = items_of(mine, shift, c);
-        for (int s = lane + 32; s < p.sequences; s += 32) n += items_of(sequence(p, s), shift, c);
+    __device__ __forceinline__ int count(int tiles) const {                          // items of at least so many
+        int n = items_of(mine, shift, tiles);
+        for (int s = lane + 32; s < p.sequences; s += 32) n += items_of(sequence(p, s), shift, tiles);
         return __reduce_add_sync(0xFFFFFFFFu, n);
     }
-    __device__ __forceinline__ PromptItem item(uint32_t index) const {
+    __device__ __forceinline__ PromptItem item(uint32_t index) {
         const int per_item = 1 << shift, rank = (int)(index / (uint32_t)groups), heads = (int)(index - (uint32_t)rank * groups);
         Sequence q = mine;
         int j = items_of(mine, shift, 1) - 1 - rank, found = 1;
         if (p.sequences > 1) {
             found = 0;
-            int lo = 1, hi = most;                   // the largest c of which there are more than `rank`
-            while (lo < hi) {
-                const int mid = lo + (hi - lo + 1) / 2;
-                if (count(mid) > rank) lo = mid;
-                else hi = mid - 1;
+            if (rank >= end) {                       // the largest c of which there are more than `rank`
+                int hi = most;
+                c = 1, end = all;
+                while (c < hi) {
+                    const int mid = c + (hi - c + 1) / 2, n = count(mid);
+                    if (n > rank) c = mid, end = n;
+                    else hi = mid - 1;
+                }
+                before = count(c + 1), s0 = 0;
             }
-            int left = rank - count(lo + 1);
-            for (int s0 = 0; s0 < p.sequences; s0 += 32) {
+            for (; s0 < p.sequences; s0 += 32) {
                 if (s0 > 0) q = s0 + lane < p.sequences ? sequence(p, s0 + lane) : Sequence{0, 0, 0, 0};
-                const int from = items_of(q, shift, lo), here = from - items_of(q, shift, lo + 1);
+                const int from = items_of(q, shift, c), here = from - items_of(q, shift, c + 1), left = rank - before;
                 int upto = here;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -127,7 +132,7 @@ struct ItemList {
                 }
                 const unsigned hit = __ballot_sync(0xFFFFFFFFu, left < upto);
                 if (hit == 0) {
-                    left -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+                    before += __shfl_sync(0xFFFFFFFFu, upto, 31);
                     continue;
                 }
                 const int in = __ffs(hit) - 1;
@@ -210,7 +215,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
         pdl_wait_prior_grids();
         PromptParams q = p;
         q.starts = after_wait(p.starts), q.kv_first = after_wait(p.kv_first), q.kv_len = after_wait(p.kv_len);
-        const ItemList items_in_order(q, lane);
+        ItemList items_in_order(q, lane);
         const uint32_t total = items_in_order.total;
         PromptItem next = {};
         if (blockIdx.x < total) next = items_in_order.item(blockIdx.x);

@@ -243,3 +243,17 @@ def test_many_short_prompts():
     q, k, v = rand(g, (T, 4, 128), torch.float16), rand(g, (T, 1, 128), torch.float16), rand(g, (T, 1, 128), torch.float16)
     got = ops.attn_prompt(q, k, v, starts_of(lengths))
     check(got, *reference(q, k, v, spans_of(lengths), 128 ** -0.5))
+
+
+def test_thousands_of_prompts_of_all_lengths():
+    """Items of one to many tiles over many more sequences than lanes, some of them empty, in groups whose heads do and do not share an item."""
+    from rptc_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(12)
+    lengths = [(0, 1, 2, 9, 130, 3, 0, 31)[i % 8] if i % 97 else 300 + i // 3 for i in range(1500)]
+    past = [(i * 13) % 40 if i % 5 else 200 * (i % 3) for i in range(1500)]
+    T, S = sum(lengths), sum(lengths) + sum(past)
+    q, k, v = rand(g, (T, 6, 64), torch.bfloat16), rand(g, (S, 2, 64), torch.bfloat16), rand(g, (S, 2, 64), torch.bfloat16)
+    spans = spans_of(lengths, past)
+    got = ops.attn_prompt(q, k, v, starts_of(lengths), int32([s[2] for s in spans]), int32([s[3] for s in spans]))
+    check(got, *reference(q, k, v, spans, 64 ** -0.5))
+    ops.device_status()
