@@ -372,7 +372,7 @@ int rptc_attn_prompt(const rptc_prompt_attention *a, rptc_stream_t stream);
  * bits = 4: k, v codes uint8 [rows][kv_heads][max_pos][64], k_scales, v_scales fp16 [rows][kv_heads][max_pos][4][2]: for each group of 32
  * values (scale, minimum), scale = fp16((max - min) / 15) and code = round((x - min) / scale), half to even, at most 15 (0 where the
  * scale is 0); the code stands for minimum + code * scale.  Value e of group g is nibble e % 4 of the 16-bit word 4 * (e / 4) + g: dims 4 i .. 4 i + 3 of all four groups
- * are eight bytes.  All 16-byte aligned, contiguous. */
+ * are eight bytes.  All 16-byte aligned, contiguous.  At most 65535 rows, 2^24 positions and 4096 kv heads. */
 typedef struct rptc_kv_cache {
     void *k, *k_scales, *v, *v_scales;
     int64_t rows, max_pos;
@@ -401,13 +401,13 @@ typedef struct rptc_append {
 int rptc_qkv_append(const rptc_append *a, rptc_stream_t stream);
 
 /* The values that the first count[r] positions of each row of a 4-bit cache stand for: k_out, v_out fp16 [rows][max_pos][kv_heads][128], other
- * positions are left as they are.  count outside [0, max_pos]: RPTC_ERR_RANGE, nothing of that row is written. */
+ * positions are left as they are.  count outside [0, max_pos]: RPTC_ERR_RANGE, nothing of that row is written.  rows * kv_heads at most 65535. */
 int rptc_kv4_values(const rptc_kv_cache *cache, const int32_t *count, void *k_out, void *v_out, rptc_stream_t stream);
 
 /* Single-query attention of each row's q heads over positions 0 .. pos[row] of a 4-bit cache: rptc_attn_decode for it.  q fp16 [rows][ld_q], 16-byte aligned,
  * ld_q % 8 == 0; out fp16 [rows][ld_out], q heads of 128.  heads a multiple of cache->kv_heads; signs_in as in rptc_attn_decode.
  * pos -1: a row of no sequence, whose out is zeros; any other position outside the cache: zeros, RPTC_ERR_RANGE.  workspace: 256-byte aligned device
- * memory of rptc_attn_decode_kv4_workspace_bytes; it holds nothing between calls. */
+ * memory of rptc_attn_decode_kv4_workspace_bytes; it holds nothing between calls, and calls that may overlap need one each. */
 int64_t rptc_attn_decode_kv4_workspace_bytes(const rptc_kv_cache *cache, int heads);
 int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *pos, const rptc_kv_cache *cache, void *out, int64_t ld_out, int heads,
                          float scale, const void *signs_in, void *workspace, int64_t workspace_bytes, rptc_stream_t stream);

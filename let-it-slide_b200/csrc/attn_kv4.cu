@@ -238,9 +238,16 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
         int n_row = row, n_head = head + 1, n_context = context, n_t1 = 0;
         if (!WHOLE && units) {
             if (n_head == heads) {
-                n_head = 0;
-                do n_context = kv4_context(p, pos, ++n_row);
-                while (n_context == 0 && n_row + 1 < p.rows);
+                n_head = n_context = 0;
+                for (++n_row; n_row < p.rows; n_row += 32) {      // over rows without positions
+                    const int here = n_row + lane < p.rows ? kv4_context(p, pos, n_row + lane) : 0;
+                    const unsigned hit = __ballot_sync(0xFFFFFFFFu, here != 0);
+                    if (hit) {
+                        n_row += __ffs(hit) - 1;
+                        n_context = __shfl_sync(0xFFFFFFFFu, here, __ffs(hit) - 1);
+                        break;
+                    }
+                }
             }
             n_t1 = kv4_tile_of(min(kv4_cost(kv4_tiles(n_context)), units));
         }

@@ -280,6 +280,21 @@ def test_attention_of_many_rows(heads, hkv, rows, max_pos, most):
     ops.device_status()
 
 
+def test_attention_of_a_few_rows_among_idle_ones():
+    """A range's next item may be hundreds of rows on."""
+    from rptc_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(5)
+    cache = random_cache(g, 400, 2200, 2)
+    q = torch.randn(400, 4 * 128, generator=g, device="cuda").half()
+    for rows in ([0, 1, 399], [31, 32, 95, 96, 300], [399], [7] + list(range(200, 330))):
+        pos = torch.full((400,), -1, dtype=torch.int32, device="cuda")
+        pos[rows] = torch.randint(0, 2200, (len(rows),), generator=g, device="cuda", dtype=torch.int32)
+        got = ops.attn_decode_kv4(q, pos, cache, 4)
+        check(got, q, pos, cache, 4)
+        assert (got[pos < 0] == 0).all()
+    ops.device_status()
+
+
 @pytest.mark.parametrize("spread,offset,q_spread,scale", [(1e-4, 0, 1, None), (300, 0, 0.1, 1e-3), (1, 50, 1, None), (1, 0, 40, None), (1, 0, 1e-4, 1.0), (0.0, 2.0, 1, None),
                                                           (1, 0, 1000, 1e-2)])
 def test_values_of_all_sizes(spread, offset, q_spread, scale):
