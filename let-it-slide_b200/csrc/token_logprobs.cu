@@ -8,8 +8,8 @@
 // that such a thread had read together with its largest entry, and at all of its entries where another of them reaches the bound too.  What is found is ranked by
 // (value, index).  Where more is found than there is room for, as in a row of equal entries, the k largest are taken one by one, a pass over the row each.
 // Few rows: a cluster of CTAs shares a row, and each one's sums and k largest meet in the first one's shared memory.
-// Bound: HBM, with the special-function unit (an exponential per entry) next: 2048 x 32000 in fp16 20.0 us of traffic, 14.6 of exponentials; 27.5 us measured, 34 with the
-// largest entry, 43 with the 20 largest (the meetings of a row's threads, while the SM's other rows read on).  1500 x 128001 in fp32: 117 of traffic, 131, 137 and 146.
+// Bound: HBM, with the special-function unit (an exponential per entry) next: 2048 x 32000 in fp16 20.0 us of traffic, 14.6 of exponentials; 27.5 us measured, 33 with the
+// largest entry, 39 with the 20 largest (the meetings of a row's threads, while the SM's other rows read on).  1500 x 128001 in fp32: 117 of traffic, 131, 137 and 146.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 
@@ -19,7 +19,7 @@ namespace rptc {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLogprobThreads = 256, kLogprobRoom = 512, kLogprobTop = 32, kLogprobUnroll = 4, kLogprobMaxCluster = 8;
+constexpr int kLogprobRoom = 512, kLogprobTop = 32, kLogprobUnroll = 4, kLogprobMaxCluster = 8;
 
 struct LogprobParams {
     const void *logits;
@@ -145,24 +145,25 @@ struct Share {
     __device__ __forceinline__ uint32_t index(int v, int e) const { return (uint32_t)(head + v * kPer + e); }
 };
 
-constexpr int kLogprobWarps = kLogprobThreads / 32;
+template <int THREADS>
 struct LogprobShared {
-    Tally tallies[kLogprobWarps];
-    alignas(16) uint32_t sample[kLogprobWarps * 32 + 16];     // the largest of every warp's threads' largest, in the order of the numbers
+    static constexpr int kWarps = THREADS / 32;
+    Tally tallies[kWarps];
+    alignas(16) uint32_t sample[kWarps * 32 + 16];     // the largest of every warp's threads' largest, in the order of the numbers
     int found, chosen, again;
-    int at[kLogprobThreads], who[kLogprobThreads], whole[kLogprobThreads];
+    int at[THREADS], who[THREADS], whole[THREADS];
     alignas(16) uint64_t keys[kLogprobRoom + 8];
-    uint64_t best[kLogprobTop], merged[kLogprobMaxCluster * kLogprobTop], round[kLogprobWarps];
+    uint64_t best[kLogprobTop], merged[kLogprobMaxCluster * kLogprobTop], round[kWarps];
     Tally tally;
 };
 
 // The k largest of the CTA's share, in order (0 where there are fewer), in sh.best.  All threads.
-template <int DTYPE>
-__device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, float mine, float second, int chunk, int k) {
-    constexpr int kPer = Share<DTYPE>::kPer, U = kLogprobUnroll;
+template <int DTYPE, int THREADS>
+__device__ void largest_entries(LogprobShared<THREADS> &sh, const Share<DTYPE> &share, float mine, float second, int chunk, int k) {
+    constexpr int kPer = Share<DTYPE>::kPer, U = kLogprobUnroll, kWarps = THREADS / 32;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     // A bound that at least k threads' largest entries reach: the k-th of a few of every warp, a few more than its part of k, so that it is seldom lower than the k-th of all.
-    const int few = min(32, (k + kLogprobWarps - 1) / kLogprobWarps + 2), samples = few * kLogprobWarps;
+    const int few = min(32, (k + kWarps - 1) / kWarps + 2), samples = few * kWarps;
     const uint32_t own = order_of(mine);
     uint32_t left = own;
     for (int j = 0; j < few; ++j) {
@@ -215,21 +216,21 @@ __device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, fl
     // All threads look at the vectors of those that reach the bound: the few that were read together with the largest
     // entry, and all the others too where one of them reaches it as well.
     const int chosen = sh.chosen, again = sh.again;
-    for (int i = t; i < chosen * U; i += kLogprobThreads) {
-        const int v = sh.at[sh.who[i / U]] + (i % U) * kLogprobThreads;
+    for (int i = t; i < chosen * U; i += THREADS) {
+        const int v = sh.at[sh.who[i / U]] + (i % U) * THREADS;
         if (v < share.last) look(v);
     }
     if (again) {
-        const int each = (share.last - share.first + kLogprobThreads - 1) / kLogprobThreads;
-        for (int i = t; i < again * each; i += kLogprobThreads) {
-            const int q = i / each, who = sh.whole[q], v = share.first + who + (i - q * each) * kLogprobThreads, from = v - sh.at[who];
-            if (v < share.last && (from < 0 || from >= U * kLogprobThreads)) look(v);
+        const int each = (share.last - share.first + THREADS - 1) / THREADS;
+        for (int i = t; i < again * each; i += THREADS) {
+            const int q = i / each, who = sh.whole[q], v = share.first + who + (i - q * each) * THREADS, from = v - sh.at[who];
+            if (v < share.last && (from < 0 || from >= U * THREADS)) look(v);
         }
     }
     __syncthreads();
     const int found = sh.found;
     if (found <= kLogprobRoom) {
-        for (int i = t; i < found; i += kLogprobThreads) {
+        for (int i = t; i < found; i += THREADS) {
             const uint64_t key = sh.keys[i];
             int rank = 0;
             for (int j = 0; j < found; j += 8) {
@@ -249,7 +250,7 @@ __device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, fl
                 const uint64_t key = order_key(x, i);
                 if (key < last && key > best) best = key;
             };
-            for (int v = share.first + t; v < share.last; v += kLogprobThreads) {
+            for (int v = share.first + t; v < share.last; v += THREADS) {
                 float x[kPer];
                 logits_of<DTYPE>(share.vector(v), x);
 #pragma unroll
@@ -264,7 +265,7 @@ __device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, fl
             __syncthreads();
             if (lane == 0) sh.round[warp] = best;
             __syncthreads();
-            for (int i = 0; i < kLogprobThreads / 32; ++i) best = sh.round[i] > best ? sh.round[i] : best;
+            for (int i = 0; i < THREADS / 32; ++i) best = sh.round[i] > best ? sh.round[i] : best;
             last = best;
             if (t == 0) sh.best[j] = best;
         }
@@ -272,10 +273,10 @@ __device__ void largest_entries(LogprobShared &sh, const Share<DTYPE> &share, fl
     __syncthreads();
 }
 
-template <int DTYPE, bool CLUSTER>
-__global__ void __launch_bounds__(kLogprobThreads, 5) token_logprobs_kernel(const LogprobParams p) {
-    constexpr int kPer = Share<DTYPE>::kPer, U = kLogprobUnroll;
-    __shared__ LogprobShared sh;
+template <int DTYPE, bool CLUSTER, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 9) token_logprobs_kernel(const LogprobParams p) {
+    constexpr int kPer = Share<DTYPE>::kPer, U = kLogprobUnroll, kWarps = THREADS / 32;
+    __shared__ LogprobShared<THREADS> sh;
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     int rank = 0, ranks = 1;
     int64_t r = blockIdx.x;
@@ -308,12 +309,12 @@ __global__ void __launch_bounds__(kLogprobThreads, 5) token_logprobs_kernel(cons
             w = fma2(q, d, w);
         }
     };
-    for (int v0 = share.first + t; v0 < share.last; v0 += U * kLogprobThreads) {
+    for (int v0 = share.first + t; v0 < share.last; v0 += U * THREADS) {
         uint4 raw[U];
         // a vector that is not there is one of forbidden tokens
         const uint32_t none = DTYPE == 0 ? 0xFC00FC00u : DTYPE == 1 ? 0xFF80FF80u : 0xFF800000u;
 #pragma unroll
-        for (int u = 0; u < U; ++u) raw[u] = v0 + u * kLogprobThreads < share.last ? share.vector(v0 + u * kLogprobThreads) : make_uint4(none, none, none, none);
+        for (int u = 0; u < U; ++u) raw[u] = v0 + u * THREADS < share.last ? share.vector(v0 + u * THREADS) : make_uint4(none, none, none, none);
         float top = -INFINITY;
         if (DTYPE == 2) {
 #pragma unroll
@@ -367,12 +368,12 @@ __global__ void __launch_bounds__(kLogprobThreads, 5) token_logprobs_kernel(cons
     if (!(warp_top == -INFINITY)) a.move(warp_top);
     for (int o = 16; o > 0; o >>= 1) a.z += __shfl_xor_sync(0xFFFFFFFFu, a.z, o), a.w += __shfl_xor_sync(0xFFFFFFFFu, a.w, o);
     if (lane == 0) sh.tallies[warp] = a;
-    if (p.k > 0) largest_entries<DTYPE>(sh, share, mine, second, chunk, p.k);
+    if (p.k > 0) largest_entries<DTYPE, THREADS>(sh, share, mine, second, chunk, p.k);
     else __syncthreads();
     if (warp == 0) {
-        a = sh.tallies[lane % kLogprobWarps];
+        a = sh.tallies[lane % kWarps];
 #pragma unroll
-        for (int o = 1; o < kLogprobWarps; o <<= 1) {
+        for (int o = 1; o < kWarps; o <<= 1) {
             Tally b;
             b.M = __shfl_xor_sync(0xFFFFFFFFu, a.M, o), b.z = __shfl_xor_sync(0xFFFFFFFFu, a.z, o), b.w = __shfl_xor_sync(0xFFFFFFFFu, a.w, o);
             a.join(b);
@@ -382,11 +383,11 @@ __global__ void __launch_bounds__(kLogprobThreads, 5) token_logprobs_kernel(cons
     if (CLUSTER) {
         cg::this_cluster().sync();
         if (rank == 0) {                                     // the others' sums and largest entries
-            for (int i = t; i < ranks * p.k; i += kLogprobThreads) sh.merged[i] = cg::this_cluster().map_shared_rank(sh.best, i / p.k)[i % p.k];
+            for (int i = t; i < ranks * p.k; i += THREADS) sh.merged[i] = cg::this_cluster().map_shared_rank(sh.best, i / p.k)[i % p.k];
             if (t == 0)
                 for (int i = 1; i < ranks; ++i) a.join(*cg::this_cluster().map_shared_rank(&sh.tally, i)), sh.tally = a;
             __syncthreads();
-            for (int i = t; i < ranks * p.k; i += kLogprobThreads) {
+            for (int i = t; i < ranks * p.k; i += THREADS) {
                 if (sh.merged[i] == 0) continue;
                 int at = 0;
                 for (int j = 0; j < ranks * p.k; ++j) at += sh.merged[j] > sh.merged[i];
@@ -419,11 +420,12 @@ __global__ void __launch_bounds__(kLogprobThreads, 5) token_logprobs_kernel(cons
 }
 
 template <int DTYPE>
-static int launch_logprobs(const LogprobParams &p, int64_t rows, int cluster, cudaStream_t s) {
-    if (cluster == 1) return launch(token_logprobs_kernel<DTYPE, false>, dim3((unsigned)rows), dim3(kLogprobThreads), 0, s, p);
+static int launch_logprobs(const LogprobParams &p, int64_t rows, int cluster, int threads, cudaStream_t s) {
+    if (threads == 128) return launch(token_logprobs_kernel<DTYPE, false, 128>, dim3((unsigned)rows), dim3(128), 0, s, p);
+    if (cluster == 1) return launch(token_logprobs_kernel<DTYPE, false, 256>, dim3((unsigned)rows), dim3(256), 0, s, p);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * cluster));
-    cfg.blockDim = dim3(kLogprobThreads);
+    cfg.blockDim = dim3(256);
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -432,7 +434,7 @@ static int launch_logprobs(const LogprobParams &p, int64_t rows, int cluster, cu
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = pdl_enabled() ? 2 : 1;
-    RPTC_CUDA(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<DTYPE, true>, p));
+    RPTC_CUDA(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<DTYPE, true, 256>, p));
     return RPTC_OK;
 }
 
@@ -460,9 +462,14 @@ extern "C" int rptc_token_logprobs(const void *logits, int dtype, int64_t ld, co
     LogprobParams p = {logits, ld, targets, logprob, entropy, top_logprobs, top_ids, n, top, device_status_word()};
     if (!p.status) return RPTC_ERR_CUDA;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int64_t bytes = n * (dtype == 2 ? 4 : 2);
     // Few rows: up to eight CTAs share one, as long as each has 32 KiB of it (one row of 8192 in fp16: four CTAs 3.8 us, one 2.5; 32000 in fp16: 4.4 and 4.6; 128001 in
     // fp32: eight 6.8, one 15.8; 148 rows of 32000: two 5.7, one 4.9).
     int cluster = 1;
-    while (cluster < kLogprobMaxCluster && rows * cluster * 2 <= 2 * num_sms() && n * (dtype == 2 ? 4 : 2) >= cluster * 2 * 32768) cluster *= 2;
-    return dtype == 0 ? launch_logprobs<0>(p, rows, cluster, s) : dtype == 1 ? launch_logprobs<1>(p, rows, cluster, s) : launch_logprobs<2>(p, rows, cluster, s);
+    while (cluster < kLogprobMaxCluster && rows * cluster * 2 <= 2 * num_sms() && bytes >= cluster * 2 * 32768) cluster *= 2;
+    // With the largest entries, whose meetings keep a row's threads waiting, rows of fewer threads and more of them on an SM, unless a row alone has to be fast or is long
+    // (top 20, 256 and 128 threads: 8000 rows of 1000 in fp16 72 and 39 us, 2048 of 32000 43 and 39, 300 of 32000 11.9 and 11.7, 800 of 128001 57 and 55, in fp32 145 and 164 for
+    // 1500; one of 1000 5.4 and 4.8, one of 32000 7.8 and 9.1).
+    const int threads = top > 0 && (bytes <= 4096 || (rows >= 2 * (int64_t)num_sms() && bytes <= 256 * 1024)) ? 128 : 256;
+    return dtype == 0 ? launch_logprobs<0>(p, rows, cluster, threads, s) : dtype == 1 ? launch_logprobs<1>(p, rows, cluster, threads, s) : launch_logprobs<2>(p, rows, cluster, threads, s);
 }
