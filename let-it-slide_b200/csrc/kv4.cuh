@@ -18,10 +18,26 @@ inline int check_kv_cache(const rptc_kv_cache &c) {
 }
 
 #ifdef __CUDACC__
-// Eight neighbouring values of a thread, whose group of 32 is that of four neighbouring lanes -> the thread's eight codes (nibbles, first value lowest) and the
-// group's scale and minimum.  The difference and its fifteenth are rounded to 32 bits each, the scale then to fp16: what is stored is what the codes are counted in.
-// Quotients by Markstein's correction (an estimate times the reciprocal, its exact remainder by a fused multiply-add, and the remainder's quotient added): one that is
+// A group's scale, as it is stored, and its reciprocal.  The difference and its fifteenth are rounded to 32 bits each, the scale then to fp16: what is stored is what the
+// codes are counted in.
+__device__ __forceinline__ __half2 kv4_scale(float lo, float hi, float &inv) {
+    const float range = hi - lo, part = range * (1.f / 15.f);
+    const __half scale = __float2half_rn(fmaf(fmaf(-part, 15.f, range), 1.f / 15.f, part));      // the rounded fifteenth, for every significand
+    const float step = __half2float(scale);
+    inv = step > 0.f ? __frcp_rn(step) : 0.f;                                                      // scale 0: codes 0
+    return __halves2half2(scale, __float2half_rn(lo));
+}
+// A value's code, as 12582912 + code: a sum of theirs and their multiples by 16, 256 and 4096 has the codes in its low 16 bits.
+// Quotient by Markstein's correction (an estimate times the reciprocal, its exact remainder by a fused multiply-add, and the remainder's quotient added): one that is
 // half-way between two codes comes out exactly; any other differs from half-way by 2^-17 of itself at least (fp16 numbers over an fp16 number), far more than the estimate is off.
+// It passes 15.5 only where the scale was rounded by more than a thirtieth: below 2^-20 (fp16's steps there are 2^-24), kKv4Exact with room to spare.
+constexpr float kKv4Exact = 1.9073486328125e-6f;                     // 2^-19
+__device__ __forceinline__ uint32_t kv4_code(float v, float lo, float step, float inv, bool small = true) {
+    const float d = v - lo, q0 = d * inv, q = fmaf(fmaf(-q0, step, d), inv, q0);
+    return __float_as_uint((small ? fminf(q, 15.f) : q) + 12582912.f);      // 1.5 * 2^23: rounds to the nearest whole number, half to even
+}
+// Eight neighbouring values of a thread, whose group of 32 is that of four neighbouring lanes -> the thread's eight codes (nibbles, first value lowest) and the
+// group's scale and minimum.
 __device__ __forceinline__ uint32_t kv4_quantise(const float (&v)[8], __half2 &scale_min) {
     float lo = fminf(fminf(fminf(v[0], v[1]), fminf(v[2], v[3])), fminf(fminf(v[4], v[5]), fminf(v[6], v[7])));
     float hi = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
@@ -30,17 +46,12 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&v)[8], __half2 &s
         lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
     }
-    const float range = hi - lo, part = range * (1.f / 15.f);
-    const __half scale = __float2half_rn(fmaf(fmaf(-part, 15.f, range), 1.f / 15.f, part));      // the rounded fifteenth, for every significand
-    scale_min = __halves2half2(scale, __float2half_rn(lo));
-    const float step = __half2float(scale), inv = step > 0.f ? __frcp_rn(step) : 0.f;      // scale 0: codes 0
+    float inv;
+    scale_min = kv4_scale(lo, hi, inv);
+    const float step = __half2float(__low2half(scale_min));
     uint32_t codes = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float d = v[i] - lo, q0 = d * inv, q = fmaf(fmaf(-q0, step, d), inv, q0);
-        const uint32_t c = __float_as_uint(fminf(q, 15.f) + 12582912.f) & 15u;             // 1.5 * 2^23: rounds to the nearest whole number, half to even
-        codes |= c << (4 * i);
-    }
+    for (int i = 0; i < 8; ++i) codes |= (kv4_code(v[i], lo, step, inv) & 15u) << (4 * i);
     return codes;
 }
 #endif

@@ -3,8 +3,10 @@
 //
 //   y = rope(scale signs H x) per head of 128;   a group of 32 values of k or v: scale = (max - min) / 15, code = round((value - min) / scale)
 //
-// Bound: HBM by bytes, the issue slots in fact (shuffles of the transform and the groups' extremes, two heads of a warp at a time): 2048 tokens of 96 heads 38 us where the
-// traffic is 17; 16 tokens 2.5 us, a launch.  The values of a cache: 8.1 us for 2048 positions of 32 kv heads, its traffic 6.7.
+// Bound: HBM by bytes; in fact the issue slots and the SM's load and store pipe, each some 60 % busy: 2048 tokens of 96 heads 30 us where the traffic is 17; 16 tokens
+// 2.5 us, a launch.  The values of a cache: 8.1 us for 2048 positions of 32 kv heads, its traffic 6.7.
+#include <type_traits>
+
 #include "fwht.cuh"
 #include "kv4.cuh"
 
@@ -22,7 +24,8 @@ struct AppendParams {
     __half2 *k_scales, *v_scales;
     int64_t rows, max_pos;
     int32_t hq, hkv, clear, out_kv;
-    int32_t chunk, chunks_q, chunks_kv, chunks;      // heads of a warp (even); warps of a token: for q, for k (and v), all
+    int32_t chunk, chunks_q, chunks_kv, chunks;      // heads of a warp (even, or eight); warps of a token: for q, for k (and v), all
+    int32_t step_tokens, step_parts;
     float scale;                     // includes 1 / sqrt(128) with the transform
     unsigned int *status;
 };
@@ -162,6 +165,203 @@ __global__ void __launch_bounds__(256) qkv_append_kernel(const AppendParams p) {
     }
 }
 
+// Many tokens of an fp16 x: the transform on the tensor core.  A warp takes eight heads of q, k or v of a token at a time.  With the dims' bits split as J = (0, 1, 2),
+// i = (3, 4, 5, 6), H128 = H8(J) x H16(i): for each of the eight J one product H16 X_J (m16n8k16, column = head, the signs exact and the sums in fp32), and H8 as
+// additions in a lane, which has the same rows of all eight.  What a lane then holds of its two heads, 2 t and 2 t + 1, are the dims 8 g .. 8 g + 7 and those 64 on: the
+// rotation's partner is its own, and a group of 32 is four lanes', of which each ends up with one (head, half) of the four that they share, works out
+// its scale and hands it out.
+template <int BITS>
+__global__ void __launch_bounds__(256, 2) qkv_append_heads_kernel(const AppendParams p) {
+    pdl_allow_next_grid();
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    // Pieces of work are eight heads of a token; `step` pieces on, so many tokens and parts on (every warp gets q, k and v in turn: they take unequal times).
+    const int64_t piece = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    int64_t token = piece / p.chunks;
+    int part = (int)(piece - token * p.chunks);
+    if (piece >= (int64_t)p.step_tokens * p.chunks + p.step_parts) return;
+    uint32_t a[4];                                           // H16: rows g and g + 8, columns i = t, t + 4 (a0, a1), t + 8, t + 12
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int r = g + 8 * (e & 1), i = t + 8 * (e >> 1);
+        a[e] = (__popc(r & i) & 1 ? 0xBC00u : 0x3C00u) | (__popc(r & (i + 4)) & 1 ? 0xBC000000u : 0x3C000000u);
+    }
+    pdl_wait_prior_grids();
+    const int32_t *pos_p = after_wait(p.pos), *slot_p = after_wait(p.slots);
+    const __half *x = static_cast<const __half *>(after_wait(p.x)) + 8 * t;
+    struct Heads {
+        int first, count, base;                              // of q, k or v: the first of eight, how many there are, where they lie in a row
+        bool q, v;
+    };
+    auto heads_of = [&](int part) {
+        Heads h;
+        h.q = part < p.chunks_q, h.v = part >= p.chunks_q + p.chunks_kv;
+        h.first = (part - (h.q ? 0 : h.v ? p.chunks_q + p.chunks_kv : p.chunks_q)) * 8;
+        h.count = h.q ? p.hq : p.hkv, h.base = h.q ? 0 : h.v ? p.hq + p.hkv : p.hq;
+        return h;
+    };
+    uint4 raw[4];                                            // dims 8 t .. 8 t + 7, and those 32, 64 and 96 on, of head g: all J of i = t, t + 4, ..
+    int next_pos = 0;
+    int64_t next_slot = 0;
+    Heads next = heads_of(part);
+    auto fetch = [&]() {
+        const uint4 *src = reinterpret_cast<const uint4 *>(x + token * p.ld_x + (next.base + min(next.first + g, next.count - 1)) * 128);
+        raw[0] = src[0], raw[1] = src[4], raw[2] = src[8], raw[3] = src[12];
+        next_pos = __ldg(pos_p + token), next_slot = slot_p ? __ldg(slot_p + token) : token;
+    };
+    if (token < p.tokens) fetch();
+    while (token < p.tokens) {
+        const Heads mine = next;
+        const int pos = next_pos, heads = mine.count, base = mine.base, first = mine.first;
+        const int64_t slot = next_slot, here = token;
+        const bool is_q = mine.q, is_v = mine.v;
+        const bool takes = pos >= 0 && pos < p.max_pos && slot >= 0 && slot < p.rows;      // the same in all lanes
+        f32x2 cs[4], sn[4];                                  // of the dims 8 g + 2 w and the next
+        if (takes && !is_v) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const float4 v = __ldg(reinterpret_cast<const float4 *>(p.angles + (int64_t)pos * 64 + 8 * g + 2 * w));
+                cs[w] = pack2(v.x, v.z), sn[w] = pack2(v.y, v.w);
+            }
+        }
+        uint4 signs[2][2];                                   // of head 2 t + c, half
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int half = 0; half < 2; ++half)
+                signs[c][half] = p.signs ? __ldg(reinterpret_cast<const uint4 *>(p.signs + (base + min(first + 2 * t + c, heads - 1)) * 128 + 64 * half + 8 * g)) : make_uint4(0u, 0u, 0u, 0u);
+        f32x2 y[8][2];                                       // [J][half]: heads 2 t and 2 t + 1
+#pragma unroll
+        for (int J = 0; J < 8; ++J) {
+            const uint32_t sel = (J & 1) ? 0x7632u : 0x5410u;
+            uint32_t x[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) x[q] = J < 2 ? raw[q].x : J < 4 ? raw[q].y : J < 6 ? raw[q].z : raw[q].w;
+            float d[4];
+            mma_first(d, a[0], a[1], a[2], a[3], __byte_perm(x[0], x[1], sel), __byte_perm(x[2], x[3], sel));
+            y[J][0] = pack2(d[0], d[1]), y[J][1] = pack2(d[2], d[3]);
+        }
+        part += p.step_parts, token += p.step_tokens;
+        if (part >= p.chunks) part -= p.chunks, ++token;
+        if (token < p.tokens) {
+            next = heads_of(part);
+            fetch();
+        }
+        if (!takes) {
+            if (pos != -1 && lane == 0) atomicExch(p.status, kStatusPosition);
+            continue;
+        }
+#pragma unroll
+        for (int h = 1; h < 8; h <<= 1)
+#pragma unroll
+            for (int J = 0; J < 8; ++J)
+                if (!(J & h))
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const f32x2 u = y[J][half], v = y[J + h][half];
+                        y[J][half] = add2(u, v), y[J + h][half] = sub2(u, v);
+                    }
+        uint32_t o[2][2][4];                                 // [head][half][w]: fp16, dims 64 half + 8 g + 2 w and the next
+        const f32x2 scale2 = pack2(p.scale, p.scale);
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                float u0, u1, v0, v1;
+                unpack2(mul2(y[2 * w][half], scale2), u0, u1);
+                unpack2(mul2(y[2 * w + 1][half], scale2), v0, v1);
+                const uint4 s0 = signs[0][half], s1 = signs[1][half];
+                o[0][half][w] = half2_as_u32(__floats2half2_rn(u0, v0)) ^ ((w == 0 ? s0.x : w == 1 ? s0.y : w == 2 ? s0.z : s0.w) & 0x80008000u);
+                o[1][half][w] = half2_as_u32(__floats2half2_rn(u1, v1)) ^ ((w == 0 ? s1.x : w == 1 ? s1.y : w == 2 ? s1.z : s1.w) & 0x80008000u);
+            }
+        if (!is_v) {
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float2 f = __half22float2(u32_as_half2(o[c][0][w])), s = __half22float2(u32_as_half2(o[c][1][w]));
+                    const f32x2 u = pack2(f.x, f.y), v = pack2(s.x, s.y);
+                    float m0, m1;
+                    unpack2(sub2(mul2(u, cs[w]), mul2(v, sn[w])), m0, m1);
+                    o[c][0][w] = half2_as_u32(__floats2half2_rn(m0, m1));
+                    unpack2(add2(mul2(v, cs[w]), mul2(u, sn[w])), m0, m1);
+                    o[c][1][w] = half2_as_u32(__floats2half2_rn(m0, m1));
+                }
+        }
+        const bool there[2] = {first + 2 * t < heads, first + 2 * t + 1 < heads};
+        if (is_q || p.out_kv) {
+            __half *dst = p.out + here * p.ld_out + (base + first + 2 * t) * 128 + 8 * g;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                if (there[c]) {
+                    *reinterpret_cast<uint4 *>(dst + 128 * c) = make_uint4(o[c][0][0], o[c][0][1], o[c][0][2], o[c][0][3]);
+                    *reinterpret_cast<uint4 *>(dst + 128 * c + 64) = make_uint4(o[c][1][0], o[c][1][1], o[c][1][2], o[c][1][3]);
+                }
+        }
+        if (is_q) continue;
+        if (BITS == 16) {
+            uint8_t *dst = (is_v ? p.v : p.k) + ((slot * p.max_pos + pos) * p.hkv + first + 2 * t) * 256 + 16 * g;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+                if (there[c]) {
+                    *reinterpret_cast<uint4 *>(dst + 256 * c) = make_uint4(o[c][0][0], o[c][0][1], o[c][0][2], o[c][0][3]);
+                    *reinterpret_cast<uint4 *>(dst + 256 * c + 128) = make_uint4(o[c][1][0], o[c][1][1], o[c][1][2], o[c][1][3]);
+                }
+            continue;
+        }
+        // (largest, minus the smallest) of the lane's eight values of a (head, half), then of the four lanes': they halve what they look at twice
+        uint32_t m[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t(&v)[4] = o[e >> 1][e & 1];
+            const uint32_t most = half2_as_u32(__hmax2(__hmax2(u32_as_half2(v[0]), u32_as_half2(v[1])), __hmax2(u32_as_half2(v[2]), u32_as_half2(v[3]))));
+            const uint32_t least = half2_as_u32(__hmin2(__hmin2(u32_as_half2(v[0]), u32_as_half2(v[1])), __hmin2(u32_as_half2(v[2]), u32_as_half2(v[3])))) ^ 0x80008000u;
+            m[e] = half2_as_u32(__hmax2(u32_as_half2(__byte_perm(most, least, 0x5410)), u32_as_half2(__byte_perm(most, least, 0x7632))));
+        }
+#pragma unroll
+        for (int h = 2; h > 0; h >>= 1) {
+            const bool up = g & h;
+#pragma unroll
+            for (int e = 0; e < h; ++e) {
+                const uint32_t keep = up ? m[e + h] : m[e], give = up ? m[e] : m[e + h];
+                m[e] = half2_as_u32(__hmax2(u32_as_half2(keep), u32_as_half2(__shfl_xor_sync(0xFFFFFFFFu, give, 4 * h))));
+            }
+        }
+        const float2 ends = __half22float2(u32_as_half2(m[0]));      // of head 2 t + (g & 3) / 2, group 2 (g & 1) + g / 4
+        float inv;
+        const uint32_t scale_min = half2_as_u32(kv4_scale(-ends.y, ends.x, inv));
+        const int64_t at = (slot * p.hkv + first + 2 * t) * p.max_pos + pos;
+        if (first + 2 * t + ((g >> 1) & 1) < heads)
+            reinterpret_cast<uint32_t *>(is_v ? p.v_scales : p.k_scales)[(at + ((g >> 1) & 1) * p.max_pos) * 4 + 2 * (g & 1) + (g >> 2)] = scale_min;
+        auto codes = [&](auto small) {
+            constexpr bool kSmall = decltype(small)::value;
+            uint8_t *dst = (is_v ? p.v : p.k) + at * kKv4Codes + 8 * (2 * (g & 3) + (g >> 2));
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t n[2][2];                            // [half]: dims 8 g .. 8 g + 3, the next four
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int from = ((g & 4) | (2 * c + half)) * 4 + t;
+                    const float2 sm = __half22float2(u32_as_half2(__shfl_sync(0xFFFFFFFFu, scale_min, from)));
+                    const float by = __shfl_sync(0xFFFFFFFFu, inv, from);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float2 u = __half22float2(u32_as_half2(o[c][half][2 * e])), v = __half22float2(u32_as_half2(o[c][half][2 * e + 1]));
+                        n[half][e] = kv4_code(u.x, sm.y, sm.x, by, kSmall) + 16u * kv4_code(u.y, sm.y, sm.x, by, kSmall) + 256u * kv4_code(v.x, sm.y, sm.x, by, kSmall) +
+                                     4096u * kv4_code(v.y, sm.y, sm.x, by, kSmall);
+                    }
+                }
+                // four dims of all four groups: those of groups 0 and 2 are in one lane, of 1 and 3 in the lane 16 on
+                const uint32_t w0 = __byte_perm(n[0][0], n[1][0], 0x5410), w1 = __byte_perm(n[0][1], n[1][1], 0x5410);
+                const uint32_t keep = g < 4 ? w0 : w1, got = __shfl_xor_sync(0xFFFFFFFFu, g < 4 ? w1 : w0, 16), even = g < 4 ? keep : got, odd = g < 4 ? got : keep;
+                if (there[c]) *reinterpret_cast<uint2 *>(dst + c * p.max_pos * kKv4Codes) = make_uint2(__byte_perm(even, odd, 0x5410), __byte_perm(even, odd, 0x7632));
+            }
+        };
+        const float step = __low2float(u32_as_half2(scale_min));
+        if (__any_sync(0xFFFFFFFFu, step > 0.f && step < kKv4Exact)) codes(std::true_type());
+        else codes(std::false_type());
+    }
+}
+
 template <bool F32, bool TRANSFORM>
 static int launch_append(const AppendParams &p, int bits, cudaStream_t s) {
     const dim3 grid((unsigned)p.tokens, (unsigned)((p.chunks + 7) / 8));
@@ -243,6 +443,31 @@ extern "C" int rptc_qkv_append(const rptc_append *a, rptc_stream_t stream) {
     p.status = device_status_word();
     if (!p.status) return RPTC_ERR_CUDA;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // Eight heads at a time where there is work for all SMs and the eights are at least half full (heads of q and of k, fp16; two heads a warp and eight): 2048 tokens of (32, 32)
+    // 38 and 30 us, of (64, 8) 29 and 21, of (16, 2) 12.2 and 10.4, of (8, 1) 9.0 and 9.2; 64 of (32, 32) 3.7 and 3.8, of (16, 2) 2.8 and 3.9.
+    const int64_t heads = p.hq + 2 * (int64_t)p.hkv, eights = (p.hq + 7) / 8 + 2 * (int64_t)((p.hkv + 7) / 8);
+    if (!a->x_is_f32 && a->transform && p.tokens * heads >= 64 * 96 && 4 * eights <= heads) {
+        p.chunk = 8;
+        p.chunks_q = (p.hq + 7) / 8, p.chunks_kv = (p.hkv + 7) / 8, p.chunks = (int)eights;
+        const int64_t pieces = p.tokens * p.chunks, warps = 16 * (int64_t)num_sms();
+        int64_t ctas = (pieces + 7) / 8, step = 8 * ctas;
+        if (pieces > warps) {                                // a step past the q heads and without a common divisor with the parts
+            ctas = warps / 8;
+            int on = p.chunks_q + 1;
+            auto divisor = [](int a, int b) {
+                while (b) {
+                    const int r = a % b;
+                    a = b, b = r;
+                }
+                return a;
+            };
+            while (divisor(on, p.chunks) != 1) ++on;
+            step = (warps - on) / p.chunks * p.chunks + on;
+        }
+        p.step_tokens = (int32_t)(step / p.chunks), p.step_parts = (int32_t)(step % p.chunks);
+        return c.bits == 4 ? launch(qkv_append_heads_kernel<4>, dim3((unsigned)ctas), dim3(256), 0, s, p)
+                           : launch(qkv_append_heads_kernel<16>, dim3((unsigned)ctas), dim3(256), 0, s, p);
+    }
     if (a->x_is_f32) return a->transform ? launch_append<true, true>(p, c.bits, s) : launch_append<true, false>(p, c.bits, s);
     return a->transform ? launch_append<false, true>(p, c.bits, s) : launch_append<false, false>(p, c.bits, s);
 }

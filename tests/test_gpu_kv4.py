@@ -121,6 +121,49 @@ def test_append(bits, dtype, transform, hq, hkv):
     ops.device_status()
 
 
+@pytest.mark.parametrize("bits", [4, 16])
+@pytest.mark.parametrize("hq,hkv,tokens", [(32, 32, 70), (12, 4, 401), (64, 8, 300), (16, 2, 1000), (5, 5, 3000), (40, 20, 77)])
+def test_append_of_many_tokens(bits, hq, hkv, tokens):
+    """Enough tokens of fp16 for the transform on the tensor core, whose sums of sixteen take the place of four of the seven stages: each is within 4 * 2^-24 of its
+    sum |x|.  Eights that are full, and not; values of all sizes; tokens of no sequence; in place, and q alone."""
+    from rptc_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    rows, max_pos, width = 7, tokens // 5, (hq + 2 * hkv) * 128
+    size = torch.tensor([3.0, 0.01, 2e-6, 100.0, 0.0, 1e-4, 0.5], device="cuda")[torch.arange(tokens, device="cuda") % 7]
+    x = torch.zeros(tokens, width + 8, dtype=torch.float16, device="cuda")[:, :width].copy_(size[:, None] * torch.randn(tokens, width, generator=g, device="cuda"))
+    signs = (torch.randint(0, 2, (width,), generator=g, device="cuda") * 2 - 1).half()
+    spot = torch.randperm(rows * max_pos, generator=g, device="cuda")[:tokens]
+    slots, pos = (spot // max_pos).int(), (spot % max_pos).int()
+    idle = torch.arange(tokens, device="cuda") % 11 == 3
+    pos[idle] = -1
+    angles = angles_of(max_pos)
+    new = lambda: ops.kv4_cache(rows, max_pos, hkv) if bits == 4 else tuple(torch.zeros(rows, max_pos, hkv, 128, dtype=torch.float16, device="cuda") for _ in range(2))
+    cache, again = new(), new()
+    out = torch.full((tokens, width), 7.0, dtype=torch.float16, device="cuda")
+    assert ops.qkv_append(x, pos, angles, cache, hq, hkv, slots=slots, signs_out=signs, scale=0.25, transform=True, out=out) is out
+    assert (out[idle] == 7).all()
+    want, tol = finished(x, signs, 0.25, True, angles, pos.clamp(min=0), hq, hkv)
+    got = out.unflatten(1, (-1, 128))
+    assert ((got.double() - want).abs() <= tol)[~idle].all(), ((got.double() - want).abs() / tol)[~idle].max()
+    k, v, at = got[~idle, hq:hq + hkv], got[~idle, hq + hkv:], (slots[~idle].long(), pos[~idle].long())
+    seen = torch.zeros(rows, max_pos, dtype=torch.bool, device="cuda")
+    seen[at] = True
+    if bits == 16:
+        assert torch.equal(cache[0][at], k) and torch.equal(cache[1][at], v) and not cache[0][~seen].any() and not cache[1][~seen].any()
+    else:
+        for i, t in ((0, k), (2, v)):
+            n, s = quantised(t)
+            assert torch.equal(codes_of(cache[i])[at[0], :, at[1]], n) and torch.equal(cache[i + 1][at[0], :, at[1]], s)
+            assert not cache[i].transpose(1, 2)[~seen].any() and not cache[i + 1].transpose(1, 2)[~seen].any()
+    q = torch.full((tokens, hq * 128), 7.0, dtype=torch.float16, device="cuda")
+    ops.qkv_append(x, pos, angles, again, hq, hkv, slots=slots, signs_out=signs, scale=0.25, transform=True, out=q)
+    assert torch.equal(q, out[:, :hq * 128]) and all(torch.equal(a, b) for a, b in zip(cache, again))
+    held = x.clone()
+    ops.qkv_append(x, pos, angles, again, hq, hkv, slots=slots, signs_out=signs, scale=0.25, transform=True, out=x)
+    assert torch.equal(x[~idle], out[~idle]) and torch.equal(x[idle], held[idle]) and all(torch.equal(a, b) for a, b in zip(cache, again))
+    ops.device_status()
+
+
 def test_append_q_alone_in_place_and_cleared():
     from rptc_b200 import ops
     g = torch.Generator(device="cuda").manual_seed(2)
