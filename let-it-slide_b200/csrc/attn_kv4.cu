@@ -15,8 +15,8 @@
 // Weights refer to a running maximum of s + log2(a tile's largest scale): the products p * scale then fit fp16 whatever the scales are (2^11 where the reference was set, and
 // it moves only when they may pass 2^15, which their sum shows: no maximum is looked for otherwise; what falls below 2^-14 is 2^-25 of the largest).
 // Bound: HBM (160 bytes per position and kv head) with the issue slots close behind, about 350 warp instructions per 16 positions: four rows in flight per scheduler at 128
-// registers leave a quarter of the slots empty.  32 rows of 500 to 32768 positions, 8 kv heads: 142 us, 4.8 TB/s; one row of 131072: 45 us, 3.7 TB/s; one of 200: 4.6 us.
-// Long contexts: all tiles of all rows and heads, laid end to end, are cut into equal ranges for the CTAs of one wave, so that rows of different lengths balance; a range's
+// registers leave a quarter of the slots empty.  32 rows of 500 to 32768 positions, 8 kv heads: 136 us, 5.0 TB/s; one row of 131072: 43.7 us, 3.8 TB/s; one of 200: 4.6 us.
+// Long contexts: all tiles of all rows and heads, laid end to end, are cut into equal ranges, two to an SM, so that rows of different lengths balance; a range's
 // part of a row goes to the workspace (fp32) and a second kernel joins the parts.  A warp's ring goes on into the range's next item: its first tiles and its q are on their
 // way while the item before is finished (32 rows as above 160 us without, and with a join that looked at every row's heads instead of the ranges' ends).
 // Short caches take one CTA per row and head and no second kernel (the rule is at kv4_whole).
@@ -27,7 +27,7 @@
 
 namespace rptc {
 
-constexpr int kKv4Warps = 8, kKv4Tile = 32, kKv4Stages = 2, kKv4CtasPerSm = 2;
+constexpr int kKv4Warps = 8, kKv4Tile = 32, kKv4Stages = 2;
 constexpr uint32_t kKv4StageBytes = 2 * kKv4Tile * (kKv4Codes + kKv4Scales);
 constexpr uint32_t kKv4Ring = kKv4Warps * kKv4Stages * kKv4StageBytes, kKv4Merge = kKv4Warps * 8 * 128 * 4, kKv4Smem = kKv4Ring + kKv4Merge + kKv4Warps * 8 * 8;
 static_assert(kKv4Stages == 2, "a stage is the other one's next");
@@ -56,23 +56,32 @@ __device__ __forceinline__ int kv4_context(const AttnKv4Params &p, const int32_t
 __device__ __forceinline__ int kv4_tiles(int context) { return (context + kKv4Tile - 1) / kKv4Tile; }
 
 // How the work is cut: every row's heads laid end to end, each worth its tiles and kKv4Start for what a CTA does around them (q, the warps' sums).  32 rows of 500 to 32768
-// take 143 us with 16 of those, 141.7 with 24, 143.5 with 32 and 147 with 48; kKv4Least is what a CTA is worth starting for.  In numbers of 32 bits: a unit stands for a tile of
+// take 139.4 us with 16 of those, 135.5 with 20, 135.8 with 24 and 136.7 with 32; kKv4Least is what a CTA is worth starting for.  In numbers of 32 bits: a unit stands for a tile of
 // 5 KiB of the cache.
 constexpr uint32_t kKv4Start = 24, kKv4Least = 16;
 __device__ __forceinline__ uint32_t kv4_cost(int tiles) { return tiles ? (uint32_t)tiles + kKv4Start : 0u; }
+// A CTA has two ranges, one for each eight of its warps, which share nothing.  (Two CTAs of eight warps on an SM: the one that came first is served first and ends long before
+// the other, which is then alone: 48 and 61 thousand clocks over 131072 positions, 58 and 58 so; 32 rows as above 142 us, 136 so.)
 struct Kv4Cut {
-    uint32_t ctas, per, extra;
-    __device__ __forceinline__ uint32_t begin(uint32_t cta) const { return cta * per + min(cta, extra); }
-    __device__ __forceinline__ uint32_t cta_of(uint32_t at) const {       // the range that a unit is in
-        return at < extra * (per + 1) ? at / (per + 1) : extra + (at - extra * (per + 1)) / per;
+    uint32_t ctas, per, extra, halves;                    // halves: 1, or 0 where all of a CTA's units are its first range's
+    __device__ __forceinline__ uint32_t first(uint32_t cta) const { return (per + (cta < extra ? 1u : 0u)) >> halves; }
+    __device__ __forceinline__ uint32_t begin(uint32_t range) const {
+        const uint32_t cta = range >> 1;
+        return cta * per + min(cta, extra) + ((range & 1) ? first(cta) : 0u);
+    }
+    __device__ __forceinline__ uint32_t range_of(uint32_t at) const {     // the range that a unit is in
+        const uint32_t cta = at < extra * (per + 1) ? at / (per + 1) : extra + (at - extra * (per + 1)) / per;
+        return 2 * cta + (at - begin(2 * cta) >= first(cta) ? 1u : 0u);
     }
 };
 __device__ __forceinline__ Kv4Cut kv4_cut(const AttnKv4Params &p, const int32_t *pos, uint32_t most_ctas, int lane) {
     uint32_t sum = 0;
     for (int r0 = 0; r0 < p.rows; r0 += 32) sum += __reduce_add_sync(0xFFFFFFFFu, r0 + lane < p.rows ? kv4_cost(kv4_tiles(kv4_context(p, pos, r0 + lane))) : 0u);
     sum *= (uint32_t)(p.hkv * p.blocks);
+    const uint32_t worth = max(sum / kKv4Least, 1u);
     Kv4Cut c;
-    c.ctas = min(most_ctas, max(sum / kKv4Least, 1u));
+    c.ctas = min(most_ctas, worth);
+    c.halves = worth < 2 * most_ctas ? 0u : 1u;              // few: a range to an SM
     c.per = sum / c.ctas, c.extra = sum - c.per * c.ctas;
     return c;
 }
@@ -179,9 +188,12 @@ __device__ __forceinline__ void kv4_store(const AttnKv4Params &p, int row, int h
 }
 
 template <bool WHOLE>
-__global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel(const AttnKv4Params p) {
-    extern __shared__ __align__(128) unsigned char smem[];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+__global__ void __launch_bounds__(32 * kKv4Warps * (WHOLE ? 1 : 2), WHOLE ? 2 : 1) attn_kv4_kernel(const AttnKv4Params p) {
+    extern __shared__ __align__(128) unsigned char all_smem[];
+    const int tid = threadIdx.x, lane = tid & 31, eight = WHOLE ? 0 : tid >> 8, warp = (tid >> 5) & 7, g = lane >> 2, t = lane & 3;
+    unsigned char *smem = all_smem + eight * kKv4Smem;
+    auto meet = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + eight), "n"(32 * kKv4Warps) : "memory"); };      // the eight warps
+    const uint32_t range = 2 * blockIdx.x + eight;
     const uint32_t ring = smem_addr(smem) + (uint32_t)warp * kKv4Stages * kKv4StageBytes;
     float *merge = reinterpret_cast<float *>(smem + kKv4Ring);
     float2 *merge_ml = reinterpret_cast<float2 *>(smem + kKv4Ring + kKv4Merge);
@@ -200,8 +212,8 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
     } else {
         const Kv4Cut cut = kv4_cut(p, pos, gridDim.x, lane);
         if (blockIdx.x >= cut.ctas) return;
-        const uint32_t at = cut.begin(blockIdx.x);
-        units = cut.begin(blockIdx.x + 1) - at;
+        const uint32_t at = cut.begin(range);
+        units = cut.begin(range + 1) - at;
         if (units == 0) return;
         const Kv4Place f = kv4_place(p, pos, at, lane);
         row = f.row, head = f.head, context = f.context;
@@ -450,7 +462,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             for (int j = 0; j < 4; ++j) raw[j] = there ? lds128_at<0>(q_lane(j)) : make_uint4(0u, 0u, 0u, 0u);
         }
         const int kvh = head / p.blocks, first = (head - kvh * p.blocks) * 8, in_block = min(8, p.group - first), q_head = kvh * p.group + first;
-        __syncthreads();                             // the last item's sums have been taken
+        meet();                                      // the last item's sums have been taken
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             float *dst = merge + (warp * 8 + 2 * t + c) * 128 + 4 * g;
@@ -462,7 +474,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
             }
             if (g == 0) merge_ml[warp * 8 + 2 * t + c] = make_float2(m[c], l[c]);
         }
-        __syncthreads();
+        meet();
         if (warp < in_block) {                       // a warp per q head
             float2 ml[kKv4Warps];
             float mx = -INFINITY, den = 0.f, sum[4] = {0.f, 0.f, 0.f, 0.f};
@@ -480,7 +492,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps, kKv4CtasPerSm) attn_kv4_kernel
                 for (int i = 0; i < 4; ++i) sum[i] = context ? sum[i] / den : 0.f;
                 kv4_store(p, row, q_head + warp, lane, sum);
             } else {
-                const uint32_t slot = (2 * blockIdx.x + (t0 == 0 ? 1 : 0)) * 8 + warp;
+                const uint32_t slot = (2 * range + (t0 == 0 ? 1 : 0)) * 8 + warp;
                 p.part[slot * 32 + lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
                 if (lane == 0) p.part_ml[slot] = make_float2(mx, den);
             }
@@ -510,13 +522,13 @@ __global__ void __launch_bounds__(32 * kKv4JoinWarps) attn_kv4_join_kernel(const
         uint32_t before = 0;
         for (int r0 = 0; r0 < row; r0 += 32) before += __reduce_add_sync(0xFFFFFFFFu, r0 + lane < row ? kv4_cost(kv4_tiles(kv4_context(p, pos, r0 + lane))) : 0u);
         first_tile = before * (uint32_t)heads + (uint32_t)head * kv4_cost(tiles) + kKv4Start;
-    } else if (blockIdx.x + 1 < cut.ctas) {
+    } else if (blockIdx.x + 1 < 2 * cut.ctas) {
         const uint32_t at = cut.begin(blockIdx.x + 1);
         const Kv4Place f = kv4_place(p, pos, at, lane);
         if (f.off > kKv4Start) row = f.row, head = f.head, tiles = kv4_tiles(f.context), first_tile = at - f.off + kKv4Start;      // else it ends in front of a first tile
     }
     int c0 = 0, c1 = 0;
-    if (tiles) c0 = (int)cut.cta_of(first_tile), c1 = (int)cut.cta_of(first_tile + tiles - 1);
+    if (tiles) c0 = (int)cut.range_of(first_tile), c1 = (int)cut.range_of(first_tile + tiles - 1);
     const int kvh = head / p.blocks, in_group = (head - kvh * p.blocks) * 8 + blockIdx.y, q_head = kvh * p.group + in_group;
     pdl_wait_prior_grids();
     pdl_allow_next_grid();
@@ -527,6 +539,7 @@ __global__ void __launch_bounds__(32 * kKv4JoinWarps) attn_kv4_join_kernel(const
         for (int h = blockIdx.y * kKv4JoinWarps + warp; h < p.hkv * p.group; h += gridDim.y * kKv4JoinWarps) kv4_store(p, r, h, lane, zero);
     }
     if (c0 == c1 || (!by_item && c0 != (int)blockIdx.x) || in_group >= p.group) return;      // one range had it all; another CTA has it
+    const int every = cut.halves ? 1 : 2, parts = (c1 - c0) / every + 1;      // every other range is empty
     const float4 *part = after_wait(p.part);
     const float2 *part_ml = after_wait(p.part_ml);
     float mx = -INFINITY, den = 0.f;
@@ -538,8 +551,8 @@ __global__ void __launch_bounds__(32 * kKv4JoinWarps) attn_kv4_join_kernel(const
         sum.x = fmaf(x.x, g, sum.x * f), sum.y = fmaf(x.y, g, sum.y * f), sum.z = fmaf(x.z, g, sum.z * f), sum.w = fmaf(x.w, g, sum.w * f);
     };
 #pragma unroll 4
-    for (int c = c0 + warp; c <= c1; c += kKv4JoinWarps) {
-        const int slot = (2 * c + (c == c0 ? 1 : 0)) * 8 + (in_group & 7);
+    for (int k = warp; k < parts; k += kKv4JoinWarps) {
+        const int slot = (2 * (c0 + k * every) + (k == 0 ? 1 : 0)) * 8 + (in_group & 7);
         add(__ldcg(part_ml + slot), __ldcg(part + slot * 32 + lane));
     }
     sums[warp][lane] = sum;
@@ -548,7 +561,7 @@ __global__ void __launch_bounds__(32 * kKv4JoinWarps) attn_kv4_join_kernel(const
     if (warp) return;
 #pragma unroll
     for (int w = 1; w < kKv4JoinWarps; ++w)
-        if (c0 + w <= c1) add(ml[w], sums[w][lane]);
+        if (w < parts) add(ml[w], sums[w][lane]);
     float out[4] = {sum.x / den, sum.y / den, sum.z / den, sum.w / den};
     kv4_store(p, row, q_head, lane, out);
 }
@@ -566,7 +579,7 @@ static bool kv4_whole(const rptc_kv_cache &c, int heads) {
 
 extern "C" int64_t rptc_attn_decode_kv4_workspace_bytes(const rptc_kv_cache *cache, int heads) {
     if (!cache || check_kv_cache(*cache) || cache->bits != 4 || heads <= 0 || kv4_whole(*cache, heads)) return 0;
-    return (int64_t)num_sms() * kKv4CtasPerSm * 2 * 8 * (128 * 4 + 8);
+    return (int64_t)num_sms() * 2 * 2 * 8 * (128 * 4 + 8);
 }
 
 extern "C" int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *pos, const rptc_kv_cache *cache, void *out, int64_t ld_out, int heads,
@@ -603,18 +616,18 @@ extern "C" int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *
         if (int e = allow_max_smem(attn_kv4_kernel<true>, opted)) return e;
         return launch(attn_kv4_kernel<true>, dim3((unsigned)(p.hkv * p.blocks), (unsigned)p.rows), dim3(32 * kKv4Warps), kKv4Smem, s, p);
     }
-    const int64_t ctas = (int64_t)num_sms() * kKv4CtasPerSm;
+    const int64_t ctas = num_sms(), ranges = 2 * ctas;
     p.part = static_cast<float4 *>(workspace);
-    p.part_ml = reinterpret_cast<float2 *>(p.part + ctas * 2 * 8 * 32);
+    p.part_ml = reinterpret_cast<float2 *>(p.part + ranges * 2 * 8 * 32);
     static SmemOptIn opted;
     if (int e = allow_max_smem(attn_kv4_kernel<false>, opted)) return e;
-    if (int e = launch(attn_kv4_kernel<false>, dim3((unsigned)ctas), dim3(32 * kKv4Warps), kKv4Smem, s, p)) return e;
+    if (int e = launch(attn_kv4_kernel<false>, dim3((unsigned)ctas), dim3(2 * 32 * kKv4Warps), 2 * kKv4Smem, s, p)) return e;
     // the second kernel starts early and waits for the first one's sums itself
     const bool before = pdl_enabled();
     rptc_set_pdl(1);
     const int64_t items = (int64_t)p.rows * p.hkv * p.blocks;
-    const int e = launch(attn_kv4_join_kernel, dim3((unsigned)(items < ctas ? items : ctas), (unsigned)(p.group < 8 ? p.group : 8)), dim3(32 * kKv4JoinWarps), 0, s, p,
-                         (uint32_t)ctas, items < ctas ? 1 : 0);
+    const int e = launch(attn_kv4_join_kernel, dim3((unsigned)(items < ranges ? items : ranges), (unsigned)(p.group < 8 ? p.group : 8)), dim3(32 * kKv4JoinWarps), 0, s, p,
+                         (uint32_t)ctas, items < ranges ? 1 : 0);
     rptc_set_pdl(before ? 1 : 0);
     return e;
 }
