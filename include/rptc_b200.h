@@ -384,7 +384,7 @@ typedef struct rptc_kv_cache {
  * (slots NULL: row t).  x [tokens][ld_x] = [q heads | k heads | v heads] of 128, fp16 or fp32 (x_is_f32: 16-byte aligned, `clear` zeroes it).
  * out fp16 [tokens][ld_out]: the q heads, and with out_kv the k and v heads behind them; may be x itself (fp16) with the same stride.  angles: fp32
  * [max_pos][64][2], cosines and sines (rptc_rope_angles).  pos -1: a token of no sequence, for which nothing is written; any other
- * position or slot outside the cache: nothing is written, RPTC_ERR_RANGE.  No two tokens of a call go to the same place.  Values that are not finite have no
+ * position or slot outside the cache: nothing is written, RPTC_ERR_RANGE.  No two tokens of a call go to the same place.  At most 2^24 tokens and 4096 q heads.  Values that are not finite have no
  * code: what a 4-bit cache holds for their group of 32 then means nothing. */
 typedef struct rptc_append {
     const void *x;
@@ -414,13 +414,11 @@ int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *pos, const 
 
 /* Log probabilities: lse = log sum_i exp(x_i) over a row of logits, logprob = x_target - lse, entropy = lse - sum_i p_i x_i (natural logarithms), and the
  * `top` largest entries as top_logprobs, top_ids, the largest first and equal ones by their index.  logits fp16, bf16 or fp32 (dtype 0, 1, 2)
- * [rows][ld], at least 1 and at most 2^24 of them in a row, aligned to their size; targets int64 [rows] or NULL (then logprob is NULL); entropy may be NULL; 0 <= top <= 32
+ * [rows][ld], at least 1 and at most 2^24 of them in a row and as many rows, aligned to their size; targets int64 [rows] or NULL (then logprob is NULL); entropy may be NULL; 0 <= top <= 32
  * and top <= n.  -inf is a forbidden token (probability 0).  A row without an allowed token, with NaN or with +inf gives NaN, and ids of some order (the forbidden
- * by their index).  target -1: no token, logprob 0; any other outside the row: NaN, RPTC_ERR_RANGE.
- * workspace: 256-byte aligned device memory of rptc_token_logprobs_workspace_bytes (0: none); it holds nothing between calls. */
-int64_t rptc_token_logprobs_workspace_bytes(int64_t rows, int64_t n, int top);
+ * by their index).  target -1: no token, logprob 0; any other outside the row: NaN, RPTC_ERR_RANGE. */
 int rptc_token_logprobs(const void *logits, int dtype, int64_t ld, const int64_t *targets, float *logprob, float *entropy, float *top_logprobs,
-                        int64_t *top_ids, int64_t rows, int64_t n, int top, void *workspace, int64_t workspace_bytes, rptc_stream_t stream);
+                        int64_t *top_ids, int64_t rows, int64_t n, int top, rptc_stream_t stream);
 
 /* --- the code-A trellis encoder (rptc.py:13-71 `quantize`, diagonal corrections; K = 2 bits per weight) ---
  * For each of `rows` sample rows (fp32 [rows][ld_samples], n used) the symbols in 0..3 (int32 [rows][ld_sym]) whose

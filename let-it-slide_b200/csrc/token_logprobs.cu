@@ -442,21 +442,12 @@ static int launch_logprobs(const LogprobParams &p, int64_t rows, int cluster, in
 
 using namespace rptc;
 
-extern "C" int64_t rptc_token_logprobs_workspace_bytes(int64_t rows, int64_t n, int top) {
-    (void)rows, (void)n, (void)top;
-    return 0;
-}
-
 extern "C" int rptc_token_logprobs(const void *logits, int dtype, int64_t ld, const int64_t *targets, float *logprob, float *entropy, float *top_logprobs,
-                                   int64_t *top_ids, int64_t rows, int64_t n, int top, void *workspace, int64_t workspace_bytes, rptc_stream_t stream) {
+                                   int64_t *top_ids, int64_t rows, int64_t n, int top, rptc_stream_t stream) {
     if (!logits || dtype < 0 || dtype > 2 || (targets && !logprob) || top < 0 || (top > 0 && (!top_logprobs || !top_ids))) return RPTC_ERR_ARG;
     if (rows < 0 || n <= 0 || top > n || ld < n) return RPTC_ERR_SHAPE;
     if (top > 32 || n > (1 << 24) || rows > (1 << 24)) return RPTC_ERR_TOO_LARGE;
     if (reinterpret_cast<uintptr_t>(logits) & (dtype == 2 ? 3 : 1)) return RPTC_ERR_ALIGN;
-    if (int64_t need = rptc_token_logprobs_workspace_bytes(rows, n, top)) {
-        if (!workspace || workspace_bytes < need) return RPTC_ERR_ARG;
-        if (reinterpret_cast<uintptr_t>(workspace) & 255) return RPTC_ERR_ALIGN;
-    }
     if (int e = rptc_check_device()) return e;
     if (rows == 0) return RPTC_OK;
     LogprobParams p = {logits, ld, targets, logprob, entropy, top_logprobs, top_ids, n, top, device_status_word()};

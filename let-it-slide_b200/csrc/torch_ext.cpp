@@ -37,7 +37,6 @@ struct {
     decltype(&rptc_kv4_values) kv4_values;
     decltype(&rptc_attn_decode_kv4_workspace_bytes) attn_decode_kv4_workspace_bytes;
     decltype(&rptc_attn_decode_kv4) attn_decode_kv4;
-    decltype(&rptc_token_logprobs_workspace_bytes) token_logprobs_workspace_bytes;
     decltype(&rptc_token_logprobs) token_logprobs;
 } g_lib;
 
@@ -539,17 +538,14 @@ PyObject *token_logprobs(PyObject *, PyObject *const *args, Py_ssize_t nargs) {
         if (dtype < 0 || top < 0 || top > 32 || top > n || !is_rows(x, device, rows, n, ld) || (args[1] != Py_None && !is(targets, device, at::kLong, {rows}))) Py_RETURN_NONE;
         const c10::cuda::OptionalCUDAGuard guard(device);
         const auto f32 = at::TensorOptions().dtype(at::kFloat).device(device);
-        at::Tensor logprob, entropy = at::empty({rows}, f32), best = at::empty({rows, top}, f32), ids = at::empty({rows, top}, f32.dtype(at::kLong)), ws;
+        at::Tensor logprob, entropy = at::empty({rows}, f32), best = at::empty({rows, top}, f32), ids = at::empty({rows, top}, f32.dtype(at::kLong));
         if (targets) logprob = at::empty({rows}, f32);
-        const int64_t need = g_lib.token_logprobs_workspace_bytes(rows, n, (int)top);
-        if (need > 0) ws = at::empty({need}, f32.dtype(at::kByte));
         const cudaStream_t s = current_stream(*x);
         int status;
         Py_BEGIN_ALLOW_THREADS
         status = g_lib.token_logprobs(x->data_ptr(), dtype, ld, targets ? static_cast<const int64_t *>(targets->data_ptr()) : nullptr,
                                       targets ? static_cast<float *>(logprob.data_ptr()) : nullptr, static_cast<float *>(entropy.data_ptr()),
-                                      top ? static_cast<float *>(best.data_ptr()) : nullptr, top ? static_cast<int64_t *>(ids.data_ptr()) : nullptr, rows, n, (int)top,
-                                      need > 0 ? ws.data_ptr() : nullptr, need, s);
+                                      top ? static_cast<float *>(best.data_ptr()) : nullptr, top ? static_cast<int64_t *>(ids.data_ptr()) : nullptr, rows, n, (int)top, s);
         Py_END_ALLOW_THREADS
         if (status != RPTC_OK) return PyLong_FromLong(status);
         PyObject *first = targets ? THPVariable_Wrap(std::move(logprob)) : Py_NewRef(Py_None);

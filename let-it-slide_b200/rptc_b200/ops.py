@@ -561,10 +561,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, to
     best, ids = torch.empty((rows, top), **f32), torch.empty((rows, top), dtype=torch.int64, device=device)
     if rows == 0:
         return logprob, entropy, best, ids
-    need = lib().rptc_token_logprobs_workspace_bytes(rows, n, top)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
     call("rptc_token_logprobs", device, ptr(logits), _LOGIT_TYPES[logits.dtype], _ld(logits, n), ptr(targets), ptr(logprob), ptr(entropy),
-         ptr(best) if top else None, ptr(ids) if top else None, rows, n, top, ptr(ws), need)
+         ptr(best) if top else None, ptr(ids) if top else None, rows, n, top)
     return logprob, entropy, best, ids
 
 

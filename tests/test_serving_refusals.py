@@ -44,8 +44,7 @@ def decode(c=None, **kw):
 def logprobs(**kw):
     from rptc_b200 import lib
     a = {**dict(logits=BASE, dtype=0, ld=100, targets=BASE, logprob=BASE, entropy=BASE, top_lp=BASE, top_ids=BASE, rows=3, n=100, top=5), **kw}
-    return lib().rptc_token_logprobs(a["logits"], a["dtype"], a["ld"], a["targets"], a["logprob"], a["entropy"], a["top_lp"], a["top_ids"], a["rows"], a["n"], a["top"], None,
-                                     0, None)
+    return lib().rptc_token_logprobs(a["logits"], a["dtype"], a["ld"], a["targets"], a["logprob"], a["entropy"], a["top_lp"], a["top_ids"], a["rows"], a["n"], a["top"], None)
 
 
 NO_DEVICE = (-5, -8)      # what a call that nothing is wrong with gets without a GPU
