@@ -19,7 +19,8 @@
 // Bound: the exponentials.  A tile of 128 keys and 256 rows takes 2770 to 3000 clocks: 2048 for its 32768 exponentials on the special-function unit (busy 69 % of the time at
 // 8192 tokens, as is the tensor pipe), 1024 for its products, the rest the softmax warps' other work.  One prompt of 2048 tokens, 32 heads of 128: 37.6 us (fp16, 0.91 PFLOP/s);
 // one of 8192, 64 heads over 8: 845 us (1.30 PFLOP/s, at the power cap).  A short prompt pays for its set-up too: first scores after some 7000 clocks, the last result 2200 after
-// the last product; 24 tokens take 6.6 us.  Sixteen sequences of 1 to 1024 tokens with `pack` heads together 80 us, with one head at a time 112.
+// the last product; 24 tokens take 6.6 us.  Sixteen sequences of 1 to 1021 tokens, 64 heads over 8, with `pack` heads together
+// 77 us; when they took 80, one head at a time took 112.
 #include <cuda_bf16.h>
 
 #include "tc_ptx.cuh"
@@ -355,6 +356,45 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
             const bool there = my_token < it.tokens;
             const float inv = l > 0.f ? 1.f / l : l == 0.f ? 0.f : l;               // NaN stays
             uint16_t *out = p.out + (int64_t)(it.token + my_token) * p.out_row + (int64_t)(it.head + my_head) * p.out_head;
+            if (p.wide) {
+                // 64 columns at a time, 128 bytes of a row.  A store in which every lane has a row of its own touches as many lines as lanes; so four lanes exchange their rows'
+                // quarters first, and each store has 128 bytes of eight rows (the sixteen sequences below 80.3 us without, 77.3 so).
+                uint16_t *rows[4];
+                uint32_t theirs = __ballot_sync(0xFFFFFFFFu, there) >> (lane & 28);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) rows[k] = reinterpret_cast<uint16_t *>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<unsigned long long>(out), (lane & 28) + k)) + 16 * (lane & 3);
+#pragma unroll 1
+                for (int c = 0; c < DP * 64; c += 64) {
+                    uint32_t o[64], w[4][8];
+                    if (tiles > 0) {
+                        tmem_load64(o_tmem + (uint32_t)c, o);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 64; ++e) o[e] = 0u;
+                    }
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) {
+                        const float a = __uint_as_float(o[2 * q]) * inv, b = __uint_as_float(o[2 * q + 1]) * inv;
+                        w[q >> 3][q & 7] = inv == 0.f ? 0u : pack16<BF16>(a, b);
+                    }
+#pragma unroll
+                    for (int h = 1; h < 4; h <<= 1) {
+                        const bool up = lane & h;
+#pragma unroll
+                        for (int b = 0; b < 4; ++b)
+                            if (!(b & h))
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) {
+                                    const uint32_t got = __shfl_xor_sync(0xFFFFFFFFu, up ? w[b][q] : w[b + h][q], h);
+                                    if (up) w[b][q] = got;
+                                    else w[b + h][q] = got;
+                                }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (theirs >> k & 1) st_32_bytes(rows[k] + c, w[k]);
+                }
+            } else {
 #pragma unroll 1
             for (int c = 0; c < DP * 64; c += 32) {
                 uint32_t o[32];
@@ -373,13 +413,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
                         const float a = __uint_as_float(o[e + 2 * q]) * inv, b = __uint_as_float(o[e + 2 * q + 1]) * inv;
                         w[q] = inv == 0.f ? 0u : pack16<BF16>(a, b);
                     }
-                    if (p.wide) {
-                        st_32_bytes(out + c + e, w);
-                    } else {
-                        *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                        *reinterpret_cast<uint4 *>(out + c + e + 8) = make_uint4(w[4], w[5], w[6], w[7]);
-                    }
+                    *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    *reinterpret_cast<uint4 *>(out + c + e + 8) = make_uint4(w[4], w[5], w[6], w[7]);
                 }
+            }
             }
             tc_fence_before();
         }
