@@ -240,7 +240,7 @@ def _quantised(x):
     """[tokens, heads, 128] -> codes [tokens, heads, 4, 32] and (scale, minimum), one rounding each"""
     g = x.unflatten(-1, (4, 32))
     low, high = g.amin(-1), g.amax(-1)
-    scale = ((high - low) / torch.full_like(high, 15.0)).half()
+    scale = ((high - low) / 15).half()
     step = scale.float()[..., None]
     codes = torch.where(step > 0, torch.round((g - low[..., None]) / step), 0.0).clamp(0, 15)
     return codes.to(torch.int32), torch.stack((scale, low.half()), dim=-1)
