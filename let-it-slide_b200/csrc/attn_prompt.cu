@@ -393,30 +393,31 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
                         if (theirs >> k & 1) st_32_bytes(rows[k] + c, w[k]);
+                    __syncwarp();                                                   // what reads tensor memory next is the whole warp
                 }
             } else {
+                // Rows or heads that lie on 16 bytes only.  The stores are up to a lane; what reads tensor memory is the whole warp, with all of its lanes together.
 #pragma unroll 1
-            for (int c = 0; c < DP * 64; c += 32) {
-                uint32_t o[32];
-                if (tiles > 0) {
-                    tmem_load32(o_tmem + (uint32_t)c, o);
-                } else {
+                for (int c = 0; c < DP * 64; c += 32) {
+                    uint32_t o[32];
+                    if (tiles > 0) {
+                        tmem_load32(o_tmem + (uint32_t)c, o);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) o[e] = 0u;
-                }
-                if (!there) continue;
-#pragma unroll
-                for (int e = 0; e < 32; e += 16) {
-                    uint32_t w[8];
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) {
-                        const float a = __uint_as_float(o[e + 2 * q]) * inv, b = __uint_as_float(o[e + 2 * q + 1]) * inv;
-                        w[q] = inv == 0.f ? 0u : pack16<BF16>(a, b);
+                        for (int e = 0; e < 32; ++e) o[e] = 0u;
                     }
-                    *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
-                    *reinterpret_cast<uint4 *>(out + c + e + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const float a = __uint_as_float(o[e + 2 * q]) * inv, b = __uint_as_float(o[e + 2 * q + 1]) * inv;
+                            w[q] = inv == 0.f ? 0u : pack16<BF16>(a, b);
+                        }
+                        if (there) *reinterpret_cast<uint4 *>(out + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    __syncwarp();
                 }
-            }
             }
             tc_fence_before();
         }
