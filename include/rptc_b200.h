@@ -407,7 +407,8 @@ int rptc_kv4_values(const rptc_kv_cache *cache, const int32_t *count, void *k_ou
 /* Single-query attention of each row's q heads over positions 0 .. pos[row] of a 4-bit cache: rptc_attn_decode for it.  q fp16 [rows][ld_q], 16-byte aligned,
  * ld_q % 8 == 0; out fp16 [rows][ld_out], q heads of 128.  heads a multiple of cache->kv_heads; signs_in as in rptc_attn_decode.
  * pos -1: a row of no sequence, whose out is zeros; any other position outside the cache: zeros, RPTC_ERR_RANGE.  workspace: 256-byte aligned device
- * memory of rptc_attn_decode_kv4_workspace_bytes; it holds nothing between calls, and calls that may overlap need one each. */
+ * memory of rptc_attn_decode_kv4_workspace_bytes; it holds nothing between calls, and calls that may overlap need one each.  Where there is one,
+ * rows * kv_heads * ceil(heads / kv_heads / 8) * (ceil(max_pos / 32) + 24) below 2^32 (RPTC_ERR_TOO_LARGE). */
 int64_t rptc_attn_decode_kv4_workspace_bytes(const rptc_kv_cache *cache, int heads);
 int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *pos, const rptc_kv_cache *cache, void *out, int64_t ld_out, int heads,
                          float scale, const void *signs_in, void *workspace, int64_t workspace_bytes, rptc_stream_t stream);

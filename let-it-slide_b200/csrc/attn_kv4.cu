@@ -56,8 +56,8 @@ __device__ __forceinline__ int kv4_context(const AttnKv4Params &p, const int32_t
 __device__ __forceinline__ int kv4_tiles(int context) { return (context + kKv4Tile - 1) / kKv4Tile; }
 
 // How the work is cut: every row's heads laid end to end, each worth its tiles and kKv4Start for what a CTA does around them (q, the warps' sums).  32 rows of 500 to 32768
-// take 139.4 us with 16 of those, 135.5 with 20, 135.8 with 24 and 136.7 with 32; kKv4Least is what a CTA is worth starting for.  In numbers of 32 bits: a unit stands for a tile of
-// 5 KiB of the cache.
+// take 139.4 us with 16 of those, 135.5 with 20, 135.8 with 24 and 136.7 with 32; kKv4Least is what a CTA is worth starting for.  In numbers of 32 bits: a call whose full rows
+// would pass them is refused (kv4_units; a tile counts once for every eight q heads of its kv head).
 constexpr uint32_t kKv4Start = 24, kKv4Least = 16;
 __device__ __forceinline__ uint32_t kv4_cost(int tiles) { return tiles ? (uint32_t)tiles + kKv4Start : 0u; }
 // A CTA has two ranges, one for each eight of its warps, which share nothing.  (Two CTAs of eight warps on an SM: the one that came first is served first and ends long before
@@ -577,6 +577,12 @@ static bool kv4_whole(const rptc_kv_cache &c, int heads) {
     return c.max_pos <= 1024 || (c.max_pos <= 2048 && 4 * items >= num_sms());
 }
 
+// What all rows' heads are worth when full, as the cut counts: below 2^48.
+static int64_t kv4_units(const rptc_kv_cache &c, int heads) {
+    const int64_t items = (int64_t)c.rows * c.kv_heads * ((heads / c.kv_heads + 7) / 8);
+    return items * ((c.max_pos + kKv4Tile - 1) / kKv4Tile + kKv4Start);
+}
+
 extern "C" int64_t rptc_attn_decode_kv4_workspace_bytes(const rptc_kv_cache *cache, int heads) {
     if (!cache || check_kv_cache(*cache) || cache->bits != 4 || heads <= 0 || kv4_whole(*cache, heads)) return 0;
     return (int64_t)num_sms() * 2 * 2 * 8 * (128 * 4 + 8);
@@ -589,7 +595,7 @@ extern "C" int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *
     if (cache->bits != 4) return RPTC_ERR_UNSUPPORTED;
     if (!(scale > 0.f && scale < 1e30f)) return RPTC_ERR_ARG;
     if (heads <= 0 || heads % cache->kv_heads || ld_q < (int64_t)heads * 128 || ld_out < (int64_t)heads * 128) return RPTC_ERR_SHAPE;
-    if (heads > 4096) return RPTC_ERR_TOO_LARGE;
+    if (heads > 4096 || (!kv4_whole(*cache, heads) && kv4_units(*cache, heads) >> 32)) return RPTC_ERR_TOO_LARGE;
     if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) || (reinterpret_cast<uintptr_t>(signs_in) & 15) || (ld_q % 8) ||
         (ld_out % 8))
         return RPTC_ERR_ALIGN;
