@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(256) qkv_append_kernel(const AppendParams p) {
     const int64_t slot = slot_p ? __ldg(slot_p + token) : token;
     const bool takes = __any_sync(0xFFFFFFFFu, pos >= 0 && pos < p.max_pos && slot >= 0 && slot < p.rows);
     if (!takes && pos != -1 && lane == 0) atomicExch(p.status, kStatusPosition);
-    // Everything advances by two heads.  Of an odd number the last is taken by both halves of the warp, which read it before either writes.
+    // Everything advances by two heads.  Of an odd number the last is taken by both halves of the warp, which read it before either writes (x itself may be cleared, or be out).
     int head = min(first + half, end - 1);
     const char *x = reinterpret_cast<const char *>(p.x) + (token * p.ld_x + (base + head) * 128 + 8 * dl) * (F32 ? 4 : 2);
     const __half *signs = p.signs + (base + head) * 128 + 8 * dl;
@@ -88,6 +88,7 @@ __global__ void __launch_bounds__(256) qkv_append_kernel(const AppendParams p) {
 #pragma unroll 1
     for (int left = end - first; left > 0; left -= 2) {
         const EightRaw<F32> raw = next;
+        __syncwarp();                                        // all lanes have read what this step writes
         if (F32 && p.clear) {
             float4 *src = reinterpret_cast<float4 *>(const_cast<char *>(x));
             src[0] = src[1] = make_float4(0.f, 0.f, 0.f, 0.f);
