@@ -589,7 +589,9 @@ class RPTCLlama:
     def prefill_packed(self, prompts: list[torch.Tensor]) -> torch.Tensor:
         """`prefill` for prompts of different lengths: prompts[r] (whole numbers, at least one) goes into row r from position 0 on.  All tokens go
         through the network packed, one prompt behind the other (`ops.attn_prompt`), so that nothing is padded.  Returns the logits behind each
-        prompt's last token, fp16 [rows, vocab]; `pos` is set to the lengths and `ids` to the greedy choices; decoding continues with `step`."""
+        prompt's last token, fp16 [rows, vocab]; `pos` is set to the lengths and `ids` to the greedy choices; decoding continues with `step`.
+        What is refused (ValueError) leaves the rows as they are."""
+        prompts = self._accepted(prompts, [0] * self.rows)
         self.reset()
         return self._greedy(self._push(prompts, whole=False))
 
@@ -597,44 +599,58 @@ class RPTCLlama:
     def extend(self, prompts: list[torch.Tensor]) -> torch.Tensor:
         """`prefill_packed` behind what the rows hold already: row r continues at `pos[r]` (a further turn of a conversation).  The new
         tokens attend over the cached positions as the cache holds them, their own among them."""
-        return self._greedy(self._push(prompts, whole=False))
+        return self._greedy(self._push(self._accepted(prompts, [self._pos_hi - b for b in self._behind]), whole=False))
 
     @torch.no_grad()
     def score(self, prompts: list[torch.Tensor], top: int = 0) -> list[tuple]:
         """How probable the model finds given texts: for each prompt (any number of them) (logprob, entropy, top_logprobs, top_ids), entry t about token
         t + 1 given the tokens up to t (`ops.token_logprobs`; one entry less than tokens).  The perplexity of a text is exp of minus the mean of
-        logprob.  Uses the rows' caches: the model is reset before and after."""
+        logprob.  Uses the rows' caches: the model is reset before and after.  What is refused (ValueError) leaves the rows as they are."""
+        if not 0 <= top <= min(32, self.cfg.vocab):
+            raise ValueError(f"top must be between 0 and {min(32, self.cfg.vocab)}, got {top}")
+        groups = [self._accepted(prompts[p0:p0 + self.rows], [0] * self.rows, fewer=True) for p0 in range(0, len(prompts), self.rows)]
         found = []
-        for p0 in range(0, len(prompts), self.rows):
-            group = [torch.as_tensor(p, device=self.device) for p in prompts[p0:p0 + self.rows]]
+        try:
+            for group in groups:
+                self.reset()
+                h = self._push(group, whole=True)
+                targets = torch.cat([torch.cat((p[1:], p.new_full((1,), -1))) for p in group])
+                xn, outs = torch.empty_like(h), []
+                ops.rmsnorm(h, self.norm_f, xn, self.cfg.rms_eps)
+                for t0 in range(0, len(targets), 4096):          # the logits of so many tokens at a time
+                    outs.append(ops.token_logprobs(xn[t0:t0 + 4096] @ self.head.t(), targets[t0:t0 + 4096], top))
+                columns = [torch.cat(c).split([len(p) for p in group]) for c in zip(*outs)]
+                found += [tuple(c[i][:-1] for c in columns) for i in range(len(group))]
+        finally:
             self.reset()
-            h = self._push(group, whole=True)
-            targets = torch.cat([torch.cat((p[1:].long(), p.new_full((1,), -1).long())) for p in group])
-            xn, outs = torch.empty_like(h), []
-            ops.rmsnorm(h, self.norm_f, xn, self.cfg.rms_eps)
-            for t0 in range(0, len(targets), 4096):              # the logits of so many tokens at a time
-                outs.append(ops.token_logprobs(xn[t0:t0 + 4096] @ self.head.t(), targets[t0:t0 + 4096], top))
-            columns = [torch.cat(c).split([len(p) for p in group]) for c in zip(*outs)]
-            found += [tuple(c[i][:-1] for c in columns) for i in range(len(group))]
-        self.reset()
         return found
 
-    def _push(self, prompts: list[torch.Tensor], whole: bool) -> torch.Tensor:
-        """Tokens of prompts[r] behind what row r holds (the first len(prompts) rows), one packed pass.  Returns the residual stream behind the blocks, of
-        every token (`whole`) or of each prompt's last; `pos` is left at the last token's position."""
-        cfg, D = self.cfg, self.cfg.head_dim
+    def _accepted(self, prompts: list[torch.Tensor], held: list[int], fewer: bool = False) -> list[torch.Tensor]:
+        """The prompts as whole numbers on the model's device, prompts[r] behind held[r] positions of row r (`fewer`: for the first rows alone), or a ValueError.
+        Nothing of the model changes."""
+        cfg = self.cfg
         prompts = [torch.as_tensor(p, device=self.device) for p in prompts]
-        lengths, n = [p.numel() for p in prompts], len(prompts)
-        if (n != self.rows and not (whole and 0 < n < self.rows)) or any(p.dim() != 1 or p.numel() == 0 or p.is_floating_point() for p in prompts):
+        n = len(prompts)
+        if (n != self.rows and not (fewer and 0 < n < self.rows)) or any(p.dim() != 1 or p.numel() == 0 or p.is_floating_point() for p in prompts):
             raise ValueError("prompts must be one row of at least one token each, one for every row of the model")
-        if D != 128:
+        if cfg.head_dim != 128:
             raise ValueError("packed prompts need heads of 128")
-        ends = [self._pos_hi - b + l for b, l in zip(self._behind, lengths + [0] * (self.rows - n))]
+        ends = [b + p.numel() for b, p in zip(held, prompts)]
         if max(ends) > cfg.max_pos:
             raise ValueError(f"row {ends.index(max(ends))} would have {max(ends)} positions, but the KV caches hold max_pos = {cfg.max_pos}")
-        ids = torch.cat([p.long() for p in prompts])
+        prompts = [p.long() for p in prompts]
+        ids = torch.cat(prompts)
         if not bool(((ids >= 0) & (ids < cfg.vocab)).all()):
             raise ValueError(f"token ids must be between 0 and {cfg.vocab - 1}")
+        return prompts
+
+    def _push(self, prompts: list[torch.Tensor], whole: bool) -> torch.Tensor:
+        """Tokens of prompts[r] (as `_accepted` gives them) behind what row r holds (the first len(prompts) rows), one packed pass.  Returns the residual stream behind
+        the blocks, of every token (`whole`) or of each prompt's last; `pos` is left at the last token's position."""
+        cfg, D = self.cfg, self.cfg.head_dim
+        lengths, n = [p.numel() for p in prompts], len(prompts)
+        ends = [self._pos_hi - b + l for b, l in zip(self._behind, lengths + [0] * (self.rows - n))]
+        ids = torch.cat(prompts)
         fresh = self._pos_hi == 0                                # no row holds anything
         total = sum(lengths)
         i32 = dict(dtype=torch.int32, device=self.device)
