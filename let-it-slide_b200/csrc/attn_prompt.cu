@@ -10,7 +10,9 @@
 //                        16 bits (the one rounding besides the result's: the tensor core multiplies 16-bit operands; l adds the weights up before it)
 //   O += P V             tcgen05.mma with P in tensor memory, V in shared memory as it lies (N-major), O in tensor memory (fp32)
 // The two halves alternate: the tensor core works on one while the other's softmax runs.  m follows the true maximum with a slack of 2^8: only a larger step
-// rescales O and l (by the thread that owns the row; the scores' barrier says that the product before has been added).  exp2 of differences up to 8 stays far inside fp16 and fp32.
+// rescales O and l (by the thread that owns the row; the scores' barrier says that the product before has been added).  fp16 weights are 2^7 for a score of m, 2^15 at
+// most: what is below fp16's normal numbers is then 2^-21 of the largest weight, and off by 2^-32 of it (with weights of 1 for m many small ones, as behind a first key that takes
+// nearly all, came out as zeros: 60000 of 2^-25.5 count for 0.0013).
 // Warps 0-3 and 4-7: softmax and output of the halves; 8: MMAs; 9: TMA loads (ring of key and value tiles); 10: the list of items.
 // Masks are applied to tiles that reach beyond a half's first row only.  Value rows behind the last key are zeroed in shared memory: a weight of 0 times whatever
 // lies there has to be 0.
@@ -35,6 +37,8 @@ constexpr int kPromptReaders = 10;                   // warps that take items of
 constexpr uint32_t kPromptPanel = 128 * 128;         // 128 rows of 64 values
 constexpr int kTileKeys = 128;
 constexpr float kSlack = 8.f;                        // log2 of how far a score may pass the maximum that its row's weights refer to
+constexpr float kHalfBias = 7.f;                     // log2 of an fp16 weight whose score is that maximum
+static_assert(kSlack + kHalfBias < 16.f, "the largest weight in fp16");
 
 struct PromptParams {
     uint16_t *out;
@@ -278,6 +282,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_tmem = tmem + 128u * half + lanes, o_tmem = tmem + 256u + 128u * half + lanes;
         const uint32_t my_s = s_full + 8 * half, my_p = p_full + 16 * half;
         uint32_t phase = 0u, o_phase = 0u;
+        constexpr float kBias = BF16 ? 0.f : kHalfBias;
         while (next_item(it)) {
             const int tiles = half ? it.tiles1 : it.tiles0, first_seen = it.seen + half * half_tokens;
             const int last = min(it.seen + my_token, it.keys - 1);                  // the last key that this row sees
@@ -322,7 +327,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attn_prompt_kernel(const Pr
                         }
                     }
                 }
-                const f32x2 scale2 = pack2(p.scale, p.scale), shift2 = pack2(-m * p.scale, -m * p.scale);
+                const f32x2 scale2 = pack2(p.scale, p.scale), shift2 = pack2(fmaf(-m, p.scale, kBias), fmaf(-m, p.scale, kBias));
                 f32x2 sum[4];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {                                       // 64 keys: the product takes them while the next are made
