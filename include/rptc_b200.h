@@ -384,8 +384,8 @@ typedef struct rptc_kv_cache {
  * (slots NULL: row t).  x [tokens][ld_x] = [q heads | k heads | v heads] of 128, fp16 or fp32 (x_is_f32: 16-byte aligned, `clear` zeroes it).
  * out fp16 [tokens][ld_out]: the q heads, and with out_kv the k and v heads behind them; may be x itself (fp16) with the same stride.  angles: fp32
  * [max_pos][64][2], cosines and sines (rptc_rope_angles).  pos -1: a token of no sequence, for which nothing is written; any other
- * position or slot outside the cache: nothing is written, RPTC_ERR_RANGE.  No two tokens of a call go to the same place.  At most 2^24 tokens and 4096 q heads.  Values that are not finite have no
- * code: what a 4-bit cache holds for their group of 32 then means nothing. */
+ * position or slot outside the cache: nothing is written, RPTC_ERR_RANGE.  No two tokens of a call go to the same place.  At most 2^24 tokens and 4096 q heads.  A value that is not finite has no
+ * code: in a 4-bit cache its group of 32 gets a scale of NaN, and stands for NaN. */
 typedef struct rptc_append {
     const void *x;
     int64_t ld_x;

@@ -18,8 +18,20 @@ inline int check_kv_cache(const rptc_kv_cache &c) {
 }
 
 #ifdef __CUDACC__
+// NaN if either is.
+__device__ __forceinline__ float kv4_min(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float kv4_max(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 // A group's scale, as it is stored, and its reciprocal.  The difference and its fifteenth are rounded to 32 bits each, the scale then to fp16: what is stored is what the
-// codes are counted in.
+// codes are counted in.  NaN where the range is NaN or infinite (the remainder is): all of a group stands for NaN as soon as one of its values is not finite, and what reads
+// the cache shows it as it would an fp16 cache's.
 __device__ __forceinline__ __half2 kv4_scale(float lo, float hi, float &inv) {
     const float range = hi - lo, part = range * (1.f / 15.f);
     const __half scale = __float2half_rn(fmaf(fmaf(-part, 15.f, range), 1.f / 15.f, part));      // the rounded fifteenth, for every significand
@@ -39,12 +51,12 @@ __device__ __forceinline__ uint32_t kv4_code(float v, float lo, float step, floa
 // Eight neighbouring values of a thread, whose group of 32 is that of four neighbouring lanes -> the thread's eight codes (nibbles, first value lowest) and the
 // group's scale and minimum.
 __device__ __forceinline__ uint32_t kv4_quantise(const float (&v)[8], __half2 &scale_min) {
-    float lo = fminf(fminf(fminf(v[0], v[1]), fminf(v[2], v[3])), fminf(fminf(v[4], v[5]), fminf(v[6], v[7])));
-    float hi = fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
+    float lo = kv4_min(kv4_min(kv4_min(v[0], v[1]), kv4_min(v[2], v[3])), kv4_min(kv4_min(v[4], v[5]), kv4_min(v[6], v[7])));
+    float hi = kv4_max(kv4_max(kv4_max(v[0], v[1]), kv4_max(v[2], v[3])), kv4_max(kv4_max(v[4], v[5]), kv4_max(v[6], v[7])));
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
+        lo = kv4_min(lo, __shfl_xor_sync(0xFFFFFFFFu, lo, o));
+        hi = kv4_max(hi, __shfl_xor_sync(0xFFFFFFFFu, hi, o));
     }
     float inv;
     scale_min = kv4_scale(lo, hi, inv);

@@ -314,9 +314,9 @@ __global__ void __launch_bounds__(256, 2) qkv_append_heads_kernel(const AppendPa
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const uint32_t(&v)[4] = o[e >> 1][e & 1];
-            const uint32_t most = half2_as_u32(__hmax2(__hmax2(u32_as_half2(v[0]), u32_as_half2(v[1])), __hmax2(u32_as_half2(v[2]), u32_as_half2(v[3]))));
-            const uint32_t least = half2_as_u32(__hmin2(__hmin2(u32_as_half2(v[0]), u32_as_half2(v[1])), __hmin2(u32_as_half2(v[2]), u32_as_half2(v[3])))) ^ 0x80008000u;
-            m[e] = half2_as_u32(__hmax2(u32_as_half2(__byte_perm(most, least, 0x5410)), u32_as_half2(__byte_perm(most, least, 0x7632))));
+            const uint32_t most = half2_as_u32(__hmax2_nan(__hmax2_nan(u32_as_half2(v[0]), u32_as_half2(v[1])), __hmax2_nan(u32_as_half2(v[2]), u32_as_half2(v[3]))));
+            const uint32_t least = half2_as_u32(__hmin2_nan(__hmin2_nan(u32_as_half2(v[0]), u32_as_half2(v[1])), __hmin2_nan(u32_as_half2(v[2]), u32_as_half2(v[3])))) ^ 0x80008000u;
+            m[e] = half2_as_u32(__hmax2_nan(u32_as_half2(__byte_perm(most, least, 0x5410)), u32_as_half2(__byte_perm(most, least, 0x7632))));
         }
 #pragma unroll
         for (int h = 2; h > 0; h >>= 1) {
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(256, 2) qkv_append_heads_kernel(const AppendPa
 #pragma unroll
             for (int e = 0; e < h; ++e) {
                 const uint32_t keep = up ? m[e + h] : m[e], give = up ? m[e] : m[e + h];
-                m[e] = half2_as_u32(__hmax2(u32_as_half2(keep), u32_as_half2(__shfl_xor_sync(0xFFFFFFFFu, give, 4 * h))));
+                m[e] = half2_as_u32(__hmax2_nan(u32_as_half2(keep), u32_as_half2(__shfl_xor_sync(0xFFFFFFFFu, give, 4 * h))));
             }
         }
         const float2 ends = __half22float2(u32_as_half2(m[0]));      // of head 2 t + (g & 3) / 2, group 2 (g & 1) + g / 4
