@@ -371,7 +371,8 @@ int rptc_attn_prompt(const rptc_prompt_attention *a, rptc_stream_t stream);
  * bits = 16: k, v fp16 [rows][max_pos][kv_heads][128]; no scales.
  * bits = 4: k, v codes uint8 [rows][kv_heads][max_pos][64], k_scales, v_scales fp16 [rows][kv_heads][max_pos][4][2]: for each group of 32
  * values (scale, minimum), scale = fp16((max - min) / 15) and code = round((x - min) / scale), half to even, at most 15 (0 where the
- * scale is 0); the code stands for minimum + code * scale.  Value e of group g is nibble e % 4 of the 16-bit word 4 * (e / 4) + g: dims 4 i .. 4 i + 3 of all four groups
+ * scale is 0), differences and quotients rounded to fp32 each (x - min of fp16 values may need more: next to half-way the code is that of the rounded difference); the
+ * code stands for minimum + code * scale.  Value e of group g is nibble e % 4 of the 16-bit word 4 * (e / 4) + g: dims 4 i .. 4 i + 3 of all four groups
  * are eight bytes.  All 16-byte aligned, contiguous.  At most 65535 rows, 2^24 positions and 4096 kv heads. */
 typedef struct rptc_kv_cache {
     void *k, *k_scales, *v, *v_scales;

@@ -40,9 +40,11 @@ __device__ __forceinline__ __half2 kv4_scale(float lo, float hi, float &inv) {
     return __halves2half2(scale, __float2half_rn(lo));
 }
 // A value's code, as 12582912 + code: a sum of theirs and their multiples by 16, 256 and 4096 has the codes in its low 16 bits.
-// Quotient by Markstein's correction (an estimate times the reciprocal, its exact remainder by a fused multiply-add, and the remainder's quotient added): one that is
-// half-way between two codes comes out exactly; any other differs from half-way by 2^-17 of itself at least (fp16 numbers over an fp16 number), far more than the estimate is off.
-// It passes 15.5 only where the scale was rounded by more than a thirtieth: below 2^-20 (fp16's steps there are 2^-24), kKv4Exact with room to spare.
+// The code is that of fp32 arithmetic, rounded half to even: v - lo rounded to 32 bits (the difference of two fp16 numbers may need some 40), over the scale, rounded to 32 bits.
+// The quotient by Markstein's correction: an estimate by the correctly rounded reciprocal, its exact remainder by a fused multiply-add, and the remainder's quotient added,
+// which is the correctly rounded quotient.  A difference that the first rounding brings to half-way between two codes goes to the even one: a minimum of -15, a scale of 2
+// and a value of -1.8e-7 give 8, where unrounded numbers give 7 (7.5 less 2^-23).  The quotient passes 15.5 only where the scale was rounded by more than a thirtieth: below 2^-20
+// (fp16's steps there are 2^-24), kKv4Exact with room to spare.
 constexpr float kKv4Exact = 1.9073486328125e-6f;                     // 2^-19
 __device__ __forceinline__ uint32_t kv4_code(float v, float lo, float step, float inv, bool small = true) {
     const float d = v - lo, q0 = d * inv, q = fmaf(fmaf(-q0, step, d), inv, q0);

@@ -1,7 +1,7 @@
 // The output side of a fused qkv layer for tokens of any sequences (output transform, rotary embedding, append to an fp16 or 4-bit
 // cache), and the values that a 4-bit cache stands for.  No reference counterpart.
 //
-//   y = rope(scale signs H x) per head of 128;   a group of 32 values of k or v: scale = (max - min) / 15, code = round((value - min) / scale)
+//   y = rope(scale signs H x) per head of 128;   a group of 32 values of k or v: scale = (max - min) / 15, code = round((value - min) / scale), in fp32
 //
 // Bound: HBM by bytes; in fact the issue slots and the SM's load and store pipe, each some 60 % busy: 2048 tokens of 96 heads 30 us where the traffic is 17; 16 tokens
 // 2.5 us, a launch.  The values of a cache: 8.1 us for 2048 positions of 32 kv heads, its traffic 6.7.
