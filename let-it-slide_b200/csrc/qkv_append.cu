@@ -385,22 +385,22 @@ __global__ void __launch_bounds__(256) kv4_values_kernel(const uint8_t *__restri
     const uint8_t *codes = after_wait(blockIdx.z ? v : k);
     const __half2 *scales = after_wait(blockIdx.z ? v_scales : k_scales);
     __half *out = blockIdx.z ? v_out : k_out;
-    for (int pos = blockIdx.x * 32 + (threadIdx.x >> 3); pos < n; pos += gridDim.x * 32) {
-        const int64_t at = (int64_t)blockIdx.y * max_pos + pos;
-        const uint2 c = *reinterpret_cast<const uint2 *>(codes + at * kKv4Codes + 8 * g);
-        const uint4 sm = *reinterpret_cast<const uint4 *>(scales + at * 4);
-        const uint32_t w[2] = {c.x, c.y}, s[4] = {sm.x, sm.y, sm.z, sm.w};
-        __half *dst = out + ((row * max_pos + pos) * hkv + head) * 128 + 4 * g;
+    const int pos = blockIdx.x * 32 + (threadIdx.x >> 3);      // the grid covers all positions of a row
+    if (pos >= n) return;
+    const int64_t at = (int64_t)blockIdx.y * max_pos + pos;
+    const uint2 c = *reinterpret_cast<const uint2 *>(codes + at * kKv4Codes + 8 * g);
+    const uint4 sm = *reinterpret_cast<const uint4 *>(scales + at * 4);
+    const uint32_t w[2] = {c.x, c.y}, s[4] = {sm.x, sm.y, sm.z, sm.w};
+    __half *dst = out + ((row * max_pos + pos) * hkv + head) * 128 + 4 * g;
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {                     // two groups at a time: one rounding, that of the fused multiply-add
-            const uint32_t scale = __byte_perm(s[j], s[j + 1], 0x5410), least = __byte_perm(s[j], s[j + 1], 0x7632);
-            uint32_t o[4];
+    for (int j = 0; j < 4; j += 2) {                     // two groups at a time: one rounding, that of the fused multiply-add
+        const uint32_t scale = __byte_perm(s[j], s[j + 1], 0x5410), least = __byte_perm(s[j], s[j + 1], 0x7632);
+        uint32_t o[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                o[i] = half2_as_u32(__hfma2(__hsub2(u32_as_half2(((w[j >> 1] >> (4 * i)) & 0x000F000Fu) | 0x64006400u), u32_as_half2(0x64006400u)), u32_as_half2(scale), u32_as_half2(least)));
-            *reinterpret_cast<uint2 *>(dst + 32 * j) = make_uint2(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410));
-            *reinterpret_cast<uint2 *>(dst + 32 * j + 32) = make_uint2(__byte_perm(o[0], o[1], 0x7632), __byte_perm(o[2], o[3], 0x7632));
-        }
+        for (int i = 0; i < 4; ++i)
+            o[i] = half2_as_u32(__hfma2(__hsub2(u32_as_half2(((w[j >> 1] >> (4 * i)) & 0x000F000Fu) | 0x64006400u), u32_as_half2(0x64006400u)), u32_as_half2(scale), u32_as_half2(least)));
+        *reinterpret_cast<uint2 *>(dst + 32 * j) = make_uint2(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410));
+        *reinterpret_cast<uint2 *>(dst + 32 * j + 32) = make_uint2(__byte_perm(o[0], o[1], 0x7632), __byte_perm(o[2], o[3], 0x7632));
     }
 }
 

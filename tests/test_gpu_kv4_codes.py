@@ -73,3 +73,17 @@ def test_such_groups_behind_the_transform(hkv, tokens):
     here = torch.arange(tokens, device="cuda")
     assert compare(k, cache[0][here, :, pos.long()][:, :, None], cache[1][here, :, pos.long()][:, :, None]) > 10
     ops.device_status()
+
+
+@pytest.mark.parametrize("spread,offset", [(1.0, 0.0), (1e-6, 0.0), (3000.0, 0.0), (0.01, 500.0), (1.0, -1e-3)])
+def test_values_are_rounded_once(spread, offset):
+    """What a cache's codes stand for, to the bit: minimum + code * scale is exact in 64 bits (fp16's exponents span 40, a product has 15 bits), and rounded to fp16 directly."""
+    from rptc_b200 import ops
+    from test_gpu_kv4 import decoded, random_cache
+    g = torch.Generator(device="cuda").manual_seed(3)
+    cache = random_cache(g, 2, 500, 3, spread, offset)
+    for i, t in zip((0, 2), ops.kv4_values(cache, int32([500, 333]))):
+        want = decoded(cache[i], cache[i + 1]).transpose(1, 2).cpu().numpy().astype(np.float16)
+        got = t.cpu().numpy()
+        assert np.array_equal(got[0], want[0]) and np.array_equal(got[1, :333], want[1, :333])
+    ops.device_status()
