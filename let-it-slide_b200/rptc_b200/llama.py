@@ -590,7 +590,7 @@ class RPTCLlama:
         """`prefill` for prompts of different lengths: prompts[r] (whole numbers, at least one) goes into row r from position 0 on.  All tokens go
         through the network packed, one prompt behind the other (`ops.attn_prompt`), so that nothing is padded.  Returns the logits behind each
         prompt's last token, fp16 [rows, vocab]; `pos` is set to the lengths and `ids` to the greedy choices; decoding continues with `step`.
-        What is refused (ValueError) leaves the rows as they are."""
+        The prompts' tokens attend over each other's keys and values as they are; a 4-bit cache rounds them for what comes behind.  What is refused (ValueError) leaves the rows as they are."""
         prompts = self._accepted(prompts, [0] * self.rows)
         self.reset()
         return self._greedy(self._push(prompts, whole=False))
@@ -605,7 +605,8 @@ class RPTCLlama:
     def score(self, prompts: list[torch.Tensor], top: int = 0) -> list[tuple]:
         """How probable the model finds given texts: for each prompt (any number of them) (logprob, entropy, top_logprobs, top_ids), entry t about token
         t + 1 given the tokens up to t (`ops.token_logprobs`; one entry less than tokens).  The perplexity of a text is exp of minus the mean of
-        logprob.  Uses the rows' caches: the model is reset before and after.  What is refused (ValueError) leaves the rows as they are."""
+        logprob.  Every text is one pass, whose tokens attend over its keys and values as they are, before a 4-bit cache rounds them.  Uses the rows' caches: the
+        model is reset before and after.  What is refused (ValueError) leaves the rows as they are."""
         if not 0 <= top <= min(32, self.cfg.vocab):
             raise ValueError(f"top must be between 0 and {min(32, self.cfg.vocab)}, got {top}")
         groups = [self._accepted(prompts[p0:p0 + self.rows], [0] * self.rows, fewer=True) for p0 in range(0, len(prompts), self.rows)]
@@ -617,8 +618,9 @@ class RPTCLlama:
                 targets = torch.cat([torch.cat((p[1:], p.new_full((1,), -1))) for p in group])
                 xn, outs = torch.empty_like(h), []
                 ops.rmsnorm(h, self.norm_f, xn, self.cfg.rms_eps)
-                for t0 in range(0, len(targets), 4096):          # the logits of so many tokens at a time
-                    outs.append(ops.token_logprobs(xn[t0:t0 + 4096] @ self.head.t(), targets[t0:t0 + 4096], top))
+                for t0 in range(0, len(targets), 2048):          # the logits of so many tokens at a time, as the product's 32-bit sums leave them
+                    logits = torch.mm(xn[t0:t0 + 2048], self.head.t(), out_dtype=torch.float32)
+                    outs.append(ops.token_logprobs(logits, targets[t0:t0 + 2048], top))
                 columns = [torch.cat(c).split([len(p) for p in group]) for c in zip(*outs)]
                 found += [tuple(c[i][:-1] for c in columns) for i in range(len(group))]
         finally:
