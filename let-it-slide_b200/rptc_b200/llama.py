@@ -563,10 +563,13 @@ class RPTCLlama:
         h = self.embed[tokens.long()].reshape(R * T, cfg.hidden)                     # fp16 residual stream
         D = cfg.head_dim
         heads_of_128 = D == 128 and self.blocks[0].qkv.block_out == 128
-        angles = ops.rope_angles(T, cfg.rope_theta, h.device) if heads_of_128 else None
+        angles = None                                # for the layers whose output side is prompt_qkv's
 
         def attend(i, b, qkv, finished):
+            nonlocal angles
             if not finished and heads_of_128:
+                if angles is None:
+                    angles = ops.rope_angles(T, cfg.rope_theta, h.device)
                 ops.prompt_qkv(qkv, b.qkv.signs_out, b.qkv.scale, R, T, self.kcache[i], self.vcache[i], self.heads_l, self.kv_heads_l, angles)
             else:
                 qkv = qkv if finished else b.qkv.finish_t(qkv)
