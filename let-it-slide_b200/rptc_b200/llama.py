@@ -641,6 +641,8 @@ class RPTCLlama:
         if cfg.head_dim != 128:
             raise ValueError("packed prompts need heads of 128")
         ends = [b + p.numel() for b, p in zip(held, prompts)]
+        if min(held) < 0:
+            raise ValueError(f"row {held.index(min(held))} is at position {min(held)}: there is nothing to go on behind")
         if max(ends) > cfg.max_pos:
             raise ValueError(f"row {ends.index(max(ends))} would have {max(ends)} positions, but the KV caches hold max_pos = {cfg.max_pos}")
         prompts = [p.long() for p in prompts]

@@ -97,3 +97,13 @@ def test_what_is_accepted():
             call([T(1)])
     m = engine([4, 4])
     assert m.score([]) == [] and m.pos.tolist() == [0, 0]
+
+
+def test_rows_in_front_of_the_first_position_are_not_extended():
+    """A token at position -1 belongs to no sequence: it would be left out without a word."""
+    m = engine([7, -1])
+    m._push = lambda *a, **kw: pytest.fail("a pass behind no position")
+    before = state(m)
+    with pytest.raises(ValueError):
+        m.extend([T(1), T(2, 3)])
+    assert state(m) == before
