@@ -15,7 +15,7 @@
 // Weights refer to a running maximum of s + log2(a tile's largest scale): the products p * scale then fit fp16 whatever the scales are (2^11 where the reference was set, and
 // it moves only when they may pass 2^15, which their sum shows: no maximum is looked for otherwise; what falls below 2^-14 is 2^-25 of the largest).
 // Bound: HBM (160 bytes per position and kv head) with the issue slots close behind, about 350 warp instructions per 16 positions: four rows in flight per scheduler at 128
-// registers leave a quarter of the slots empty.  32 rows of 500 to 32768 positions, 8 kv heads: 136 us, 5.0 TB/s; one row of 131072: 43.7 us, 3.8 TB/s; one of 200: 4.6 us.
+// registers leave a quarter of the slots empty (a round of 16 tiles is 2900 clocks, 163 thousand of the batch's 232 thousand; where the others go was not measured).  32 rows of 500 to 32768 positions, 8 kv heads: 136 us, 5.0 TB/s; one row of 131072: 43.7 us, 3.8 TB/s; one of 200: 4.6 us.
 // Long contexts: all tiles of all rows and heads, laid end to end, are cut into equal ranges, two to an SM, so that rows of different lengths balance; a range's
 // part of a row goes to the workspace (fp32) and a second kernel joins the parts.  A warp's ring goes on into the range's next item: its first tiles and its q are on their
 // way while the item before is finished (32 rows as above 160 us without, and with a join that looked at every row's heads instead of the ranges' ends).
@@ -510,7 +510,8 @@ __global__ void __launch_bounds__(32 * kKv4JoinWarps) attn_kv4_join_kernel(const
     __shared__ float4 sums[kKv4JoinWarps][32];
     __shared__ float2 ml[kKv4JoinWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // pos was there before the first kernel let this one start: where the parts lie is found while that one works.
+    // pos was there before the first kernel let this one start: where the parts lie is found before the wait.  (A block of the first kernel has all of its SM's registers, so that
+    // a CTA here starts when that block has ended, beside what other SMs still do.)
     const int32_t *pos = after_wait(p.pos);
     const int heads = p.hkv * p.blocks;
     const Kv4Cut cut = kv4_cut(p, pos, most_ctas, lane);
@@ -571,7 +572,9 @@ __global__ void __launch_bounds__(32 * kKv4JoinWarps) attn_kv4_join_kernel(const
 using namespace rptc;
 
 // A CTA per row and head, or ranges.  Measured on full caches of 8 kv heads: 1024 positions 9.1 against 9.9 us (one row), 9.3 and 16.7 (16), 51 and 87 (148); 2048 positions
-// 13.8 against 10.3 (one row), 14.0 and 13.8 (4), 13.9 and 20.8 (16), 83 and 95 (148).  Longer ones go by ranges whatever the rows are, as those may differ in length.
+// 13.8 against 10.3 (one row), 14.0 and 13.8 (4), 13.9 and 20.8 (16), 83 and 95 (148).  Longer ones go by ranges whatever the rows are, as those may differ in length; what a long cache
+// that holds little costs by that (64 heads over 8; a cache of about its contents, and one of 32768): 200 positions 5.3 and 9.2 us (one row), 5.6 and 13.6 (16), 8.0 and 18.3 (32); 2000
+// positions 10.8 and 10.8, 14.2 and 22.0, 23.2 and 33.7.
 static bool kv4_whole(const rptc_kv_cache &c, int heads) {
     const int64_t items = (int64_t)c.rows * c.kv_heads * ((heads / c.kv_heads + 7) / 8);
     return c.max_pos <= 1024 || (c.max_pos <= 2048 && 4 * items >= num_sms());
@@ -628,7 +631,7 @@ extern "C" int rptc_attn_decode_kv4(const void *q, int64_t ld_q, const int32_t *
     static SmemOptIn opted;
     if (int e = allow_max_smem(attn_kv4_kernel<false>, opted)) return e;
     if (int e = launch(attn_kv4_kernel<false>, dim3((unsigned)ctas), dim3(2 * 32 * kKv4Warps), 2 * kKv4Smem, s, p)) return e;
-    // the second kernel starts early and waits for the first one's sums itself
+    // the second kernel starts as SMs come free and waits for the first one's sums itself
     const bool before = pdl_enabled();
     rptc_set_pdl(1);
     const int64_t items = (int64_t)p.rows * p.hkv * p.blocks;

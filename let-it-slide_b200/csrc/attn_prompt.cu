@@ -6,7 +6,7 @@
 // 256 / pack tokens, so that grouped heads of a short prompt fill the tensor core's 128 rows and share the keys' tiles.  A CTA takes items one after
 // the other.  For each tile of 128 keys and each half:
 //   S = Q K^T            tcgen05.mma from shared memory into tensor memory (fp32)
-//   P = exp2(S - m)      a softmax thread owns a row: it reads its 128 scores, keeps the running maximum m and sum l in registers, and puts P back over S in
+//   P = exp2(S - m)      a softmax thread owns a row: it reads its 128 scores, keeps the running maximum m and sum l in registers (as Milakov and Gimelshein, 2018), and puts P back over S in
 //                        16 bits (the one rounding besides the result's: the tensor core multiplies 16-bit operands; l adds the weights up before it)
 //   O += P V             tcgen05.mma with P in tensor memory, V in shared memory as it lies (N-major), O in tensor memory (fp32)
 // The two halves alternate: the tensor core works on one while the other's softmax runs.  m follows the true maximum with a slack of 2^8: only a larger step
@@ -18,11 +18,13 @@
 // lies there has to be 0.
 // Items go to CTAs longest first, there and back again (the longest of a round meets the shortest of the next): the order is worked out from
 // `starts` on the device, by counting items of at least a number of tiles.
-// Bound: the exponentials.  A tile of 128 keys and 256 rows takes 2770 to 3000 clocks: 2048 for its 32768 exponentials on the special-function unit (busy 69 % of the time at
-// 8192 tokens, as is the tensor pipe), 1024 for its products, the rest the softmax warps' other work.  One prompt of 2048 tokens, 32 heads of 128: 37.6 us (fp16, 0.91 PFLOP/s);
-// one of 8192, 64 heads over 8: 845 us (1.30 PFLOP/s, at the power cap).  A short prompt pays for its set-up too: first scores after some 7000 clocks, the last result 2200 after
-// the last product; 24 tokens take 6.6 us.  Sixteen sequences of 1 to 1021 tokens, 64 heads over 8, with `pack` heads together
-// 77 us; when they took 80, one head at a time took 112.
+// Bound: exponentials and products evenly.  A tile of 128 keys and 256 rows takes 2770 to 3000 clocks: 2048 for its 32768 exponentials on the special-function unit, 2048 for its
+// products on the tensor core (each busy 69 % of the time at 8192 tokens), which overlap but for a half's softmax that waits for its own product and next scores, and the softmax warps'
+// other work.  How long a clock is, power decides: one prompt of 8192 tokens, 64 heads over 8 of 128, fp16, is 1.32 million clocks; ten calls in a row take 845 us each (1.30 PFLOP/s), a
+// second of them 965 to 980 (1.45 GHz at the power cap), and queries of zeros 746.  One of 2048 tokens, 32 heads: 64 thousand clocks, 16 tiles of them 47, the set-up (first scores) 7,
+// the last result 2; 36 to 38 us.  24 tokens: 6.6 us.  Heads of 64, whose products are half as long and whose exponentials are not: 32 us for 2048 tokens of 32 heads, 675 for 8192 of 64
+// over 8.  Sixteen sequences of 1 to 1021 tokens, 64 heads over 8, with `pack` heads together 77 us; when they took 80, one head at a time took 112.  They are 1072 items: a CTA has
+// seven, whose starts and ends do not overlap, and at most 37 tiles where the mean is 31, so that an SM has work for 123 of the 145 thousand clocks.
 #include <cuda_bf16.h>
 
 #include "tc_ptx.cuh"

@@ -3,8 +3,8 @@
 //
 //   y = rope(scale signs H x) per head of 128;   a group of 32 values of k or v: scale = (max - min) / 15, code = round((value - min) / scale), in fp32
 //
-// Bound: HBM by bytes; in fact the issue slots and the SM's load and store pipe, each some 60 % busy: 2048 tokens of 96 heads 30 us where the traffic is 17; 16 tokens
-// 2.5 us, a launch.  The values of a cache: 8.1 us for 2048 positions of 32 kv heads, its traffic 6.7.
+// Bound: HBM by bytes; in fact the issue slots and the SM's load and store pipe, each some 60 % busy: 2048 tokens of 96 heads 30 us where the traffic is 17 (29 to 31 without the transform
+// and into an fp16 cache); 16 tokens 2.5 to 3.0 us, a launch.  The values of a cache: 8.1 us for 2048 positions of 32 kv heads, its traffic 6.7.
 #include <type_traits>
 
 #include "fwht.cuh"
@@ -369,7 +369,8 @@ static int launch_append(const AppendParams &p, int bits, cudaStream_t s) {
     return bits == 4 ? launch(qkv_append_kernel<F32, TRANSFORM, 4>, grid, dim3(256), 0, s, p) : launch(qkv_append_kernel<F32, TRANSFORM, 16>, grid, dim3(256), 0, s, p);
 }
 
-// Eight lanes take a position of one kv head: a lane's eight bytes of codes are four values of each group.
+// Eight lanes take a position of one kv head: a lane's eight bytes of codes are four values of each group.  There are CTAs for all positions of the rows, whatever they hold: 100 positions
+// of 32 rows and 8 kv heads take 4.5 us in a cache of 128, 18 in one of 1024, 544 in one of 32768.
 __global__ void __launch_bounds__(256) kv4_values_kernel(const uint8_t *__restrict__ k, const __half2 *__restrict__ k_scales, const uint8_t *__restrict__ v,
                                                          const __half2 *__restrict__ v_scales, const int32_t *__restrict__ count, __half *__restrict__ k_out,
                                                          __half *__restrict__ v_out, int max_pos, int hkv, unsigned int *status) {
