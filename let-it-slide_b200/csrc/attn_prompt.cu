@@ -22,7 +22,7 @@
 // products on the tensor core (each busy 69 % of the time at 8192 tokens), which overlap but for a half's softmax that waits for its own product and next scores, and the softmax warps'
 // other work.  How long a clock is, power decides: one prompt of 8192 tokens, 64 heads over 8 of 128, fp16, is 1.32 million clocks; ten calls in a row take 845 us each (1.30 PFLOP/s), a
 // second of them 965 to 980 (1.45 GHz at the power cap), and queries of zeros 746.  One of 2048 tokens, 32 heads: 64 thousand clocks, 16 tiles of them 47, the set-up (first scores) 7,
-// the last result 2; 36 to 38 us.  24 tokens: 6.6 us.  Heads of 64, whose products are half as long and whose exponentials are not: 32 us for 2048 tokens of 32 heads, 675 for 8192 of 64
+// the last result 2; 36 to 38 us.  24 tokens: 6.6 to 7.1 us.  Heads of 64, whose products are half as long and whose exponentials are not: 32 us for 2048 tokens of 32 heads, 675 for 8192 of 64
 // over 8.  Sixteen sequences of 1 to 1021 tokens, 64 heads over 8, with `pack` heads together 77 us; when they took 80, one head at a time took 112.  They are 1072 items: a CTA has
 // seven, whose starts and ends do not overlap, and at most 37 tiles where the mean is 31, so that an SM has work for 123 of the 145 thousand clocks.
 #include <cuda_bf16.h>
